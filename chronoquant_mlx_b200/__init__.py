@@ -18,6 +18,8 @@ from .patch import (
 from .attention import chronoquant_sdpa
 from .graph import DecodeGraph
 from .prompt_cache import load_prompt_cache, save_prompt_cache
+from .rope import qk_norm_rope
+from .sparse import BlockIndex, chronoquant_sparse_sdpa
 
 __all__ = [
     "ChronoQuantCache",
@@ -30,4 +32,7 @@ __all__ = [
     "DecodeGraph",
     "save_prompt_cache",
     "load_prompt_cache",
+    "BlockIndex",
+    "chronoquant_sparse_sdpa",
+    "qk_norm_rope",
 ]

@@ -36,6 +36,8 @@ EXPORTED = [
     "cq_append_at", "cq_attention_at", "cq_decode_step_at", "cq_prefill_prepare", "cq_prefill_attend",
     "cq_rmsnorm", "cq_qk_norm_rope", "cq_silu_mul", "cq_peer_sum_norm", "cq_peer_region_bytes",
     "cq_peer_region_alloc", "cq_peer_region_open", "cq_peer_region_close", "cq_peer_region_free",
+    "cq_qk_norm_rope_rows", "cq_block_bounds", "cq_block_bounds_at", "cq_block_bounds_read", "cq_block_select",
+    "cq_block_select_workspace", "cq_sparse_attention", "cq_sparse_attention_workspace",
 ]
 
 
@@ -113,6 +115,17 @@ def _declare(lib):
         "cq_peer_region_open": [P, ctypes.POINTER(P)],
         "cq_peer_region_close": [P],
         "cq_peer_region_free": [P],
+        "cq_qk_norm_rope_rows": [P, I64, I64, I32, I32, I32, I32, I32, I32, I32, P, P, P, P, I64, I64, F, P, P,
+                                 ctypes.c_int, P],
+        "cq_block_bounds": [C, I64, I64, I32, P, P, I64, P],
+        "cq_block_bounds_at": [C, P, I64, I32, I32, P, P, I64, P],
+        "cq_block_bounds_read": [P, P, I64, I64, I64, I64, I32, P, P],
+        "cq_block_select": [P, P, I64, I32, I32, I32, I32, I64, P, P, ctypes.c_int, I32, I32, I64, I64, I64, P, I32,
+                            I32, I32, P, P, P, SZ, P],
+        "cq_block_select_workspace": [I32, I32, I32, I64, I32, ctypes.POINTER(SZ)],
+        "cq_sparse_attention": [C, I64, P, P, ctypes.c_int, I32, I32, I64, I64, I64, F, P, P, I32, I32, P,
+                                ctypes.c_int, P, P, SZ, P],
+        "cq_sparse_attention_workspace": [C, I64, I32, I32, I32, I32, ctypes.POINTER(SZ)],
     }
     for name, args in sig.items():
         fn = getattr(lib, name)

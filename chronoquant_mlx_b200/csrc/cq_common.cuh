@@ -189,6 +189,7 @@ int read_bounds_error_layout(int clear);
 int read_bounds_error_attention(int clear);
 int read_bounds_error_prefill(int clear);
 int read_bounds_error_decode(int clear);
+int read_bounds_error_sparse(int clear);
 
 // Locations of token t (absolute) of (b, h) in component comp.
 struct TokLoc {

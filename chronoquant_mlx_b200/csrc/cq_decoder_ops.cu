@@ -7,8 +7,11 @@
 //                     (q and k), then rotate-half RoPE at one position;
 //                     q, k, v written as contiguous [B][H][D]
 //   cq_silu_mul       y = bf16(silu(g)) * u                          (SwiGLU)
+//   cq_qk_norm_rope_rows  the head norm and rotation for any number of tokens,
+//                     each at its own position (prompts, ragged batches), q and
+//                     k written head-major [B][H][S][D]
 //
-// Each keeps the rounding points of the equivalent torch expression in
+// The first three keep the rounding points of the equivalent torch expression in
 // bf16/fp16: products in fp32, one rounding to the tensor dtype after each
 // torch op.  Only the order of the fp32 sum of squares differs from torch's
 // reduction, so a value can land one dtype ulp away.
@@ -97,6 +100,84 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const void *qkv, int6
   for (int i = 0; i < 4; ++i) store_from_float(o, dst + i, out[i], dt);
 }
 
+// Head norm and rotation of many tokens: one CTA per token, a warp per head in
+// turn.  The angle of a channel pair is pos * inv_freq in fp64 (a product of
+// two fp32 numbers is off by radians at far positions), reduced to
+// [-pi, pi] there; its sine and cosine are shared by the token's heads.  All
+// arithmetic is fp32 with one rounding to the tensor type at the end.
+struct RopeArgs {
+  const void *qkv;
+  int64_t sb, ss;        // element strides of a sequence and a token
+  int B, S, Hq, Hkv, D, rot, adjacent;
+  const void *wq, *wk;   // both null: rotation only
+  const float *inv_freq;
+  const int64_t *pos;
+  int64_t p_sb, p_ss;
+  float eps;
+  void *q_out, *k_out;
+};
+
+constexpr int kRopeWarps = 8;
+
+template <int DT>
+__global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_rows_kernel(RopeArgs A) {
+  __shared__ float2 s_cs[128];              // (cos, sin) of each pair
+  __shared__ float s_x[kRopeWarps][256];    // a head's normalised channels
+  const int64_t tok = blockIdx.x;
+  const int b = (int)(tok / A.S), s = (int)(tok - (int64_t)b * A.S);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int half = A.rot / 2, D = A.D, H = A.Hq + A.Hkv;
+  for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    const double ang = (double)A.pos[b * A.p_sb + s * A.p_ss] * (double)A.inv_freq[i];
+    // 2 pi as the sum of two doubles: the remainder keeps its digits for any angle below 2^53 turns
+    const double hi = 6.283185307179586, lo = 2.4492935982947064e-16;
+    const double n = rint(ang / hi);
+    const float r = (float)fma(-n, lo, fma(-n, hi, ang));
+    float sn, cs;
+    sincosf(r, &sn, &cs);
+    s_cs[i] = make_float2(cs, sn);
+  }
+  __syncthreads();
+  float *x = s_x[warp];
+  for (int h = warp; h < H; h += kRopeWarps) {
+    const int64_t src = b * A.sb + s * A.ss + (int64_t)h * D;
+    const void *w = h < A.Hq ? A.wq : A.wk;
+    float v[8], sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = lane + 32 * k;
+      v[k] = d < D ? load_as_float(A.qkv, src + d, DT) : 0.f;
+      sq = fmaf(v[k], v[k], sq);
+    }
+    const float r = w ? rsqrtf(warp_sum(sq) / (float)D + A.eps) : 1.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = lane + 32 * k;
+      if (d < D) x[d] = w ? v[k] * r * load_as_float(w, d, DT) : v[k];
+    }
+    __syncwarp();
+    const bool is_q = h < A.Hq;
+    void *out = is_q ? A.q_out : A.k_out;
+    const int64_t dst = is_q ? (((int64_t)b * A.Hq + h) * A.S + s) * D
+                             : (((int64_t)b * A.Hkv + (h - A.Hq)) * A.S + s) * D;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int d = lane + 32 * k;
+      if (d >= D) continue;
+      float y = x[d];
+      if (d < A.rot) {
+        const int i = A.adjacent ? d >> 1 : (d < half ? d : d - half);
+        const bool second = A.adjacent ? (d & 1) : d >= half;
+        const float o = x[A.adjacent ? d ^ 1 : (second ? d - half : d + half)];
+        const float2 cs = s_cs[i];
+        y = second ? fmaf(y, cs.x, o * cs.y) : fmaf(y, cs.x, -o * cs.y);
+      }
+      store_from_float(out, dst + d, y, DT);
+    }
+    __syncwarp();
+  }
+}
+
 // gu: [rows][2*ffn] (gate | up); y: [rows][ffn]
 __global__ void silu_mul_kernel(const void *gu, void *y, int64_t rows, int ffn, int dt) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -146,4 +227,33 @@ extern "C" int cq_silu_mul(const void *gu, void *y, int64_t rows, int32_t ffn, i
   CQ_REQUIRE((n + 255) / 256 < (1LL << 31), CQ_ERR_INVALID, "cq_silu_mul: too large");
   dec::silu_mul_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>(gu, y, rows, ffn, dtype);
   return check_launch("cq_silu_mul");
+}
+
+extern "C" int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t row_stride, int32_t batch,
+                                    int32_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                                    int32_t rot_dim, int32_t adjacent, const void *q_norm_w, const void *k_norm_w,
+                                    const float *inv_freq, const int64_t *pos, int64_t pos_sb, int64_t pos_ss,
+                                    float eps, void *q_out, void *k_out, int dtype, void *stream) {
+  CQ_REQUIRE((q_norm_w == nullptr) == (k_norm_w == nullptr), CQ_ERR_INVALID,
+             "cq_qk_norm_rope_rows: give both norm weights or neither");
+  CQ_REQUIRE(batch >= 0 && tokens >= 0 && n_q_heads >= 1 && n_kv_heads >= 1, CQ_ERR_INVALID,
+             "cq_qk_norm_rope_rows: bad sizes");
+  CQ_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, CQ_ERR_UNSUPPORTED,
+             "cq_qk_norm_rope_rows: head_dim must be a multiple of 8 in [8, 256]");
+  CQ_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, CQ_ERR_INVALID,
+             "cq_qk_norm_rope_rows: rot_dim must be even and at most head_dim");
+  CQ_REQUIRE(dtype == CQ_F16 || dtype == CQ_BF16 || dtype == CQ_F32, CQ_ERR_UNSUPPORTED,
+             "cq_qk_norm_rope_rows: dtype must be f16, bf16 or f32");
+  const int64_t n = (int64_t)batch * tokens;
+  if (n == 0) return CQ_OK;
+  CQ_REQUIRE(n < (1LL << 31), CQ_ERR_INVALID, "cq_qk_norm_rope_rows: too many tokens");
+  CQ_REQUIRE(qkv && q_out && k_out, CQ_ERR_INVALID, "cq_qk_norm_rope_rows: null pointer");
+  CQ_REQUIRE(rot_dim == 0 || (inv_freq && pos), CQ_ERR_INVALID, "cq_qk_norm_rope_rows: inv_freq or pos is null");
+  const dec::RopeArgs A{qkv,      seq_stride, row_stride, batch, tokens, n_q_heads, n_kv_heads, head_dim, rot_dim, adjacent,
+                        q_norm_w, k_norm_w,   inv_freq,   pos,   pos_sb, pos_ss,    eps,        q_out,    k_out};
+  auto *fn = dtype == CQ_F16    ? dec::qk_norm_rope_rows_kernel<CQ_F16>
+             : dtype == CQ_BF16 ? dec::qk_norm_rope_rows_kernel<CQ_BF16>
+                                : dec::qk_norm_rope_rows_kernel<CQ_F32>;
+  fn<<<(unsigned)n, dec::kRopeWarps * 32, 0, (cudaStream_t)stream>>>(A);
+  return check_launch("cq_qk_norm_rope_rows");
 }

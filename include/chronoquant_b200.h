@@ -357,6 +357,84 @@ int cq_qk_norm_rope(const void *qkv, int64_t row_stride, int32_t batch, int32_t 
                     const int64_t *pos, float eps, void *q_out, void *k_out, void *v_out, int dtype, void *stream);
 int cq_silu_mul(const void *gu, void *y, int64_t rows, int32_t ffn, int dtype, void *stream);
 
+/* Head norm and rotation of many tokens (no reference counterpart).  qkv:
+ * fused rows of sequence b, token s at b*seq_stride + s*row_stride (elements),
+ * heads [q (n_q_heads) | k (n_kv_heads) | ...] of head_dim each (a multiple of
+ * 8, <= 256).  Per q and k head x: x * rsqrt(mean(x^2) + eps) * w (q_norm_w /
+ * k_norm_w [head_dim]; both NULL: no norm), then the first rot_dim channels
+ * are rotated by the angles pos[b*pos_sb + s*pos_ss] * inv_freq[i], i <
+ * rot_dim/2 (fp64 product; inv_freq fp32, pos int64): pairs (i, i +
+ * rot_dim/2), or (2i, 2i + 1) with adjacent != 0.  fp32 arithmetic, one
+ * rounding at the end.  q_out [batch][n_q_heads][tokens][head_dim], k_out
+ * [batch][n_kv_heads][tokens][head_dim], contiguous.  dtype CQ_F16, CQ_BF16 or
+ * CQ_F32 for qkv, weights and outputs. */
+int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t row_stride, int32_t batch, int32_t tokens,
+                         int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t rot_dim, int32_t adjacent,
+                         const void *q_norm_w, const void *k_norm_w, const float *inv_freq, const int64_t *pos,
+                         int64_t pos_sb, int64_t pos_ss, float eps, void *q_out, void *k_out, int dtype,
+                         void *stream);
+
+/* Sparse attention over blocks of cached tokens (no reference counterpart:
+ * the reference attends to every token).  Block j of a sequence is its tokens
+ * j*block_tokens .. (j+1)*block_tokens - 1.
+ *
+ * cq_block_bounds: for the blocks holding tokens t0 .. T-1, per (sequence,
+ * kv-head) and channel the range [lo, hi] of the decoded fp16 keys of the
+ * block's tokens (cq_reconstruct mode 0; NaN left out, values clamped to the
+ * finite fp16 range), as int8 codes with one fp32 scale s = max|.| / 126 per
+ * block: the largest lower code with code * s <= lo and the least upper code
+ * with code * s >= hi.  codes: [batch*kv_heads][max_blocks][2][head_dim] (lower,
+ * upper), scales: [batch*kv_heads][max_blocks].  cq_block_bounds_at: the blocks
+ * holding the last S tokens of the device-resident length len_dev[0] (at most
+ * max_len), for captured graphs.  cq_block_bounds_read: code * scale of blocks
+ * first .. first+n-1 of every unit, fp32 [units][n][2][head_dim].
+ *
+ * codes is 16-byte aligned in all of these. */
+int cq_block_bounds(const cq_paged_cache *cache, int64_t t0, int64_t T, int32_t block_tokens, int8_t *codes,
+                    float *scales, int64_t max_blocks, void *stream);
+int cq_block_bounds_at(const cq_paged_cache *cache, const int64_t *len_dev, int64_t max_len, int32_t S,
+                       int32_t block_tokens, int8_t *codes, float *scales, int64_t max_blocks, void *stream);
+int cq_block_bounds_read(const int8_t *codes, const float *scales, int64_t units, int64_t max_blocks, int64_t first,
+                         int64_t n, int32_t head_dim, float *out, void *stream);
+
+/* cq_block_select: for each query token i (at position T - q_len + i) and
+ * kv-head, up to `top` (<= 4096) of the blocks it may see -- those between its
+ * own and the one holding starts[b] (int64 [batch], the first real token of a
+ * left-padded sequence; NULL: 0) -- as an ascending int32 list blocks
+ * [batch][kv_heads][q_len][top], -1 behind.  The `first` lowest and `recent`
+ * highest visible blocks are always listed (first + recent <= top); the others
+ * by score, ties to the lower index.  Score of block j: the largest over the
+ * group's heads of (s_g * s_j) * dot, s_g = amax(q_g)/127, dot = sum_d max(q8_d
+ * lo_d, q8_d hi_d), q8 = rint(q * (127/amax)) (fp32 operations in this order;
+ * NaN queries count as 0, values are clamped to the finite fp16 range).
+ * block_scores (optional): fp32, the listed blocks' scores, -inf behind.  q as
+ * in cq_attention.  T: tokens summarised; with len_dev (may be NULL) the
+ * length is read from device memory and T is the largest it may be.
+ * workspace: cq_block_select_workspace bytes, contents ignored. */
+int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t q_len, int64_t T, int32_t block_tokens,
+                              size_t *bytes);
+int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens, int32_t batch,
+                    int32_t kv_heads, int32_t head_dim, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
+                    int32_t n_q_heads, int32_t q_len, int64_t q_sb, int64_t q_sh, int64_t q_sq, const int64_t *starts,
+                    int32_t first, int32_t recent, int32_t top, int32_t *blocks, float *block_scores, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* cq_sparse_attention: attention of q_len queries per sequence, query i at
+ * position T - q_len + i, over the tokens of its kv-head's listed blocks that
+ * are neither behind it nor before starts[b].  blocks: int32
+ * [batch][kv_heads][q_len][top] ascending; an entry that is negative or not
+ * above the one before it is left out, and blocks behind the query hold no
+ * token it sees.  A query that sees no token gets zeros (log-sum-exp -inf).
+ * q, scale, out, lse_out, T and len_dev as in cq_attention and
+ * cq_block_select; a device-resident length outside [q_len, T] gives zeros and
+ * sets cq_device_error (4). */
+int cq_sparse_attention_workspace(const cq_paged_cache *cache, int64_t T, int32_t n_q_heads, int32_t q_len,
+                                  int32_t top, int32_t block_tokens, size_t *bytes);
+int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
+                        int32_t n_q_heads, int32_t q_len, int64_t q_sb, int64_t q_sh, int64_t q_sq, float scale,
+                        const int64_t *starts, const int32_t *blocks, int32_t top, int32_t block_tokens, void *out,
+                        int out_dtype, float *lse_out, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,626 @@
+"""Block index, block selection and sparse attention over the compressed cache.
+
+Every operator is compared with a plain 64-bit implementation on the cache's
+own saved state (``cache.state``: the reference layout).
+
+Bars.  Bounds and block lists are whole numbers and fp32 products in a fixed
+order: equal.  Attention: the decode kernel rounds P to fp16 (2^-11 relative),
+P * scale to fp16, the per-anchor sums of P to fp16 and the denominator is a
+sum of the rounded P, so with sum p = 1 the output is within 5 * 2^-11 * max|v|
+of the exact one (fp32 score errors of ~1e-5 are inside that), plus half a step
+of the output type; the log-sum-exp within 2^-10."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from chronoquant_mlx_b200 import BlockIndex, ChronoQuantCache, _lib, chronoquant_sdpa, chronoquant_sparse_sdpa
+
+gpu = pytest.mark.gpu
+
+
+def make_cache(B, H, T, D, seed=0, dtype=torch.float16, step=None, **kw):
+    """A cache of AR(1) keys and values with a few strong key channels."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    k = torch.randn((B, H, T, D), generator=g, device="cuda")
+    v = torch.randn((B, H, T, D), generator=g, device="cuda")
+    drift = torch.randn((B, H, -(-T // 16), D), generator=g, device="cuda").repeat_interleave(16, 2)[:, :, :T]
+    k = 0.35 * k + drift + 2 * torch.randn((1, H, 1, D), generator=g, device="cuda")
+    v = 0.3 * v + drift
+    cache = ChronoQuantCache(**kw)
+    k, v = k.to(dtype), v.to(dtype)
+    for a in range(0, T, step or T):
+        b = min(T, a + (step or T))
+        cache.update_and_fetch(k[:, :, a:b], v[:, :, a:b])
+    return cache
+
+
+def decoded(cache, fp16_keys=False):
+    """K and V in 64 bits from the saved state: anchor + code * scale (or the
+    keys as reconstruct_history rounds them)."""
+    st = cache.state
+    kf, packed, scales = [st[0], st[1]], [], []
+    rest = st[2:]
+    i = 0
+    out = []
+    T = cache.offset
+    for c, s in enumerate((cache.stride_k, cache.stride_v)):
+        t = torch.arange(T, device="cuda")
+        a = t // s
+        x = kf[c][:, :, a].double()
+        if T > kf[c].shape[2]:
+            pk, sc = rest[i], rest[i + 1]
+            i += 2
+            w = pk.view(torch.int32).unsqueeze(-1)
+            code = (((w >> torch.arange(0, 32, 4, device="cuda", dtype=torch.int32)) & 15) - 8).flatten(-2)
+            code = code[..., :x.shape[-1]].double()
+            pf = (t - a - 1).clamp(min=0)
+            r = (code * sc.double().unsqueeze(-1))[:, :, pf]
+            if fp16_keys and c == 0:
+                y = (x + r.half().double()).half().double()
+            else:
+                y = x + r
+            x = torch.where((t % s == 0)[:, None], x, y)
+        out.append(x)
+    return out
+
+
+def ref_bounds(keys, bt):
+    """(codes int [B, H, n, 2, D], scales fp32 [B, H, n]) of fp16-valued keys."""
+    B, H, T, D = keys.shape
+    lo, hi = [], []
+    for a in range(0, T, bt):
+        x = keys[:, :, a:a + bt]
+        lo.append(torch.where(x.isnan(), math.inf, x).amin(2))
+        hi.append(torch.where(x.isnan(), -math.inf, x).amax(2))
+    lo, hi = torch.stack(lo, 2), torch.stack(hi, 2)
+    none = lo > hi
+    lo = torch.where(none, 0.0, lo).clamp(-65504, 65504)
+    hi = torch.where(none, 0.0, hi).clamp(-65504, 65504)
+    s = (torch.maximum(lo.abs(), hi.abs()).amax(-1).float() / torch.full((), 126.0, device=keys.device)).double()
+    d = torch.where(s > 0, s, 1.0).unsqueeze(-1)
+    return torch.stack((torch.floor(lo / d), torch.ceil(hi / d)), 3), s.float()
+
+
+def ref_select(codes, scales, q, T, bt, top, first, recent, starts=None):
+    """Lists and scores by the definition, one row at a time."""
+    B, Hq, S, D = q.shape
+    H = codes.shape[1]
+    G = Hq // H
+    x = torch.nan_to_num(q.float(), nan=0.0, posinf=65504.0, neginf=-65504.0).clamp(-65504, 65504)
+    amax = x.abs().amax(-1, keepdim=True)
+    zero = amax < 1e-30
+    r = torch.full_like(amax, 127.0) / torch.where(zero, 1.0, amax)
+    q8 = torch.where(zero, 0.0, torch.round(x * r)).double().view(B, H, G, S, D)
+    sg = torch.where(zero, 0.0, amax / torch.full_like(amax, 127.0)).view(B, H, G, S)
+    lists = torch.full((B, H, S, top), -1, dtype=torch.int32)
+    out = torch.full((B, H, S, top), -math.inf)
+    for b in range(B):
+        st = 0 if starts is None else max(0, int(starts[b]))
+        for h in range(H):
+            dot = (q8[b, h].clamp(min=0) @ codes[b, h, :, 1].T + q8[b, h].clamp(max=0) @ codes[b, h, :, 0].T).float()
+            score = (sg[b, h].unsqueeze(-1) * scales[b, h]).float() * dot
+            score = score.amax(0).cpu()  # [S, n]
+            for i in range(S):
+                p = T - S + i
+                if st > p:
+                    continue
+                fb, lb = st // bt, p // bt
+                seen = list(range(fb, lb + 1))
+                forced = {j for j in seen if j < fb + first or j > lb - recent}
+                order = sorted(seen, key=lambda j: (j not in forced, -float(score[i, j]) if j not in forced else 0.0, j))
+                got = sorted(order[:top])
+                lists[b, h, i, :len(got)] = torch.tensor(got, dtype=torch.int32)
+                out[b, h, i, :len(got)] = score[i, got]
+    return lists, out
+
+
+def ref_sparse(K, V, q, scale, blocks, bt, starts=None):
+    """64-bit attention over the listed blocks; (out, lse, max|v| per row)."""
+    B, Hq, S, D = q.shape
+    H, T = K.shape[1], K.shape[2]
+    G = Hq // H
+    qs = (q * torch.tensor(scale, dtype=q.dtype, device=q.device)).double()
+    out = torch.zeros((B, Hq, S, D), dtype=torch.float64, device=q.device)
+    lse = torch.full((B, Hq, S), -math.inf, dtype=torch.float64, device=q.device)
+    vmax = torch.zeros((B, Hq, S, 1), dtype=torch.float64, device=q.device)
+    lists = blocks.cpu()
+    for b in range(B):
+        st = 0 if starts is None else max(0, int(starts[b]))
+        for h in range(H):
+            for i in range(S):
+                row = lists[b, h, i].tolist()
+                keep = [j for n, j in enumerate(row) if j >= 0 and (n == 0 or j > row[n - 1])]
+                t = [x for j in keep for x in range(max(st, j * bt), min(T - S + i + 1, (j + 1) * bt))]
+                if not t:
+                    continue
+                t = torch.tensor(t, device=q.device)
+                w = qs[b, h * G:(h + 1) * G, i] @ K[b, h, t].T
+                lse[b, h * G:(h + 1) * G, i] = torch.logsumexp(w, -1)
+                out[b, h * G:(h + 1) * G, i] = torch.softmax(w, -1) @ V[b, h, t]
+                vmax[b, h * G:(h + 1) * G, i] = V[b, h, t].abs().max()
+    return out, lse, vmax
+
+
+def check_attention(got, ref, vmax):
+    half = torch.finfo(got.dtype).eps / 2
+    err = (got.double() - ref).abs()
+    assert torch.isfinite(got).all()
+    tol = 5 * 2.0 ** -11 * vmax + half * ref.abs() + 1e-12
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+def queries(B, Hq, S, D, dtype, seed=5, amp=1.3):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (amp * torch.randn((B, Hq, S, D), generator=g, device="cuda")).to(dtype)
+
+
+# ----------------------------------------------------------------------------- bounds
+@gpu
+@pytest.mark.parametrize("T,bt", [(1, 16), (15, 16), (64, 64), (65, 64), (333, 64), (700, 128), (1000, 48)])
+@pytest.mark.parametrize("kw", [dict(), dict(stride_k=64, stride_v=32, delta_bits_v=3), dict(stride_k=1, stride_v=1),
+                                dict(stride_k=12, stride_v=4)])
+def test_bounds_equal_definition(T, bt, kw):
+    cache = make_cache(2, 3, T, 128, seed=T, **kw)
+    index = BlockIndex(cache, bt).update()
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], bt)
+    n = -(-T // bt)
+    assert index.n_blocks == n and index.covered == T
+    assert torch.equal(index.codes[:, :, :n].double(), codes)
+    assert torch.equal(index.scales[:, :, :n], scales)
+    assert torch.equal(index.bounds(), codes.float() * scales[..., None, None])
+    assert torch.equal(index.bounds(n - 1), (codes.float() * scales[..., None, None])[:, :, n - 1:])
+    x = cache.reconstruct_history()[0].double()  # the ranges hold every decoded key
+    t = torch.arange(T, device="cuda") // bt
+    lo, hi = codes[:, :, :, 0] * scales.double()[..., None], codes[:, :, :, 1] * scales.double()[..., None]
+    assert (lo[:, :, t] <= x).all() and (x <= hi[:, :, t]).all()
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 64, 72, 256])
+def test_bounds_head_dims(D):
+    cache = make_cache(1, 2, 200, D, seed=D)
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 32)
+    index = BlockIndex(cache, 32).update()
+    assert torch.equal(index.codes[:, :, :7].double(), codes) and torch.equal(index.scales[:, :, :7], scales)
+
+
+@gpu
+def test_bounds_follow_the_cache():
+    """Updates after appends of 1 .. 100 tokens (across page and pool growth)
+    leave the same ranges as one pass over everything; untouched blocks keep
+    their bytes, rows behind the last block stay as they were."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache = ChronoQuantCache(stride_k=32, stride_v=8)
+    index, T = BlockIndex(cache, 64), 0
+    for n in (1, 1, 62, 1, 100, 37, 1, 300, 64, 9):
+        cache.update_and_fetch(*(torch.randn((2, 2, n, 128), generator=g, device="cuda").half() for _ in range(2)))
+        T += n
+        index.update()
+        assert index.covered == T
+        whole = BlockIndex(cache, 64).update()
+        m = index.n_blocks
+        assert torch.equal(index.codes[:, :, :m], whole.codes[:, :, :m])
+        assert torch.equal(index.scales[:, :, :m], whole.scales[:, :, :m])
+        assert not index.codes[:, :, m:].any() and not index.scales[:, :, m:].any()
+    before = index.codes.clone()
+    index.update(T - 1)  # recomputing the last block changes nothing
+    assert torch.equal(index.codes, before)
+    other = make_cache(2, 2, 100, 128, seed=9)
+    cache.state = other.state  # a restored state is another store: the index starts again
+    index.update()
+    assert index.covered == 100
+    assert torch.equal(index.codes[:, :, :2], BlockIndex(other, 64).update().codes[:, :, :2])
+
+
+@gpu
+def test_bounds_with_infinite_and_nan_keys():
+    """A block with an infinite or NaN anchor keeps finite ranges; the others are untouched."""
+    clean, dirty = make_cache(1, 1, 256, 128, seed=4, stride_k=16), make_cache(1, 1, 256, 128, seed=4, stride_k=16)
+    st = dirty.state
+    st[0][0, 0, 4, 7], st[0][0, 0, 4, 8], st[0][0, 0, 4, 9] = math.nan, math.inf, -math.inf
+    dirty.state = st
+    a, b = BlockIndex(clean, 64).update(), BlockIndex(dirty, 64).update()
+    assert torch.isfinite(b.bounds()).all()
+    keep = [0, 2, 3]
+    assert torch.equal(a.codes[:, :, keep], b.codes[:, :, keep])
+    codes, scales = ref_bounds(decoded(dirty, fp16_keys=True)[0], 64)
+    assert torch.equal(b.codes[:, :, :4].double(), codes) and torch.equal(b.scales[:, :, :4], scales)
+
+
+@gpu
+def test_bounds_of_equal_keys_are_exact():
+    """All keys zero: zero scale and codes.  One value everywhere: its range is the value."""
+    cache = ChronoQuantCache()
+    z = torch.zeros((1, 1, 80, 128), device="cuda").half()
+    cache.update_and_fetch(z, z)
+    index = BlockIndex(cache, 64).update()
+    assert not index.bounds().any()
+
+
+# ----------------------------------------------------------------------------- selection
+SELECT = [  # B, H, G, S, T, bt, top, first, recent
+    (1, 1, 1, 1, 1, 16, 1, 0, 0), (1, 2, 4, 1, 40, 16, 2, 1, 1), (2, 2, 4, 1, 1000, 32, 8, 1, 2),
+    (1, 2, 4, 7, 700, 64, 5, 1, 2), (1, 1, 8, 33, 300, 16, 6, 0, 1), (2, 1, 3, 2, 513, 32, 40, 2, 3),
+    (1, 2, 2, 1, 5000, 16, 64, 1, 2), (1, 1, 4, 16, 16, 16, 3, 1, 1), (3, 1, 16, 1, 700, 64, 4, 0, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("shape", SELECT)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_select_equals_definition(shape, dtype):
+    B, H, G, S, T, bt, top, first, recent = shape
+    cache = make_cache(B, H, T, 128, seed=T + S)
+    q = queries(B, H * G, S, 128, dtype)
+    index = BlockIndex(cache, bt)
+    blocks, scores = index.select(q, top, first=first, recent=recent, return_scores=True)  # updates by itself
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], bt)
+    ref, ref_s = ref_select(codes, scales, q, T, bt, top, first, recent)
+    assert torch.equal(blocks.cpu(), ref)
+    assert torch.equal(scores.cpu(), ref_s)
+    assert torch.equal(index.select(q, top, first=first, recent=recent), blocks)
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 64, 72, 256])
+def test_select_head_dims(D):
+    cache = make_cache(2, 2, 600, D, seed=D)
+    q = queries(2, 6, 3, D, torch.float16)
+    got = BlockIndex(cache, 16).select(q, 9)
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 16)
+    assert torch.equal(got.cpu(), ref_select(codes, scales, q, 600, 16, 9, 1, 2)[0])
+
+
+@gpu
+def test_select_ties_go_to_the_lowest_index():
+    """Constant keys: every block has the same score, so the list is the first
+    ones and the recent ones; a zero query scores every block 0."""
+    cache = ChronoQuantCache()
+    one = torch.ones((1, 1, 640, 128), device="cuda").half()
+    cache.update_and_fetch(one, one)
+    index = BlockIndex(cache, 16)
+    for q in (queries(1, 4, 1, 128, torch.float16), torch.zeros((1, 4, 1, 128), device="cuda").half()):
+        got, s = index.select(q, 10, first=1, recent=2, return_scores=True)
+        assert got.flatten().tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 38, 39]
+        assert (s == s.flatten()[0]).all()
+
+
+@gpu
+def test_select_odd_queries():
+    """NaN, infinite, huge, tiny and denormal query values follow the definition; strided queries too."""
+    cache = make_cache(1, 2, 900, 128, seed=1)
+    index = BlockIndex(cache, 16).update()
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 16)
+    q = queries(1, 8, 4, 128, torch.bfloat16)
+    q[0, 0, 0, 3], q[0, 1, 0, 4], q[0, 2, 1, 5] = math.nan, math.inf, -math.inf
+    q[0, 3, 2] *= 1e36
+    q[0, 4, 2] *= 1e-36
+    q[0, 5, 3] = 0
+    q[0, 4:8, 3] = 1e-39
+    ref, ref_s = ref_select(codes, scales, q, 900, 16, 12, 1, 2)
+    got, s = index.select(q, 12, return_scores=True)
+    assert torch.equal(got.cpu(), ref) and torch.equal(s.cpu(), ref_s)
+    strided = torch.zeros((1, 4, 8, 256), dtype=torch.bfloat16, device="cuda").transpose(1, 2)[..., 64:192]
+    strided.copy_(q)
+    assert torch.equal(index.select(strided, 12), got)
+    spread = torch.zeros((1, 8, 4, 256), dtype=torch.bfloat16, device="cuda")[..., ::2]
+    spread.copy_(q)
+    assert torch.equal(index.select(spread, 12), got)
+
+
+@gpu
+def test_select_padded_batch():
+    """Left padding: nothing before a sequence's first token is listed; a
+    sequence that is all padding gets an empty list, a negative start is 0."""
+    cache = make_cache(5, 1, 500, 128, seed=6)
+    starts = torch.tensor([0, 130, 499, 500, -3], device="cuda")
+    q = queries(5, 4, 3, 128, torch.bfloat16)
+    index = BlockIndex(cache, 16).update()
+    codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 16)
+    got, s = index.select(q, 8, starts=starts, return_scores=True)
+    ref, ref_s = ref_select(codes, scales, q, 500, 16, 8, 1, 2, starts)
+    assert torch.equal(got.cpu(), ref) and torch.equal(s.cpu(), ref_s)
+    assert (got[3] == -1).all() and (got[2, 0, 0] == -1).all() and got[2, 0, 2, 0] == 31
+
+
+# ----------------------------------------------------------------------------- attention
+LAYOUTS = [dict(), dict(stride_k=64, stride_v=32, delta_bits_v=3), dict(stride_k=16, stride_v=16),
+           dict(stride_k=64, stride_v=32, delta_bits_v=3, v_pack=3), dict(stride_k=32, stride_v=8, delta_bits_v=2,
+                                                                          v_pack=2),
+           dict(stride_k=12, stride_v=4), dict(stride_k=1, stride_v=1)]
+SPARSE = [  # B, H, G, S, T, bt, top
+    (1, 1, 1, 1, 1, 64, 1), (2, 2, 4, 1, 333, 64, 3), (1, 2, 8, 1, 2000, 64, 9), (1, 2, 4, 5, 700, 64, 4),
+    (1, 1, 16, 2, 400, 128, 3), (2, 1, 3, 40, 257, 16, 5), (1, 2, 2, 1, 1500, 256, 4), (2, 1, 7, 3, 130, 48, 6),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kw", LAYOUTS)
+@pytest.mark.parametrize("shape", SPARSE)
+def test_sparse_attention_matches_64_bits(kw, shape):
+    B, H, G, S, T, bt, top = shape
+    cache = make_cache(B, H, T, 128, seed=T, **kw)
+    dtype = torch.bfloat16 if T % 2 else torch.float16
+    q = queries(B, H * G, S, 128, dtype)
+    blocks = BlockIndex(cache, bt).select(q, top, first=0, recent=1)
+    scale = 128 ** -0.5
+    ref, rlse, vmax = ref_sparse(*decoded(cache), q, scale, blocks, bt)
+    check_attention(chronoquant_sparse_sdpa(q, cache, scale, blocks, bt), ref, vmax)
+    out, lse = chronoquant_sparse_sdpa(q, cache, scale, blocks, bt, return_lse=True)
+    assert out.dtype == lse.dtype == torch.float32
+    check_attention(out, ref, vmax)
+    assert (lse.double() - rlse).abs().max() <= 2.0 ** -10
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 64, 72, 256])
+def test_sparse_attention_head_dims(D):
+    cache = make_cache(2, 2, 300, D, seed=D)
+    q = queries(2, 4, 2, D, torch.float16)
+    blocks = BlockIndex(cache, 32).select(q, 4)
+    ref, _, vmax = ref_sparse(*decoded(cache), q, D ** -0.5, blocks, 32)
+    check_attention(chronoquant_sparse_sdpa(q, cache, D ** -0.5, blocks, 32), ref, vmax)
+
+
+@gpu
+@pytest.mark.parametrize("kw", LAYOUTS[:3] + LAYOUTS[5:6])
+def test_sparse_attention_over_every_block_is_dense_attention(kw):
+    """With every block listed the result is the dense decode's, and lists that
+    split the blocks merge back by their log-sum-exps."""
+    cache = make_cache(2, 2, 777, 128, seed=3, **kw)
+    q = queries(2, 8, 1, 128, torch.float16)
+    scale = 128 ** -0.5
+    every = torch.arange(13, dtype=torch.int32, device="cuda").expand(2, 2, 1, 13)
+    K, V = decoded(cache)
+    ref, _, vmax = ref_sparse(K, V, q, scale, every, 64)
+    check_attention(chronoquant_sparse_sdpa(q, cache, scale, every, 64), ref, vmax)
+    check_attention(chronoquant_sdpa(q, None, None, cache, scale), ref, vmax)
+    parts = [chronoquant_sparse_sdpa(q, cache, scale, every[..., s], 64, return_lse=True)
+             for s in (slice(0, 5), slice(5, 6), slice(6, 13))]
+    lse = torch.stack([p[1] for p in parts])
+    w = torch.softmax(lse, 0).unsqueeze(-1)
+    check_attention((w * torch.stack([p[0] for p in parts])).sum(0), ref, vmax)
+
+
+@gpu
+@pytest.mark.parametrize("kw", [LAYOUTS[0], LAYOUTS[1], LAYOUTS[5]])
+def test_sparse_attention_lists(kw):
+    """Absent entries anywhere, repeats, blocks behind the query or past the
+    cache, an empty list (zeros, -inf) and lists of one entry."""
+    cache = make_cache(1, 3, 500, 128, seed=8, **kw)
+    q = queries(1, 6, 2, 128, torch.float16)
+    rows = [[[-1, 0, 0, 3, 7, 7], [2, -1, -1, 5, 6, 7]], [[-1] * 6, [7, 8, 100, 2 ** 30, 2 ** 31 - 1, -7]],
+            [[7, -1, -1, -1, -1, -1], [8, 9, 10, 11, 12, 13]]]
+    blocks = torch.tensor(rows, dtype=torch.int32, device="cuda").unsqueeze(0)
+    ref, rlse, vmax = ref_sparse(*decoded(cache), q, 0.1, blocks, 64)
+    out, lse = chronoquant_sparse_sdpa(q, cache, 0.1, blocks, 64, return_lse=True)
+    check_attention(out, ref, vmax)
+    empty = torch.isinf(rlse)
+    assert torch.equal(torch.isinf(lse), empty) and empty[0, 2, 0] and empty[0, 5, 1]
+    assert not out[empty].any()
+    assert (lse[~empty].double() - rlse[~empty]).abs().max() <= 2.0 ** -10
+    one = blocks[..., 3:4]
+    ref, _, vmax = ref_sparse(*decoded(cache), q, 0.1, one, 64)
+    check_attention(chronoquant_sparse_sdpa(q, cache, 0.1, one, 64), ref, vmax)  # a strided list
+
+
+@gpu
+@pytest.mark.parametrize("kw", [LAYOUTS[0], LAYOUTS[1], LAYOUTS[5]])
+def test_sparse_attention_padded_batch(kw):
+    """Left padding that ends inside a block, at a block border, in the last
+    token and beyond it (zeros); NaN in the padding reaches no output."""
+    T = 300
+    g = torch.Generator(device="cuda").manual_seed(1)
+    starts = torch.tensor([0, 70, 128, 299, 300, -5], device="cuda")
+    k, v = (torch.randn((6, 2, T, 128), generator=g, device="cuda").half() for _ in range(2))
+    for b, s in enumerate(starts.tolist()):
+        if 0 < s <= T:  # the codec spreads an anchor over its stride: poison whole anchor groups only
+            s = s // 64 * 64
+            k[b, :, :s], v[b, :, :s] = math.nan, math.nan
+    cache = ChronoQuantCache(**kw)
+    if 64 % cache.stride_k or 64 % cache.stride_v:
+        k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    cache.update_and_fetch(k, v)
+    q = queries(6, 8, 2, 128, torch.bfloat16)
+    index = BlockIndex(cache, 16 if kw == LAYOUTS[5] else 64)
+    blocks = index.select(q, 3, starts=starts)
+    K, V = decoded(cache)
+    ref, _, vmax = ref_sparse(K, V, q, 0.09, blocks, index.block_tokens, starts)
+    out = chronoquant_sparse_sdpa(q, cache, 0.09, blocks, index.block_tokens, starts=starts)
+    check_attention(out, ref, vmax)
+    assert not out[4].any() and not out[3, :, 0].any() and out[3, :, 1].any()
+
+
+@gpu
+def test_sparse_attention_extreme_scores():
+    """Scores of +-1e4: no overflow, and the largest key alone decides."""
+    cache = make_cache(1, 1, 400, 128, seed=2)
+    q = queries(1, 4, 1, 128, torch.float16, amp=300.0)
+    blocks = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda").view(1, 1, 1, 4)
+    K, V = decoded(cache)
+    ref, rlse, vmax = ref_sparse(K, V, q, 0.25, blocks, 64)
+    out, lse = chronoquant_sparse_sdpa(q, cache, 0.25, blocks, 64, return_lse=True)
+    # fp32 accumulation of scores of magnitude |s|: 2^-22 |s| each, and p changes by that factor
+    slack = 2.0 ** -20 * rlse.abs().max()
+    assert (lse.double() - rlse).abs().max() <= 2.0 ** -10 + slack
+    assert ((out.double() - ref).abs() <= (5 * 2.0 ** -11 + 2 * slack) * vmax).all()
+
+
+@gpu
+def test_run_of_the_operators_together():
+    """A decode loop as a program runs it: append, update, select, attend --
+    the whole against 64 bits at every step, across block and page ends."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    cache = make_cache(2, 2, 250, 128, seed=1, stride_k=64, stride_v=32, delta_bits_v=3)
+    index = BlockIndex(cache, 64).update()
+    for step in range(10):
+        cache.update_and_fetch(*(torch.randn((2, 2, 1, 128), generator=g, device="cuda").bfloat16() for _ in range(2)))
+        q = queries(2, 8, 1, 128, torch.bfloat16, seed=step)
+        index.update()
+        blocks = index.select(q, 3, first=1, recent=1)
+        codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 64)
+        assert torch.equal(blocks.cpu(), ref_select(codes, scales, q, cache.offset, 64, 3, 1, 1)[0])
+        out = chronoquant_sparse_sdpa(q, cache, 128 ** -0.5, blocks, 64)
+        ref, _, vmax = ref_sparse(*decoded(cache), q, 128 ** -0.5, blocks, 64)
+        check_attention(out, ref, vmax)
+
+
+@gpu
+def test_captured_and_on_another_stream():
+    """The three calls captured into one graph and replayed with other queries,
+    and two captures replayed in turn on a side stream: their own results."""
+    cache = make_cache(1, 2, 900, 128, seed=5)
+    index = BlockIndex(cache, 32).update()
+    qa, qb = queries(1, 8, 1, 128, torch.bfloat16, seed=1), queries(1, 8, 1, 128, torch.bfloat16, seed=2)
+
+    def step(q):
+        blocks = index.update(cache.offset - 1).select(q, 7)
+        return blocks, chronoquant_sparse_sdpa(q, cache, 0.1, blocks, 32)
+
+    want = [[x.clone() for x in step(q)] for q in (qa, qb)]
+    bufs, graphs = [torch.empty_like(qa), torch.empty_like(qa)], []
+    for q in bufs:
+        q.copy_(qa)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(q)
+        graphs.append((graph, out))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        bufs[0].copy_(qa)
+        bufs[1].copy_(qb)
+        for _ in range(3):
+            for graph, _ in graphs:
+                graph.replay()
+        bufs[0].copy_(qb)
+        graphs[0][0].replay()
+        got0 = [x.clone() for x in graphs[0][1]]
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(got0, want[1]):
+        assert torch.equal(x, y)
+    for x, y in zip(graphs[1][1], want[1]):
+        assert torch.equal(x, y)
+
+
+# ----------------------------------------------------------------------------- refusals
+@gpu
+def test_refusals():
+    cache = make_cache(2, 2, 100, 128)
+    index = BlockIndex(cache, 32).update()
+    q = queries(2, 4, 1, 128, torch.float16)
+    blocks = index.select(q, 3)
+    for kw in (dict(top=0), dict(top=2, first=1, recent=2), dict(top=5000), dict(top=3, first=-1)):
+        with pytest.raises(ValueError):
+            index.select(q, **kw)
+    bad = [q[:1], q[:, :3], q[..., :64], q[0], q.expand(2, 4, 101, 128), q[:, :0], q[:, :, :0]]
+    for x in bad:
+        with pytest.raises(ValueError):
+            index.select(x, 3)
+        with pytest.raises(ValueError):
+            chronoquant_sparse_sdpa(x, cache, 1.0, blocks, 32)
+    with pytest.raises(TypeError):
+        index.select(q.float(), 3)
+    with pytest.raises(TypeError):
+        chronoquant_sparse_sdpa(q.float(), cache, 1.0, blocks, 32)
+    with pytest.raises(ValueError):
+        index.select(q.cpu(), 3)
+    for x in (blocks.long(), blocks[0], blocks[:1], blocks[..., :0], blocks.cpu(), blocks.expand(2, 2, 2, 3)):
+        with pytest.raises(ValueError):
+            chronoquant_sparse_sdpa(q, cache, 1.0, x, 32)
+    for s in (torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda"),
+              torch.zeros(2, dtype=torch.int64)):
+        with pytest.raises(ValueError):
+            index.select(q, 3, starts=s)
+        with pytest.raises(ValueError):
+            chronoquant_sparse_sdpa(q, cache, 1.0, blocks, 32, starts=s)
+    for bt in (0, 8, 40):
+        with pytest.raises(ValueError):
+            chronoquant_sparse_sdpa(q, cache, 1.0, blocks, bt)
+    with pytest.raises(ValueError):
+        index.update(101)
+    with pytest.raises(ValueError):
+        index.bounds(5)
+    with pytest.raises(ValueError):
+        index.bounds(-1)
+
+
+def test_empty_cache_and_bad_blocks_are_refused():
+    cache = ChronoQuantCache()
+    for bt in (0, 8, 17, -64):
+        with pytest.raises(ValueError):
+            BlockIndex(cache, bt)
+    index = BlockIndex(cache)
+    with pytest.raises(ValueError, match="empty"):
+        index.update()
+    with pytest.raises(ValueError):
+        index.bounds()
+    with pytest.raises(ValueError, match="empty"):
+        index.select(torch.zeros((1, 1, 1, 128), dtype=torch.float16), 3)
+    with pytest.raises(ValueError, match="empty"):
+        chronoquant_sparse_sdpa(torch.zeros((1, 1, 1, 128)), cache, 1.0, torch.zeros((1, 1, 1, 1)), 64)
+    assert index.n_blocks == 0 and index.nbytes == 0
+
+
+def _desc(**over):
+    d = _lib.CqPagedCache()
+    d.batch, d.kv_heads, d.head_dim, d.page_tokens, d.max_pages, d.n_pages = 2, 8, 128, 256, 4, 8
+    d.block_table = 0x1000
+    for name, s in (("k", 32), ("v", 8)):
+        c = getattr(d, name)
+        c.stride, c.bits, c.anchors_per_page, c.pframes_per_page = s, 4, 256 // s, 256 - 256 // s
+        c.scale_row, c.scale_index = 256, 1
+        c.keyframes, c.codes, c.scales = 0x2000, 0x3000, 0x4000
+    for k, v in over.items():
+        setattr(d, k, v)
+    return d
+
+
+P = 0x10000  # a pointer that the refused calls never follow
+BOUNDS = dict(t0=0, T=1000, bt=64, codes=P, scales=P, max_blocks=16)
+SELECT_ARGS = dict(codes=P, scales=P, max_blocks=16, bt=64, B=2, H=8, D=128, T=1000, len=None, q=P, dt=0, Hq=32, S=1,
+                   sb=4096, sh=128, sq=128, starts=None, first=1, recent=2, top=8, blocks=P, scores=None, ws=P,
+                   nws=1 << 20)
+SPARSE_ARGS = dict(T=1000, len=None, q=P, dt=0, Hq=32, S=1, sb=4096, sh=128, sq=128, scale=1.0, starts=None, blocks=P,
+                   top=8, bt=64, out=P, odt=0, lse=None, ws=P, nws=1 << 30)
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(codes=None), -1), (dict(scales=None), -1), (dict(bt=0), -1), (dict(T=0), -1), (dict(T=1025), -1),
+    (dict(max_blocks=15), -1), (dict(t0=-1), -1), (dict(t0=1001), -1)])
+def test_c_bounds_refusals(over, status):
+    a = {**BOUNDS, **over}
+    d = ctypes.byref(_desc())
+    assert _lib.lib().cq_block_bounds(d, *a.values(), None) == status
+    assert _lib.lib().cq_last_error()
+    if "t0" not in over:
+        assert _lib.lib().cq_block_bounds_at(d, P, a["T"], 1, a["bt"], a["codes"], a["scales"], a["max_blocks"],
+                                             None) == status
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(codes=None), -1), (dict(q=None), -1), (dict(blocks=None), -1), (dict(dt=2), -2), (dict(D=12), -2),
+    (dict(D=264), -2), (dict(Hq=12), -1), (dict(Hq=0), -1), (dict(S=0), -1), (dict(S=1001), -1), (dict(top=0), -1),
+    (dict(top=2), -1), (dict(first=-1), -1), (dict(recent=-1), -1), (dict(top=4097), -2), (dict(max_blocks=15), -1),
+    (dict(ws=None), -4), (dict(nws=8), -4), (dict(bt=0), -1), (dict(B=0), -1), (dict(recent=2 ** 31 - 1), -1)])
+def test_c_select_refusals(over, status):
+    assert _lib.lib().cq_block_select(*{**SELECT_ARGS, **over}.values(), None) == status
+
+
+@pytest.mark.parametrize("over,status", [
+    (dict(q=None), -1), (dict(blocks=None), -1), (dict(out=None), -1), (dict(dt=2), -2), (dict(odt=3), -2),
+    (dict(Hq=12), -1), (dict(S=0), -1), (dict(S=1001), -1), (dict(T=1025), -1), (dict(top=0), -1), (dict(bt=0), -1),
+    (dict(top=4097), -2), (dict(ws=None), -4), (dict(nws=64), -4)])
+def test_c_sparse_refusals(over, status):
+    assert _lib.lib().cq_sparse_attention(ctypes.byref(_desc()), *{**SPARSE_ARGS, **over}.values(), None) == status
+
+
+def test_c_bounds_read_refusals():
+    L = _lib.lib()
+    for args in ((None, P, 16, 16, 0, 4, 128, P), (P, P, 16, 16, 0, 17, 128, P), (P, P, 16, 16, -1, 4, 128, P),
+                 (P, P, 16, 16, 13, 4, 128, P), (P, P, 0, 16, 0, 4, 128, P), (P, P, 16, 16, 0, 4, 300, P),
+                 (P, P, 16, 16, 0, 4, 128, None)):
+        assert L.cq_block_bounds_read(*args, None) == -1
