@@ -19,6 +19,21 @@ int check_launch(const char *what) {
   return CQ_OK;
 }
 
+int sm_count() {
+  static int n[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  if (!n[dev]) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) cudaGetLastError();
+    n[dev] = v > 0 ? v : 148;
+  }
+  return n[dev];
+}
+
 static int validate_component(const cq_paged_cache *c, const cq_component &k, const char *name) {
   std::string n(name);
   CQ_REQUIRE(k.stride >= 1, CQ_ERR_INVALID, n + ": stride must be >= 1");

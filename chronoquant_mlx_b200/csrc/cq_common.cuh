@@ -17,6 +17,7 @@ namespace cq {
 // ---------------------------------------------------------------------------
 int set_error(int code, const std::string &msg);
 int check_launch(const char *what);
+int sm_count();  // of the current device
 
 #define CQ_REQUIRE(cond, code, msg)                  \
   do {                                               \
@@ -190,6 +191,7 @@ int read_bounds_error_attention(int clear);
 int read_bounds_error_prefill(int clear);
 int read_bounds_error_decode(int clear);
 int read_bounds_error_sparse(int clear);
+int read_bounds_error_sparse_fast(int clear);
 
 // Locations of token t (absolute) of (b, h) in component comp.
 struct TokLoc {

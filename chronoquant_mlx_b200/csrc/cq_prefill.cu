@@ -617,13 +617,6 @@ bool prefill_supported(const cq_paged_cache &c, int n_q_heads, int q_len) {
   return G >= 1 && G <= 16 && (G & (G - 1)) == 0;
 }
 
-static int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    n = 0;
-  return n > 0 ? n : 148;
-}
-
 struct Shape {
   int n_kt, TQ, n_qt, splits;
   int64_t rows;  // output rows B * Hq * q_len

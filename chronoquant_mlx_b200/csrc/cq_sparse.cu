@@ -398,7 +398,8 @@ int read_sparse_error(int clear) {
     const int z = 0;
     cudaMemcpyToSymbol(sparse::g_sparse_error, &z, sizeof(int));
   }
-  return v;
+  const int f = read_sparse_fast_error(clear);
+  return v ? v : f;
 }
 int read_bounds_error_sparse(int clear) { return read_bounds_error_here(clear); }
 
@@ -529,6 +530,10 @@ extern "C" int cq_sparse_attention_workspace(const cq_paged_cache *cache, int64_
   int r = sparse_checks(cache, T, n_q_heads, q_len, top, block_tokens);
   if (r) return r;
   CQ_REQUIRE(bytes, CQ_ERR_INVALID, "cq_sparse_attention_workspace: bytes is null");
+  if (sparse_fast_supported(*cache, n_q_heads, block_tokens)) {
+    *bytes = 0;
+    return CQ_OK;
+  }
   const int64_t rows = (int64_t)cache->batch * n_q_heads * q_len;
   *bytes = sparse::generic_bytes(rows, sparse::pick_list_splits(rows, top), cache->head_dim);
   return CQ_OK;
@@ -547,6 +552,9 @@ extern "C" int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const
   CQ_REQUIRE(out_dtype == CQ_F16 || out_dtype == CQ_BF16 || out_dtype == CQ_F32, CQ_ERR_UNSUPPORTED,
              "cq_sparse_attention: bad out dtype");
   const int64_t rows = (int64_t)cache->batch * n_q_heads * q_len;
+  if (sparse_fast_supported(*cache, n_q_heads, block_tokens))
+    return run_sparse_fast(*cache, T, len_dev, q, q_dtype, n_q_heads, q_len, q_sb, q_sh, q_sq, scale, starts, blocks,
+                           top, block_tokens, out, out_dtype, lse_out, (cudaStream_t)stream);
   const int splits = sparse::pick_list_splits(rows, top), D = cache->head_dim;
   CQ_REQUIRE(workspace && workspace_bytes >= sparse::generic_bytes(rows, splits, D), CQ_ERR_WORKSPACE,
              "cq_sparse_attention: workspace too small");
