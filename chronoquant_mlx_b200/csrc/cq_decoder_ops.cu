@@ -100,11 +100,11 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const void *qkv, int6
   for (int i = 0; i < 4; ++i) store_from_float(o, dst + i, out[i], dt);
 }
 
-// Head norm and rotation of many tokens: one CTA per token, a warp per head in
-// turn.  The angle of a channel pair is pos * inv_freq in fp64 (a product of
-// two fp32 numbers is off by radians at far positions), reduced to
-// [-pi, pi] there; its sine and cosine are shared by the token's heads.  All
-// arithmetic is fp32 with one rounding to the tensor type at the end.
+// Head norm and rotation of many tokens.  The angle of a channel pair is pos *
+// inv_freq in fp64 (a product of two fp32 numbers is off by radians at far
+// positions), reduced to [-pi, pi] there; its sine and cosine are shared by the
+// token's heads.  All arithmetic is fp32 with one rounding to the tensor type at
+// the end.
 struct RopeArgs {
   const void *qkv;
   int64_t sb, ss;        // element strides of a sequence and a token
@@ -119,6 +119,146 @@ struct RopeArgs {
 
 constexpr int kRopeWarps = 8;
 
+// (cos, sin) of pair i at position p.
+__device__ __forceinline__ float2 rope_angle(int64_t p, float inv_freq) {
+  const double ang = (double)p * (double)inv_freq;
+  // 2 pi as the sum of two doubles: the remainder keeps its digits for any angle below 2^53 turns
+  const double hi = 6.283185307179586, lo = 2.4492935982947064e-16;
+  const double n = rint(ang * (1.0 / hi));
+  float sn, cs;
+  sincosf((float)fma(-n, lo, fma(-n, hi, ang)), &sn, &cs);
+  return make_float2(cs, sn);
+}
+
+// Four consecutive channels in one access (the addresses are 4 elements aligned).
+template <int DT>
+__device__ __forceinline__ float4 load4(const void *p, int64_t i) {
+  if constexpr (DT == CQ_F32) return *(const float4 *)((const float *)p + i);
+  const uint2 u = *(const uint2 *)((const uint16_t *)p + i);
+  float2 a, b;
+  if constexpr (DT == CQ_F16) {
+    a = __half22float2(*(const __half2 *)&u.x);
+    b = __half22float2(*(const __half2 *)&u.y);
+  } else {
+    a = __bfloat1622float2(*(const __nv_bfloat162 *)&u.x);
+    b = __bfloat1622float2(*(const __nv_bfloat162 *)&u.y);
+  }
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <int DT>
+__device__ __forceinline__ void store4(void *p, int64_t i, const float4 v) {
+  if constexpr (DT == CQ_F32) {
+    *(float4 *)((float *)p + i) = v;
+  } else if constexpr (DT == CQ_F16) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    *(uint2 *)((uint16_t *)p + i) = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *(uint2 *)((uint16_t *)p + i) = make_uint2(*(const uint32_t *)&a, *(const uint32_t *)&b);
+  }
+}
+
+// D / 8 lanes hold a head, each two quads of channels that rotate with each
+// other: with halves, lane l < rot/8 the quads at 4l and rot/2 + 4l; with
+// adjacent pairs, 8l and 8l + 4; lanes past the rotated channels take theirs in
+// order and turn by 0.  So a head needs no exchange between lanes but the sum of
+// squares.  A CTA takes `tile` tokens: their angles once into shared memory,
+// then a group of lanes a (head, token) at a time, neighbouring groups
+// neighbouring tokens of one head, whose output rows are contiguous.
+template <int DT, int D>
+__global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_quads_kernel(RopeArgs A, int tile) {
+  constexpr int LPH = D / 8, GPW = 32 / LPH, UN = 2;
+  extern __shared__ float2 s_cs[];  // [tile][D / 2]
+  const int64_t tok0 = (int64_t)blockIdx.x * tile, n_tok = (int64_t)A.B * A.S;
+  const int nt = (int)min((int64_t)tile, n_tok - tok0), half = A.rot / 2;
+  for (int i = threadIdx.x; i < nt * (D / 2); i += blockDim.x) {
+    const int tt = i / (D / 2), k = i - tt * (D / 2);
+    const int64_t tok = tok0 + tt, b = tok / A.S, s = tok - b * A.S;
+    s_cs[i] = k < half ? rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]) : make_float2(1.f, 0.f);
+  }
+  __syncthreads();
+  const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH, groups = kRopeWarps * GPW;
+  const bool turns = l < A.rot / 8;
+  const bool halves = !A.adjacent && turns;
+  const int da = halves ? 4 * l : 8 * l, db = halves ? half + 4 * l : 8 * l + 4;
+  const int ca = 4 * l;  // the lane's first pair (from rot/2 on: no turn)
+  const int H = A.Hq + A.Hkv, items = H * nt;
+  const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+  float4 wqa = one, wqb = one, wka = one, wkb = one;
+  if (A.wq) {
+    wqa = load4<DT>(A.wq, da);
+    wqb = load4<DT>(A.wq, db);
+    wka = load4<DT>(A.wk, da);
+    wkb = load4<DT>(A.wk, db);
+  }
+  for (int base = 0; base < items; base += groups * UN) {  // the same trips for every lane: the sums are shuffles
+    float4 a[UN], c[UN];
+    int tt[UN], h[UN];
+    int64_t bb[UN], ss[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int it = base + u * groups + group;
+      if (it < items) {
+        h[u] = it / nt;
+        tt[u] = it - h[u] * nt;
+        const int64_t tok = tok0 + tt[u];
+        bb[u] = tok / A.S;
+        ss[u] = tok - bb[u] * A.S;
+        const int64_t src = bb[u] * A.sb + ss[u] * A.ss + (int64_t)h[u] * D;
+        a[u] = load4<DT>(A.qkv, src + da);
+        c[u] = load4<DT>(A.qkv, src + db);
+      } else {
+        h[u] = -1;
+        a[u] = c[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const bool is_q = h[u] < A.Hq;
+      if (A.wq) {
+        float sq = a[u].x * a[u].x;
+        sq = fmaf(a[u].y, a[u].y, sq);
+        sq = fmaf(a[u].z, a[u].z, sq);
+        sq = fmaf(a[u].w, a[u].w, sq);
+        sq = fmaf(c[u].x, c[u].x, sq);
+        sq = fmaf(c[u].y, c[u].y, sq);
+        sq = fmaf(c[u].z, c[u].z, sq);
+        sq = fmaf(c[u].w, c[u].w, sq);
+#pragma unroll
+        for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        const float r = rsqrtf(sq * (1.f / D) + A.eps);
+        const float4 wa = is_q ? wqa : wka, wb = is_q ? wqb : wkb;
+        a[u] = make_float4(a[u].x * r * wa.x, a[u].y * r * wa.y, a[u].z * r * wa.z, a[u].w * r * wa.w);
+        c[u] = make_float4(c[u].x * r * wb.x, c[u].y * r * wb.y, c[u].z * r * wb.z, c[u].w * r * wb.w);
+      }
+      if (h[u] < 0) continue;
+      const float4 *cs = (const float4 *)(s_cs + tt[u] * (D / 2) + ca);
+      const float4 p01 = cs[0], p23 = cs[1];  // cos, sin, cos, sin of four pairs
+      float4 x = a[u], y = c[u];
+      if (!turns) {  // channels past the rotated ones
+      } else if (!A.adjacent) {
+        x = make_float4(a[u].x * p01.x - c[u].x * p01.y, a[u].y * p01.z - c[u].y * p01.w,
+                        a[u].z * p23.x - c[u].z * p23.y, a[u].w * p23.z - c[u].w * p23.w);
+        y = make_float4(c[u].x * p01.x + a[u].x * p01.y, c[u].y * p01.z + a[u].y * p01.w,
+                        c[u].z * p23.x + a[u].z * p23.y, c[u].w * p23.z + a[u].w * p23.w);
+      } else {
+        x = make_float4(a[u].x * p01.x - a[u].y * p01.y, a[u].y * p01.x + a[u].x * p01.y,
+                        a[u].z * p01.z - a[u].w * p01.w, a[u].w * p01.z + a[u].z * p01.w);
+        y = make_float4(c[u].x * p23.x - c[u].y * p23.y, c[u].y * p23.x + c[u].x * p23.y,
+                        c[u].z * p23.z - c[u].w * p23.w, c[u].w * p23.z + c[u].z * p23.w);
+      }
+      void *out = is_q ? A.q_out : A.k_out;
+      const int64_t head = is_q ? bb[u] * A.Hq + h[u] : bb[u] * A.Hkv + (h[u] - A.Hq);
+      const int64_t dst = (head * A.S + ss[u]) * D;
+      store4<DT>(out, dst + da, x);
+      store4<DT>(out, dst + db, y);
+    }
+  }
+}
+
+// Every other shape (head sizes that are no 64, 128 or 256, rotations that end
+// inside a quad, rows off the quads' alignment): one CTA per token, a warp per
+// head in turn, channels exchanged through shared memory.
 template <int DT>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_rows_kernel(RopeArgs A) {
   __shared__ float2 s_cs[128];              // (cos, sin) of each pair
@@ -127,16 +267,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_rows_kernel(Rope
   const int b = (int)(tok / A.S), s = (int)(tok - (int64_t)b * A.S);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = A.rot / 2, D = A.D, H = A.Hq + A.Hkv;
-  for (int i = threadIdx.x; i < half; i += blockDim.x) {
-    const double ang = (double)A.pos[b * A.p_sb + s * A.p_ss] * (double)A.inv_freq[i];
-    // 2 pi as the sum of two doubles: the remainder keeps its digits for any angle below 2^53 turns
-    const double hi = 6.283185307179586, lo = 2.4492935982947064e-16;
-    const double n = rint(ang / hi);
-    const float r = (float)fma(-n, lo, fma(-n, hi, ang));
-    float sn, cs;
-    sincosf(r, &sn, &cs);
-    s_cs[i] = make_float2(cs, sn);
-  }
+  for (int i = threadIdx.x; i < half; i += blockDim.x)
+    s_cs[i] = rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[i]);
   __syncthreads();
   float *x = s_x[warp];
   for (int h = warp; h < H; h += kRopeWarps) {
@@ -251,9 +383,30 @@ extern "C" int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t
   CQ_REQUIRE(rot_dim == 0 || (inv_freq && pos), CQ_ERR_INVALID, "cq_qk_norm_rope_rows: inv_freq or pos is null");
   const dec::RopeArgs A{qkv,      seq_stride, row_stride, batch, tokens, n_q_heads, n_kv_heads, head_dim, rot_dim, adjacent,
                         q_norm_w, k_norm_w,   inv_freq,   pos,   pos_sb, pos_ss,    eps,        q_out,    k_out};
+  cudaStream_t st = (cudaStream_t)stream;
+  // the quads need 4-element alignment of every row and of the weights, and a rotation that ends with a quad
+  const uintptr_t unit = dtype == CQ_F32 ? 16 : 8, es = unit / 4;
+  const bool quads = (head_dim == 64 || head_dim == 128 || head_dim == 256) && rot_dim % 8 == 0 &&
+                     (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)q_norm_w |
+                       (uintptr_t)k_norm_w | (uintptr_t)(seq_stride * (int64_t)es) |
+                       (uintptr_t)(row_stride * (int64_t)es)) & (unit - 1)) == 0;
+  if (quads) {
+    // tokens per CTA: their angles are computed once for all heads, so several where there are CTAs enough
+    const int tile = n >= 8 * 1024 ? 8 : n >= 4 * 1024 ? 4 : 1;
+    const int64_t grid = (n + tile - 1) / tile;
+    const size_t smem = (size_t)tile * (head_dim / 2) * sizeof(float2);
+#define CQ_ROPE(DT)                                                                                         \
+  (head_dim == 64    ? dec::qk_norm_rope_quads_kernel<DT, 64>                                               \
+   : head_dim == 128 ? dec::qk_norm_rope_quads_kernel<DT, 128>                                              \
+                     : dec::qk_norm_rope_quads_kernel<DT, 256>)
+    auto *fn = dtype == CQ_F16 ? CQ_ROPE(CQ_F16) : dtype == CQ_BF16 ? CQ_ROPE(CQ_BF16) : CQ_ROPE(CQ_F32);
+#undef CQ_ROPE
+    fn<<<(unsigned)grid, dec::kRopeWarps * 32, smem, st>>>(A, tile);
+    return check_launch("cq_qk_norm_rope_rows");
+  }
   auto *fn = dtype == CQ_F16    ? dec::qk_norm_rope_rows_kernel<CQ_F16>
              : dtype == CQ_BF16 ? dec::qk_norm_rope_rows_kernel<CQ_BF16>
                                 : dec::qk_norm_rope_rows_kernel<CQ_F32>;
-  fn<<<(unsigned)n, dec::kRopeWarps * 32, 0, (cudaStream_t)stream>>>(A);
+  fn<<<(unsigned)n, dec::kRopeWarps * 32, 0, st>>>(A);
   return check_launch("cq_qk_norm_rope_rows");
 }
