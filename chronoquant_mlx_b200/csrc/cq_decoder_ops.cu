@@ -132,21 +132,36 @@ __device__ __forceinline__ float2 rope_angle(int64_t p, float inv_freq) {
 
 // Four consecutive channels in one access (the addresses are 4 elements aligned).
 template <int DT>
-__device__ __forceinline__ float4 load4(const void *p, int64_t i) {
-  if constexpr (DT == CQ_F32) return *(const float4 *)((const float *)p + i);
-  const uint2 u = *(const uint2 *)((const uint16_t *)p + i);
-  float2 a, b;
-  if constexpr (DT == CQ_F16) {
-    a = __half22float2(*(const __half2 *)&u.x);
-    b = __half22float2(*(const __half2 *)&u.y);
-  } else {
-    a = __bfloat1622float2(*(const __nv_bfloat162 *)&u.x);
-    b = __bfloat1622float2(*(const __nv_bfloat162 *)&u.y);
-  }
-  return make_float4(a.x, a.y, b.x, b.y);
+struct Quad {
+  using Raw = uint2;
+};
+template <>
+struct Quad<CQ_F32> {
+  using Raw = uint4;
+};
+template <int DT>
+__device__ __forceinline__ typename Quad<DT>::Raw load_quad(const void *p, int64_t i) {
+  using R = typename Quad<DT>::Raw;
+  return *(const R *)((const char *)p + i * (int64_t)(sizeof(R) / 4));
 }
 template <int DT>
-__device__ __forceinline__ void store4(void *p, int64_t i, const float4 v) {
+__device__ __forceinline__ float4 widen(const typename Quad<DT>::Raw &u) {
+  if constexpr (DT == CQ_F32) {
+    return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    float2 a, b;
+    if constexpr (DT == CQ_F16) {
+      a = __half22float2(*(const __half2 *)&u.x);
+      b = __half22float2(*(const __half2 *)&u.y);
+    } else {
+      a = __bfloat1622float2(*(const __nv_bfloat162 *)&u.x);
+      b = __bfloat1622float2(*(const __nv_bfloat162 *)&u.y);
+    }
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_quad(void *p, int64_t i, const float4 v) {
   if constexpr (DT == CQ_F32) {
     *(float4 *)((float *)p + i) = v;
   } else if constexpr (DT == CQ_F16) {
@@ -161,97 +176,93 @@ __device__ __forceinline__ void store4(void *p, int64_t i, const float4 v) {
 // D / 8 lanes hold a head, each two quads of channels that rotate with each
 // other: with halves, lane l < rot/8 the quads at 4l and rot/2 + 4l; with
 // adjacent pairs, 8l and 8l + 4; lanes past the rotated channels take theirs in
-// order and turn by 0.  So a head needs no exchange between lanes but the sum of
-// squares.  A CTA takes `tile` tokens: their angles once into shared memory,
-// then a group of lanes a (head, token) at a time, neighbouring groups
-// neighbouring tokens of one head, whose output rows are contiguous.
+// order and keep them.  So a head needs no exchange between lanes but the sum of
+// squares.  A CTA takes `tile` tokens (a power of two): their angles once, in
+// shared memory, then each group of lanes keeps one token and its angles in
+// registers and walks its share of the heads, UN heads' loads in flight.
+// Neighbouring groups hold neighbouring tokens, whose output rows are contiguous.
 template <int DT, int D>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_quads_kernel(RopeArgs A, int tile) {
-  constexpr int LPH = D / 8, GPW = 32 / LPH, UN = 2;
+  constexpr int LPH = D / 8, groups = kRopeWarps * 32 / LPH, UN = 4;
+  using Raw = typename Quad<DT>::Raw;
   extern __shared__ float2 s_cs[];  // [tile][D / 2]
   const int64_t tok0 = (int64_t)blockIdx.x * tile, n_tok = (int64_t)A.B * A.S;
-  const int nt = (int)min((int64_t)tile, n_tok - tok0), half = A.rot / 2;
-  for (int i = threadIdx.x; i < nt * (D / 2); i += blockDim.x) {
-    const int tt = i / (D / 2), k = i - tt * (D / 2);
-    const int64_t tok = tok0 + tt, b = tok / A.S, s = tok - b * A.S;
-    s_cs[i] = k < half ? rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]) : make_float2(1.f, 0.f);
+  const int half = A.rot / 2;
+  for (int i = threadIdx.x; i < tile * half; i += blockDim.x) {
+    const int tt = i / half, k = i - tt * half;
+    const int64_t tok = min(tok0 + tt, n_tok - 1), b = tok / A.S, s = tok - b * A.S;
+    s_cs[tt * (D / 2) + k] = rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]);
+  }
+  const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH;
+  const int tt = group & (tile - 1), h0 = group / tile, dh = groups / tile;
+  const bool turns = l < A.rot / 8, halves = !A.adjacent && turns, live = tok0 + tt < n_tok;
+  const int da = halves ? 4 * l : 8 * l, db = halves ? half + 4 * l : 8 * l + 4;
+  const int64_t tok = min(tok0 + tt, n_tok - 1), b = tok / A.S, s = tok - b * A.S;
+  const int64_t src = b * A.sb + s * A.ss;
+  const int H = A.Hq + A.Hkv;
+  Raw ra[UN], rc[UN];
+#pragma unroll
+  for (int u = 0; u < UN; ++u) {
+    const int64_t at = src + (int64_t)min(h0 + u * dh, H - 1) * D;
+    ra[u] = load_quad<DT>(A.qkv, at + da);
+    rc[u] = load_quad<DT>(A.qkv, at + db);
   }
   __syncthreads();
-  const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH, groups = kRopeWarps * GPW;
-  const bool turns = l < A.rot / 8;
-  const bool halves = !A.adjacent && turns;
-  const int da = halves ? 4 * l : 8 * l, db = halves ? half + 4 * l : 8 * l + 4;
-  const int ca = 4 * l;  // the lane's first pair (from rot/2 on: no turn)
-  const int H = A.Hq + A.Hkv, items = H * nt;
-  const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
-  float4 wqa = one, wqb = one, wka = one, wkb = one;
-  if (A.wq) {
-    wqa = load4<DT>(A.wq, da);
-    wqb = load4<DT>(A.wq, db);
-    wka = load4<DT>(A.wk, da);
-    wkb = load4<DT>(A.wk, db);
+  float4 p01 = make_float4(1.f, 0.f, 1.f, 0.f), p23 = p01;  // cos, sin of the lane's four pairs
+  if (turns) {
+    const float4 *cs = (const float4 *)(s_cs + tt * (D / 2) + 4 * l);
+    p01 = cs[0];
+    p23 = cs[1];
   }
-  for (int base = 0; base < items; base += groups * UN) {  // the same trips for every lane: the sums are shuffles
-    float4 a[UN], c[UN];
-    int tt[UN], h[UN];
-    int64_t bb[UN], ss[UN];
+  for (int base = 0; base < H; base += dh * UN) {  // the same trips for every lane: the sums are shuffles
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
-      const int it = base + u * groups + group;
-      if (it < items) {
-        h[u] = it / nt;
-        tt[u] = it - h[u] * nt;
-        const int64_t tok = tok0 + tt[u];
-        bb[u] = tok / A.S;
-        ss[u] = tok - bb[u] * A.S;
-        const int64_t src = bb[u] * A.sb + ss[u] * A.ss + (int64_t)h[u] * D;
-        a[u] = load4<DT>(A.qkv, src + da);
-        c[u] = load4<DT>(A.qkv, src + db);
-      } else {
-        h[u] = -1;
-        a[u] = c[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      const int h = base + h0 + u * dh;
+      float4 a = widen<DT>(ra[u]), c = widen<DT>(rc[u]);
+      {  // this slot's next head
+        const int64_t at = src + (int64_t)min(h + dh * UN, H - 1) * D;
+        if (base + dh * UN < H) {
+          ra[u] = load_quad<DT>(A.qkv, at + da);
+          rc[u] = load_quad<DT>(A.qkv, at + db);
+        }
       }
-    }
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const bool is_q = h[u] < A.Hq;
+      const bool is_q = h < A.Hq;
       if (A.wq) {
-        float sq = a[u].x * a[u].x;
-        sq = fmaf(a[u].y, a[u].y, sq);
-        sq = fmaf(a[u].z, a[u].z, sq);
-        sq = fmaf(a[u].w, a[u].w, sq);
-        sq = fmaf(c[u].x, c[u].x, sq);
-        sq = fmaf(c[u].y, c[u].y, sq);
-        sq = fmaf(c[u].z, c[u].z, sq);
-        sq = fmaf(c[u].w, c[u].w, sq);
+        float sq = a.x * a.x;
+        sq = fmaf(a.y, a.y, sq);
+        sq = fmaf(a.z, a.z, sq);
+        sq = fmaf(a.w, a.w, sq);
+        sq = fmaf(c.x, c.x, sq);
+        sq = fmaf(c.y, c.y, sq);
+        sq = fmaf(c.z, c.z, sq);
+        sq = fmaf(c.w, c.w, sq);
 #pragma unroll
         for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
         const float r = rsqrtf(sq * (1.f / D) + A.eps);
-        const float4 wa = is_q ? wqa : wka, wb = is_q ? wqb : wkb;
-        a[u] = make_float4(a[u].x * r * wa.x, a[u].y * r * wa.y, a[u].z * r * wa.z, a[u].w * r * wa.w);
-        c[u] = make_float4(c[u].x * r * wb.x, c[u].y * r * wb.y, c[u].z * r * wb.z, c[u].w * r * wb.w);
+        const void *w = is_q ? A.wq : A.wk;
+        const float4 wa = widen<DT>(load_quad<DT>(w, da)), wb = widen<DT>(load_quad<DT>(w, db));
+        a = make_float4(a.x * r * wa.x, a.y * r * wa.y, a.z * r * wa.z, a.w * r * wa.w);
+        c = make_float4(c.x * r * wb.x, c.y * r * wb.y, c.z * r * wb.z, c.w * r * wb.w);
       }
-      if (h[u] < 0) continue;
-      const float4 *cs = (const float4 *)(s_cs + tt[u] * (D / 2) + ca);
-      const float4 p01 = cs[0], p23 = cs[1];  // cos, sin, cos, sin of four pairs
-      float4 x = a[u], y = c[u];
+      if (h >= H || !live) continue;
+      float4 x = a, y = c;
       if (!turns) {  // channels past the rotated ones
       } else if (!A.adjacent) {
-        x = make_float4(a[u].x * p01.x - c[u].x * p01.y, a[u].y * p01.z - c[u].y * p01.w,
-                        a[u].z * p23.x - c[u].z * p23.y, a[u].w * p23.z - c[u].w * p23.w);
-        y = make_float4(c[u].x * p01.x + a[u].x * p01.y, c[u].y * p01.z + a[u].y * p01.w,
-                        c[u].z * p23.x + a[u].z * p23.y, c[u].w * p23.z + a[u].w * p23.w);
+        x = make_float4(a.x * p01.x - c.x * p01.y, a.y * p01.z - c.y * p01.w, a.z * p23.x - c.z * p23.y,
+                        a.w * p23.z - c.w * p23.w);
+        y = make_float4(c.x * p01.x + a.x * p01.y, c.y * p01.z + a.y * p01.w, c.z * p23.x + a.z * p23.y,
+                        c.w * p23.z + a.w * p23.w);
       } else {
-        x = make_float4(a[u].x * p01.x - a[u].y * p01.y, a[u].y * p01.x + a[u].x * p01.y,
-                        a[u].z * p01.z - a[u].w * p01.w, a[u].w * p01.z + a[u].z * p01.w);
-        y = make_float4(c[u].x * p23.x - c[u].y * p23.y, c[u].y * p23.x + c[u].x * p23.y,
-                        c[u].z * p23.z - c[u].w * p23.w, c[u].w * p23.z + c[u].z * p23.w);
+        x = make_float4(a.x * p01.x - a.y * p01.y, a.y * p01.x + a.x * p01.y, a.z * p01.z - a.w * p01.w,
+                        a.w * p01.z + a.z * p01.w);
+        y = make_float4(c.x * p23.x - c.y * p23.y, c.y * p23.x + c.x * p23.y, c.z * p23.z - c.w * p23.w,
+                        c.w * p23.z + c.z * p23.w);
       }
       void *out = is_q ? A.q_out : A.k_out;
-      const int64_t head = is_q ? bb[u] * A.Hq + h[u] : bb[u] * A.Hkv + (h[u] - A.Hq);
-      const int64_t dst = (head * A.S + ss[u]) * D;
-      store4<DT>(out, dst + da, x);
-      store4<DT>(out, dst + db, y);
+      const int64_t head = is_q ? b * A.Hq + h : b * A.Hkv + (h - A.Hq);
+      const int64_t dst = (head * A.S + s) * D;
+      store_quad<DT>(out, dst + da, x);
+      store_quad<DT>(out, dst + db, y);
     }
   }
 }
