@@ -16,6 +16,8 @@
 // the order of summation, and the three roundings after it are fixed: the
 // chosen lists are the same for every split of the work.
 #include <algorithm>
+#include <string>
+#include <type_traits>
 
 #include "cq_prefill.cuh"
 #include "cq_sparse.cuh"
@@ -108,15 +110,163 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
   if (threadIdx.x == 0) A.scales[row] = s;
 }
 
-// out [units][n][2][D] fp32 = code * scale of blocks first .. first + n - 1
-__global__ void bounds_read_kernel(const int8_t *codes, const float *scales, int64_t units, int64_t max_blocks,
-                                   int64_t first, int64_t n, int D, float *out) {
+// The same for the common layouts: head sizes D of 64, 128 or 256, K codes in
+// natural order with token-indexed scales, rows 16-byte aligned, strides that
+// are a multiple of the rows a warp takes at once.  A warp per block: D / 32
+// lanes hold a token's code row (16 bytes, 32 channels each), so 32 / (D / 32)
+// tokens at a time; every code pair becomes the fp16 pair code * scale + anchor
+// with the roundings of reconstruct and goes through packed min and max.  The
+// lanes that hold the same channels then meet by halves: each step a lane hands
+// over half of its channels and keeps the other half.  An I-frame's scale slot
+// is 0, so whatever its row reads (the row before it, inside the chunk block)
+// becomes the anchor itself (the chunk's first token reads row 0).
+template <int D>
+__global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, int64_t n_warps) {
+  constexpr int LPR = D / 32, RPI = 32 / LPR;  // lanes per row, rows at once
+  constexpr int W = D / 8;                     // words of a code row
+  const int lane = threadIdx.x & 31;
+  const CacheView &cv = A.cv;
+  const CompView &c = cv.c[0];
+  int64_t T = A.T, t0 = A.t0;
+  if (A.len_dev) {
+    T = launch_length(A.T, A.len_dev, A.S);
+    if (T == 0) {
+      if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+      return;
+    }
+    t0 = T - A.S;
+  }
+  const int64_t wi = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (wi >= n_warps) return;
+  const int64_t unit = wi / A.nb, j = t0 / A.bt + (wi - unit * A.nb);
+  const int64_t ta = j * A.bt, tb = min(T, ta + A.bt);
+  if (ta >= T) return;
+  const int b = (int)(unit / cv.H), h = (int)(unit - (int64_t)b * cv.H);
+  const int row = lane / LPR, part = lane % LPR;  // which of the rows at once, which 32 channels
+  const __half2 inf = __float2half2_rn(INFINITY);
+  __half2 lo[16], hi[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) lo[k] = inf, hi[k] = __hneg2(inf);
+
+  int64_t t = ta;
+  while (t < tb) {  // one anchor's tokens at a time: they lie in one chunk of one page
+    const int64_t lp = t / cv.P;
+    const int tl = (int)(t - lp * cv.P);
+    const int a = tl / c.stride;
+    const int64_t te = min(tb, t - (tl - a * c.stride) + c.stride);
+    const int64_t pg = page_of(cv, b, lp);
+    const int ct = c.pc + c.ac, jc = tl / ct, x0 = tl - jc * ct;  // chunk, position in it
+    const __half *arow = c.kf + kf_index(c, cv.H, D, pg, h, a) + part * 32;
+    const uint32_t *crow = c.codes + (pg * cv.H + h) * c.cd_hs + jc * c.cd_cs + part * 4;
+    const int i0 = x0 - x0 / c.stride - 1 + row;  // this lane's first code row
+    const __half *sc = c.scales + (pg * cv.H + h) * c.sc_hs + jc * c.sc_cs + x0 + row;
+    // the anchor's channels in the code words' pairs: (d, d + 4) of each 8
+    __half2 an[16];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint4 u = *(const uint4 *)(arow + 8 * w);
+      const uint32_t p[4] = {u.x, u.y, u.z, u.w};  // (0,1) (2,3) (4,5) (6,7)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t pr = __byte_perm(p[k >> 1], p[2 + (k >> 1)], (k & 1) ? 0x7632u : 0x5410u);
+        an[4 * w + k] = *(const __half2 *)&pr;
+      }
+    }
+    const int n = (int)(te - t);
+    for (int r0 = 0; r0 < n; r0 += 2 * RPI) {
+      uint4 code[2];
+      __half s1[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = r0 + u * RPI;
+        if (r + row < n) {
+          code[u] = *(const uint4 *)(crow + max(i0 + r, 0) * W);
+          s1[u] = sc[r];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (r0 + u * RPI + row >= n) continue;
+        const __half2 sv = __half2half2(s1[u]);
+        const uint32_t word[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // nibbles k and k + 4 as 1024 + n, minus 1032: the codes, exactly
+            const uint32_t v = ((word[w] >> (4 * k)) & 0x000f000fu) | 0x64006400u;
+            const __half2 code2 = __hsub2(*(const __half2 *)&v, __float2half2_rn(1032.f));
+            const __half2 key = __hadd2_rn(an[4 * w + k], __hmul2_rn(code2, sv));
+            lo[4 * w + k] = __hmin2(lo[4 * w + k], key);  // a NaN is left out
+            hi[4 * w + k] = __hmax2(hi[4 * w + k], key);
+          }
+      }
+    }
+    t = te;
+  }
+  // lanes of the same channels: rows meet by halves until a lane holds 16 / RPI pairs
+  int k0 = 0;  // first pair this lane still holds
+  auto meet = [&](auto pairs, int o) {
+    constexpr int n = decltype(pairs)::value / 2;
+    const bool up = lane & o;
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const __half2 gl = up ? lo[k] : lo[k + n], gh = up ? hi[k] : hi[k + n];
+      const __half2 kl = up ? lo[k + n] : lo[k], kh = up ? hi[k + n] : hi[k];
+      lo[k] = __hmin2(kl, __shfl_xor_sync(0xffffffffu, gl, o));
+      hi[k] = __hmax2(kh, __shfl_xor_sync(0xffffffffu, gh, o));
+    }
+    if (up) k0 += n;
+  };
+  meet(std::integral_constant<int, 16>(), 16);
+  meet(std::integral_constant<int, 8>(), 8);
+  if constexpr (LPR <= 4) meet(std::integral_constant<int, 4>(), 4);
+  if constexpr (LPR <= 2) meet(std::integral_constant<int, 2>(), 2);
+  constexpr int NP = RPI >= 16 ? 1 : 16 / RPI;  // pairs a lane ends with
+  float l[2 * NP], u[2 * NP], amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const float2 x = __half22float2(lo[k]), y = __half22float2(hi[k]);
+    const float lv[2] = {x.x, x.y}, uv[2] = {y.x, y.y};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float p = lv[e], q = uv[e];
+      if (p > q) p = q = 0.f;  // no value at all
+      p = fminf(fmaxf(p, -65504.f), 65504.f);
+      q = fminf(fmaxf(q, -65504.f), 65504.f);
+      l[2 * k + e] = p;
+      u[2 * k + e] = q;
+      amax = fmaxf(amax, fmaxf(fabsf(p), fabsf(q)));
+    }
+  }
+  amax = warp_max(amax);
+  const float s = __fdiv_rn(amax, 126.f);
+  const int64_t at = unit * A.max_blocks + j;
+  int8_t *codes = A.codes + at * 2 * D;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int pair = k0 + k, d = part * 32 + (pair >> 2) * 8 + (pair & 3);
+    store_codes(codes, d, D, l[2 * k], u[2 * k], s);
+    store_codes(codes, d + 4, D, l[2 * k + 1], u[2 * k + 1], s);
+  }
+  if (lane == 0) A.scales[at] = s;
+}
+
+// out [units][n][2][D] fp32 = code * scale of blocks first .. first + n - 1;
+// a warp per block, four codes a lane at a time (2D is a multiple of 4).
+__global__ void __launch_bounds__(256) bounds_read_kernel(const int8_t *codes, const float *scales, int64_t units,
+                                                          int64_t max_blocks, int64_t first, int64_t n, int D,
+                                                          float *out) {
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (row >= units * n) return;
   const int64_t u = row / n, j = first + (row - u * n);
-  const int8_t *c = codes + (u * max_blocks + j) * 2 * D;
+  const char4 *c = (const char4 *)(codes + (u * max_blocks + j) * 2 * D);
   const float s = scales[u * max_blocks + j];
-  for (int i = threadIdx.x & 31; i < 2 * D; i += 32) out[row * 2 * D + i] = (float)c[i] * s;
+  float4 *o = (float4 *)(out + row * 2 * D);
+  for (int i = threadIdx.x & 31; i < D / 2; i += 32) {
+    const char4 v = c[i];
+    o[i] = make_float4((float)v.x * s, (float)v.y * s, (float)v.z * s, (float)v.w * s);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -136,11 +286,136 @@ struct SelectArgs {
   int first, recent, top;
   int32_t *blocks;
   float *block_scores;
-  int64_t n;     // score row length: blocks of T
-  float *score;  // [units][q_len][n]
+  int64_t n, ns;  // blocks of T, stride of a score row (a multiple of 8)
+  float *score;   // [units][q_len][ns]
 };
 
-// One warp per (unit, query token, block).
+// One row of query codes: values x (finite, in the fp16 range) of amax, code rint(x * (127 / amax)).
+struct QueryScale {
+  float r, s;
+  __device__ explicit QueryScale(float amax) {
+    const bool zero = amax < kTinyQuery;
+    r = zero ? 0.f : __fdiv_rn(127.f, amax);
+    s = zero ? 0.f : __fdiv_rn(amax, 127.f);
+  }
+  __device__ int code(float x) const { return (int)rintf(__fmul_rn(x, r)); }
+};
+
+// D(16x8 s32) += A(16x32 s8, row) * B(32x8 s8, col)
+__device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Scores on the tensor cores (head sizes of KS * 32, groups of at most 16).
+// Rows of the product are (query token, head) pairs, GP = the group rounded up
+// to a power of two; columns are blocks; the sum runs over 2D codes, a query
+// row holding [min(q8, 0) | max(q8, 0)] against a block's [lower | upper] codes.
+// A lane loads 16 bytes of a block at a time; the order of the sum's terms is
+// permuted alike in both operands, so these are two steps' B fragments as they
+// come.  A CTA quantises `tiles` row tiles into shared memory once (rows 64
+// bytes apart modulo 128: no bank conflicts), then each warp keeps the codes of
+// two column tiles in registers and passes over the rows.
+constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
+
+template <int KS>
+__global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(SelectArgs A, int tiles, int gp, int passes) {
+  constexpr int D = KS * 32, STR = 2 * D + 64;
+  extern __shared__ __align__(16) unsigned char s_a[];  // [tiles * 16][STR], then fp32 [tiles * 16]
+  float *s_sg = (float *)(s_a + tiles * 16 * STR);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int tpt = 16 / gp;  // query tokens per row tile
+  const int64_t unit = blockIdx.z;
+  const int b = (int)(unit / A.H), h = (int)(unit - (int64_t)b * A.H);
+  const int i0 = blockIdx.y * tiles * tpt;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+  if (T == 0) return;
+  for (int r = warp; r < tiles * 16; r += kScoreWarps) {
+    const int i = i0 + r / gp, hd = r & (gp - 1);
+    const bool real = i < A.q_len && hd < A.G;
+    const int64_t qb = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq;
+    float x[KS], amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      x[k] = real ? finite_query(load_as_float(A.q, qb + lane * KS + k, A.q_dtype)) : 0.f;
+      amax = fmaxf(amax, fabsf(x[k]));
+    }
+    const QueryScale qs(warp_max(amax));
+    int8_t *row = (int8_t *)s_a + r * STR + lane * KS;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int c = qs.code(x[k]);
+      row[k] = (int8_t)min(c, 0);
+      row[D + k] = (int8_t)max(c, 0);
+    }
+    if (lane == 0) s_sg[r] = qs.s;
+  }
+  __syncthreads();
+  // the last block any of this CTA's tokens sees
+  const int i_last = min(A.q_len, i0 + tiles * tpt) - 1;
+  const int64_t j_end = min(A.n, (T - A.q_len + i_last) / A.bt + 1);
+  const int real_tiles = (i_last - i0) / tpt + 1;
+  const int8_t *codes = A.codes + unit * A.max_blocks * 2 * D;
+  const float *scales = A.scales + unit * A.max_blocks;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int64_t j0 = (((int64_t)blockIdx.x * passes + pass) * kScoreWarps + warp) * kScoreCols;
+    if (j0 >= j_end) break;
+    uint4 bf[2][KS];
+    float sj[2][2];
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const int8_t *src = codes + min(j0 + nb * 8 + g, A.n - 1) * 2 * D + 16 * t;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) bf[nb][k] = *(const uint4 *)(src + 64 * k);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sj[nb][e] = scales[min(j0 + nb * 8 + 2 * t + e, A.n - 1)];
+    }
+    for (int rt = 0; rt < real_tiles; ++rt) {
+      int acc[2][4] = {};
+      const unsigned char *a = s_a + (rt * 16 + g) * STR + 16 * t;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint4 x = *(const uint4 *)(a + 64 * k), y = *(const uint4 *)(a + 8 * STR + 64 * k);
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          mma_s8_16832(acc[nb], x.x, y.x, x.y, y.y, bf[nb][k].x, bf[nb][k].y);
+          mma_s8_16832(acc[nb], x.z, y.z, x.w, y.w, bf[nb][k].z, bf[nb][k].w);
+        }
+      }
+      const float sg[2] = {s_sg[rt * 16 + g], s_sg[rt * 16 + g + 8]};
+      const bool pad0 = (g & (gp - 1)) >= A.G, pad1 = ((g + 8) & (gp - 1)) >= A.G;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          v[e] = pad0 ? -INFINITY : __fmul_rn(__fmul_rn(sg[0], sj[nb][e]), (float)acc[nb][e]);
+          v[2 + e] = pad1 ? -INFINITY : __fmul_rn(__fmul_rn(sg[1], sj[nb][e]), (float)acc[nb][2 + e]);
+        }
+        if (gp == 16) v[0] = fmaxf(v[0], v[2]), v[1] = fmaxf(v[1], v[3]);
+        for (int o = 4; o < 4 * min(gp, 8); o <<= 1)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaxf(v[e], __shfl_xor_sync(0xffffffffu, v[e], o));
+        if ((g & (min(gp, 8) - 1)) == 0) {
+          const int64_t col = j0 + nb * 8 + 2 * t;
+          const int ia = i0 + rt * tpt + g / gp, ib = ia + 8 / gp;  // the tokens of rows g and g + 8
+          float *dst = A.score + (unit * A.q_len + ia) * A.ns + col;
+          if (col < A.ns) {
+            if (ia < A.q_len) *(float2 *)dst = make_float2(__fadd_rn(v[0], 0.f), __fadd_rn(v[1], 0.f));
+            if (gp < 16 && ib < A.q_len)
+              *(float2 *)(dst + (int64_t)(8 / gp) * A.ns) = make_float2(__fadd_rn(v[2], 0.f), __fadd_rn(v[3], 0.f));
+          }
+        }
+      }
+    }
+  }
+}
+
+// Every other shape: one warp per (unit, query token, block).
 __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
   if (T == 0) return;
@@ -165,27 +440,143 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
       x[k] = d < A.D ? finite_query(load_as_float(A.q, qb + d, A.q_dtype)) : 0.f;
       amax = fmaxf(amax, fabsf(x[k]));
     }
-    amax = warp_max(amax);
-    const bool zero = amax < kTinyQuery;
-    const float r = zero ? 0.f : __fdiv_rn(127.f, amax);
+    const QueryScale qs(warp_max(amax));
     int dot = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int d = lane + 32 * k;
       if (d < A.D) {
-        const int q8 = (int)rintf(__fmul_rn(x[k], r));
+        const int q8 = qs.code(x[k]);
         dot += q8 * (int)(q8 > 0 ? c[A.D + d] : c[d]);
       }
     }
     dot = __reduce_add_sync(0xffffffffu, dot);
-    const float sg = zero ? 0.f : __fdiv_rn(amax, 127.f);
-    best = fmaxf(best, __fmul_rn(__fmul_rn(sg, sj), (float)dot));
+    best = fmaxf(best, __fmul_rn(__fmul_rn(qs.s, sj), (float)dot));
   }
-  if (lane == 0) A.score[row * A.n + j] = __fadd_rn(best, 0.f);  // -0 becomes +0: equal scores have equal keys
+  if (lane == 0) A.score[row * A.ns + j] = __fadd_rn(best, 0.f);  // -0 becomes +0: equal scores have equal keys
 }
 
-// One CTA per (unit, query token): the `top` best visible blocks.  A radix
-// select finds the key of the last one taken (4 passes of 8 bits), and an
+// The `top` best visible blocks of a (unit, query token) row with every key in a
+// register: W warps hold KPT keys a thread.  The key of the last block taken is
+// found bit by bit (counts of keys at or above a candidate), and stops early
+// where a candidate has exactly `top`; the list is written in index order, of
+// equal keys the lowest indexes.
+template <int KPT, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W, int64_t rows) {
+  __shared__ int s_cnt[2][32];
+  __shared__ int s_pre[KPT * 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  if (T == 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+    return;
+  }
+  if (row >= rows) return;  // whole CTAs, or single warps that never meet others
+  const int i = (int)(row % A.q_len);
+  const int b = (int)(row / ((int64_t)A.q_len * A.H));
+  const int64_t p = T - A.q_len + i, st = first_token(A.starts, b);
+  const int fb = (int)min(st / A.bt, (int64_t)INT32_MAX), lb = (int)(p / A.bt);
+  const int nv = st > p ? 0 : lb - fb + 1;
+  const float *score = A.score + row * A.ns;
+  const int tid = warp * 32 + lane, step = W * 32;
+  uint32_t key[KPT];  // 0: no block (visible ones are above it)
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) {
+    const int x = k * step + tid;
+    key[k] = x >= nv ? 0u : (x < A.first || x >= nv - A.recent) ? 0xffffffffu : order_key(score[fb + x]);
+  }
+  int par = 0;
+  auto total = [&](int c) {  // over the row's threads
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (W == 1) return c;
+    if (lane == 0) s_cnt[par][warp] = c;
+    __syncthreads();
+    c = __reduce_add_sync(0xffffffffu, lane < W ? s_cnt[par][lane] : 0);
+    par ^= 1;
+    return c;
+  };
+  uint32_t thr = 1;  // keys at or above it are taken, those equal to it from the lowest index on
+  if (nv > A.top) {
+    thr = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t cand = thr | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) c += key[k] >= cand;
+      c = total(c);
+      if (c >= A.top) thr = cand;
+      if (c == A.top) break;
+    }
+  }
+  // per key slot k and warp: keys above the threshold (low half) and equal to it (high half)
+  int mine = 0, all_gt = 0;
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) {
+    const unsigned gt = __ballot_sync(0xffffffffu, key[k] > thr), eq = __ballot_sync(0xffffffffu, key[k] == thr);
+    const int packed = __popc(gt) | (__popc(eq) << 16);
+    if (W > 1) {
+      if (lane == 0) s_pre[k * W + warp] = packed;
+    } else if (lane == k) {
+      mine = packed;
+    }
+    all_gt += __popc(gt);
+  }
+  int running = 0;
+  if (W > 1) {
+    __syncthreads();
+    if (warp == 0) {  // exclusive prefix in index order: KPT * W <= KPT * 32 entries
+      int sum = 0;
+      for (int e = 0; e < KPT; ++e) {
+        const int at = lane * KPT + e;
+        if (at < KPT * W) sum += s_pre[at];
+      }
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+      }
+      if (lane == 31) s_cnt[0][0] = before;
+      before -= sum;
+      for (int e = 0; e < KPT; ++e) {
+        const int at = lane * KPT + e;
+        if (at < KPT * W) {
+          const int x = s_pre[at];
+          s_pre[at] = before;
+          before += x;
+        }
+      }
+    }
+    __syncthreads();
+    all_gt = s_cnt[0][0] & 0xffff;
+  }
+  const int need = A.top - all_gt;  // equal keys to take
+  int32_t *out = A.blocks + row * A.top;
+  float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) {
+    const bool gt = key[k] > thr, eq = key[k] == thr;
+    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    const int base = W > 1 ? s_pre[k * W + warp] : running;
+    const unsigned below = (1u << lane) - 1u;
+    const int g0 = (base & 0xffff) + __popc(bg & below), e0 = (base >> 16) + __popc(be & below);
+    if (gt || (eq && e0 < need)) {
+      const int at = g0 + min(e0, need), j = fb + k * step + tid;
+      out[at] = j;
+      if (out_s) out_s[at] = score[j];
+    }
+    if (W == 1) running += __shfl_sync(0xffffffffu, mine, k);
+  }
+  for (int k = min(nv, A.top) + tid; k < A.top; k += step) {
+    out[k] = -1;
+    if (out_s) out_s[k] = -INFINITY;
+  }
+}
+
+// The same for rows too long for registers: one CTA per row.  A radix select
+// finds the key of the last one taken (4 passes of 8 bits), and an
 // ordered pass writes the list, taking equal keys from the lowest index on.
 __global__ void __launch_bounds__(256) block_topk_kernel(SelectArgs A) {
   __shared__ int hist[256];
@@ -206,7 +597,7 @@ __global__ void __launch_bounds__(256) block_topk_kernel(SelectArgs A) {
   float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
   const int fb = (int)min(st / A.bt, (int64_t)INT32_MAX), lb = (int)(p / A.bt);
   const int nv = st > p ? 0 : lb - fb + 1;
-  const float *score = A.score + row * A.n;
+  const float *score = A.score + row * A.ns;
   auto key = [&](int j) -> uint32_t {
     return (j < fb + A.first || j > lb - A.recent) ? 0xffffffffu : order_key(score[j]);
   };
@@ -420,9 +811,22 @@ static int bounds_checks(const cq_paged_cache *cache, int64_t T, int32_t bt, con
   return CQ_OK;
 }
 
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const char *what) {
   const int64_t grid = (int64_t)A.cv.B * A.cv.H * A.nb;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_INVALID, std::string(what) + ": grid too large");
+  const CompView &c = A.cv.c[0];
+  const int D = A.cv.D, rows = D == 64 ? 16 : D == 128 ? 8 : 4;  // code rows a warp takes at once
+  if ((D == 64 || D == 128 || D == 256) && c.order == CQ_ORDER_NATURAL && c.stok && c.stride % rows == 0 &&
+      c.stride > 1 && A.bt % rows == 0 && aligned16(c.codes) && aligned16(c.kf) && (c.cd_hs | c.cd_cs) % 4 == 0 &&
+      (c.kf_hs | c.kf_cs) % 8 == 0) {
+    auto *fn = D == 64    ? sparse::block_bounds_rows_kernel<64>
+               : D == 128 ? sparse::block_bounds_rows_kernel<128>
+                          : sparse::block_bounds_rows_kernel<256>;
+    fn<<<(unsigned)((grid + 3) / 4), 128, 0, st>>>(A, grid);
+    return check_launch(what);
+  }
   const int threads = (A.cv.D + 31) & ~31;
   sparse::block_bounds_kernel<<<(unsigned)grid, threads, 0, st>>>(A);
   return check_launch(what);
@@ -467,7 +871,7 @@ static int select_sizes(int32_t batch, int32_t kv_heads, int32_t q_len, int64_t 
                         size_t *bytes) {
   CQ_REQUIRE(batch >= 1 && kv_heads >= 1 && block_tokens >= 1, CQ_ERR_INVALID, "cq_block_select: bad sizes");
   CQ_REQUIRE(q_len >= 1 && q_len <= T, CQ_ERR_INVALID, "cq_block_select: need 1 <= q_len <= T");
-  *bytes = (size_t)batch * kv_heads * q_len * ((T + block_tokens - 1) / block_tokens) * sizeof(float);
+  *bytes = (size_t)batch * kv_heads * q_len * (((T + block_tokens - 1) / block_tokens + 7) & ~7LL) * sizeof(float);
   return CQ_OK;
 }
 
@@ -475,6 +879,79 @@ extern "C" int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_
                                          int32_t block_tokens, size_t *bytes) {
   CQ_REQUIRE(bytes, CQ_ERR_INVALID, "cq_block_select_workspace: bytes is null");
   return select_sizes(batch, kv_heads, q_len, T, block_tokens, bytes);
+}
+
+// A launch that may start while the kernel before it in the stream drains (it
+// waits for that kernel's results itself).
+template <class... P, class... X>
+static int launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const char *what,
+                        X... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
+  if (e != cudaSuccess) return set_error(CQ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
+  using namespace sparse;
+  const int64_t rows = (int64_t)A.B * A.H * A.q_len, units = (int64_t)A.B * A.H;
+  void (*fn)(SelectArgs, int, int, int) = A.D == 64    ? block_score_mma_kernel<2>
+                                          : A.D == 96  ? block_score_mma_kernel<3>
+                                          : A.D == 128 ? block_score_mma_kernel<4>
+                                          : A.D == 256 ? block_score_mma_kernel<8>
+                                                       : nullptr;
+  if (fn && A.G <= 16 && aligned16(A.codes) && aligned16(A.score) && units < 65536) {
+    int gp = 1;
+    while (gp < A.G) gp *= 2;
+    const int tpt = 16 / gp, row_tiles = (A.q_len + tpt - 1) / tpt;
+    // row tiles per CTA: their quantisation is shared by its columns; 48 KB hold 8 of them up to head size 128
+    const int tiles = std::min(row_tiles, A.D > 128 ? 4 : 8);
+    const int64_t groups = (row_tiles + tiles - 1) / tiles;
+    const int per = kScoreWarps * kScoreCols;
+    const int64_t cols = (A.n + per - 1) / per;
+    // several passes per CTA where there are CTAs enough without
+    const int passes = (int)std::max<int64_t>(1, std::min<int64_t>(cols, cols * groups * units / (8 * sm_count())));
+    const dim3 grid((unsigned)((cols + passes - 1) / passes), (unsigned)groups, (unsigned)units);
+    CQ_REQUIRE(groups < 65536, CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
+    return launch_after(fn, grid, kScoreWarps * 32, (size_t)tiles * 16 * (2 * A.D + 64 + 4), st, "cq_block_select", A,
+                        tiles, gp, passes);
+  }
+  const int64_t grid = (rows * A.n * 32 + 255) / 256;
+  CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many scores");
+  block_score_kernel<<<(unsigned)grid, 256, 0, st>>>(A);
+  return check_launch("cq_block_select");
+}
+
+static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t st) {
+  using namespace sparse;
+  CQ_REQUIRE(rows < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
+  // a warp per row where rows abound, else several warps with few keys a thread
+  const bool many = rows >= 16 * sm_count() && A.n <= 32 * 32;
+  int kpt = many ? 8 : 4;
+  while (kpt < (many ? 32 : 16) && A.n > (int64_t)kpt * 32 * (many ? 1 : 32)) kpt *= 2;
+  const int64_t W = (A.n + kpt * 32 - 1) / (kpt * 32);
+  if (W > 32) {
+    block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
+    return check_launch("cq_block_select");
+  }
+  void (*fn)(SelectArgs, int, int64_t) = many ? (kpt == 8    ? block_topk_regs_kernel<8, 128>
+                                                 : kpt == 16 ? block_topk_regs_kernel<16, 128>
+                                                             : block_topk_regs_kernel<32, 128>)
+                                              : (kpt == 4   ? block_topk_regs_kernel<4, 1024>
+                                                 : kpt == 8 ? block_topk_regs_kernel<8, 1024>
+                                                            : block_topk_regs_kernel<16, 1024>);
+  const int threads = W == 1 ? 128 : (int)W * 32;
+  const int64_t grid = W == 1 ? (rows + 3) / 4 : rows;
+  return launch_after(fn, dim3((unsigned)grid), threads, 0, st, "cq_block_select", A, (int)W, rows);
 }
 
 extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens,
@@ -500,15 +977,12 @@ extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t
   CQ_REQUIRE(workspace && workspace_bytes >= need, CQ_ERR_WORKSPACE, "cq_block_select: workspace too small");
   sparse::SelectArgs A{codes,  scales, max_blocks, block_tokens, batch, kv_heads, head_dim, n_q_heads / kv_heads,
                        q_len,  T,      len_dev,    q,            q_dtype, q_sb,   q_sh,     q_sq,
-                       starts, first,  recent,     top,          blocks,  block_scores,     n, (float *)workspace};
-  const int64_t rows = (int64_t)batch * kv_heads * q_len, grid = (rows * n * 32 + 255) / 256;
-  CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_INVALID, "cq_block_select: grid too large");
+                       starts, first,  recent,     top,          blocks,  block_scores,     n, (n + 7) & ~7LL, (float *)workspace};
+  const int64_t rows = (int64_t)batch * kv_heads * q_len;
   cudaStream_t st = (cudaStream_t)stream;
-  sparse::block_score_kernel<<<(unsigned)grid, 256, 0, st>>>(A);
-  r = check_launch("cq_block_select");
+  r = launch_scores(A, st);
   if (r) return r;
-  sparse::block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
-  return check_launch("cq_block_select");
+  return launch_topk(A, rows, st);
 }
 
 static int sparse_checks(const cq_paged_cache *cache, int64_t T, int32_t n_q_heads, int32_t q_len, int32_t top,
