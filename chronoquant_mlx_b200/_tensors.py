@@ -28,7 +28,12 @@ def require_cuda(*tensors: torch.Tensor) -> None:
                              f"got a tensor on {t.device}")
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without building a Stream object
+
+
 def stream_ptr(device: torch.device | None = None) -> int:
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

@@ -211,10 +211,9 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, in
     const bool up = lane & o;
 #pragma unroll
     for (int k = 0; k < n; ++k) {
-      const __half2 gl = up ? lo[k] : lo[k + n], gh = up ? hi[k] : hi[k + n];
-      const __half2 kl = up ? lo[k + n] : lo[k], kh = up ? hi[k + n] : hi[k];
-      lo[k] = __hmin2(kl, __shfl_xor_sync(0xffffffffu, gl, o));
-      hi[k] = __hmax2(kh, __shfl_xor_sync(0xffffffffu, gh, o));
+      const __half2 la = lo[k], lb = lo[k + n], ha = hi[k], hb = hi[k + n];
+      lo[k] = __hmin2(up ? lb : la, __shfl_xor_sync(0xffffffffu, up ? la : lb, o));
+      hi[k] = __hmax2(up ? hb : ha, __shfl_xor_sync(0xffffffffu, up ? ha : hb, o));
     }
     if (up) k0 += n;
   };

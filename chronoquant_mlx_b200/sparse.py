@@ -29,24 +29,35 @@ import torch
 
 from . import _lib
 from .trace import traced
-from ._tensors import cq_dtype, on_device, require_cuda, stream_ptr
+from ._tensors import on_device, require_cuda, stream_ptr
 
 MAX_TOP = 4096  # longest block list
 
 
-def _check_queries(q: torch.Tensor, B: int, H: int, D: int, T: int, device, what: str) -> torch.Tensor:
-    if q.dim() != 4 or q.shape[0] != B or q.shape[3] != D:
-        raise ValueError(f"{what}: queries must be [{B}, Hq, Tq, {D}], got {tuple(q.shape)}")
-    if q.device != device:
+_QUERY_DT = {torch.float16: _lib.CQ_F16, torch.bfloat16: _lib.CQ_BF16}
+
+
+def _check_queries(q: torch.Tensor, st, T: int, what: str):
+    """(queries with contiguous channels, C dtype, Hq, Tq, strides) after the checks against a store."""
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != st.B or shape[3] != st.D:
+        raise ValueError(f"{what}: queries must be [{st.B}, Hq, Tq, {st.D}], got {tuple(shape)}")
+    if q.device != st.device:
         require_cuda(q)
-        raise ValueError(f"{what}: queries on {q.device}, the cache on {device}")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: queries on {q.device}, the cache on {st.device}")
+    dt = _QUERY_DT.get(q.dtype)
+    if dt is None:
         raise TypeError(f"{what}: queries must be float16 or bfloat16, got {q.dtype}")
-    if q.shape[1] == 0 or q.shape[1] % H:
-        raise ValueError(f"{what}: {q.shape[1]} query heads are no multiple of {H} kv-heads")
-    if not 1 <= q.shape[2] <= T:
-        raise ValueError(f"{what}: {q.shape[2]} query tokens, {T} tokens cached")
-    return q if q.stride(3) == 1 else q.contiguous()
+    _, Hq, S, _ = shape
+    if Hq == 0 or Hq % st.H:
+        raise ValueError(f"{what}: {Hq} query heads are no multiple of {st.H} kv-heads")
+    if not 1 <= S <= T:
+        raise ValueError(f"{what}: {S} query tokens, {T} tokens cached")
+    strides = q.stride()
+    if strides[3] != 1:
+        q = q.contiguous()
+        strides = q.stride()
+    return q, dt, Hq, S, strides
 
 
 def _check_starts(starts, B: int, device, what: str):
@@ -156,23 +167,32 @@ class BlockIndex:
         if self.covered != self.cache.offset or self.cache.store is not self._store or self.covered == 0:
             self.update()
         st, T = self._store, self.covered
-        q = _check_queries(queries, st.B, st.H, st.D, T, st.device, "select")
+        q, dt, Hq, S, (sb, sh, sq, _) = _check_queries(queries, st, T, "select")
         starts = _check_starts(starts, st.B, st.device, "select")
-        B, Hq, S, D = q.shape
-        sb, sh, sq, _ = q.stride()
-        L = _lib.lib()
-        need = ctypes.c_size_t(0)
-        _lib.check(L.cq_block_select_workspace(B, st.H, S, T, self.block_tokens, ctypes.byref(need)), "select")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=st.device)
-        blocks = torch.empty((B, st.H, S, top), dtype=torch.int32, device=st.device)
-        scores = torch.empty((B, st.H, S, top), dtype=torch.float32, device=st.device) if return_scores else None
+        B, H, bt = st.B, st.H, self.block_tokens
+        row = -(-T // bt) + 7 & ~7  # a score row: cq_block_select_workspace, without the call
+        ws = q.new_empty((B * H * S * row,), dtype=torch.float32)
+        blocks = q.new_empty((B, H, S, top), dtype=torch.int32)
+        scores = torch.empty_like(blocks, dtype=torch.float32) if return_scores else None
         with on_device(st.device):
-            _lib.check(L.cq_block_select(self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[2],
-                                         self.block_tokens, B, st.H, D, T, None, q.data_ptr(), cq_dtype(q), Hq, S, sb,
-                                         sh, sq, None if starts is None else starts.data_ptr(), first, recent, top,
-                                         blocks.data_ptr(), None if scores is None else scores.data_ptr(),
-                                         ws.data_ptr(), need.value, stream_ptr(st.device)), "select")
+            _lib.check(_lib.lib().cq_block_select(
+                self.codes.data_ptr(), self.scales.data_ptr(), self.codes.shape[2], bt, B, H, st.D, T, None,
+                q.data_ptr(), dt, Hq, S, sb, sh, sq, None if starts is None else starts.data_ptr(), first, recent, top,
+                blocks.data_ptr(), None if scores is None else scores.data_ptr(), ws.data_ptr(), ws.numel() * 4,
+                stream_ptr(st.device)), "select")
         return (blocks, scores) if return_scores else blocks
+
+
+def _attention_workspace(st, d, T: int, Hq: int, S: int, top: int, bt: int) -> int:
+    """cq_sparse_attention_workspace, kept per store: it depends on these numbers and the store's layout alone."""
+    sizes = st.__dict__.setdefault("_sparse_ws", {})
+    need = sizes.get((Hq, S, top, bt))
+    if need is None:
+        n = ctypes.c_size_t(0)
+        _lib.check(_lib.lib().cq_sparse_attention_workspace(d, T, Hq, S, top, bt, ctypes.byref(n)),
+                   "chronoquant_sparse_sdpa")
+        need = sizes[Hq, S, top, bt] = n.value
+    return need
 
 
 @traced("cq.sparse_sdpa")
@@ -187,33 +207,34 @@ def chronoquant_sparse_sdpa(queries: torch.Tensor, cache, scale: float, blocks: 
     st, T = cache.store, cache.offset
     if st is None or T == 0:
         raise ValueError("chronoquant_sparse_sdpa: the cache is empty")
-    q = _check_queries(queries, st.B, st.H, st.D, T, st.device, "chronoquant_sparse_sdpa")
-    B, Hq, S, D = q.shape
-    if blocks.dim() != 4 or blocks.shape[:3] != (B, st.H, S) or blocks.dtype != torch.int32:
-        raise ValueError(f"chronoquant_sparse_sdpa: blocks must be int32 [{B}, {st.H}, {S}, n], got {blocks.dtype} "
-                         f"{tuple(blocks.shape)}")
-    if blocks.device != st.device:
-        raise ValueError(f"chronoquant_sparse_sdpa: blocks on {blocks.device}, the cache on {st.device}")
-    if not 1 <= blocks.shape[3] <= MAX_TOP:
-        raise ValueError(f"chronoquant_sparse_sdpa: lists of 1 to {MAX_TOP} blocks, got {blocks.shape[3]}")
+    q, dt, Hq, S, (sb, sh, sq, _) = _check_queries(queries, st, T, "chronoquant_sparse_sdpa")
+    B, H, dev = st.B, st.H, st.device
+    shape = blocks.shape
+    if len(shape) != 4 or shape[0] != B or shape[1] != H or shape[2] != S or blocks.dtype != torch.int32:
+        raise ValueError(f"chronoquant_sparse_sdpa: blocks must be int32 [{B}, {H}, {S}, n], got {blocks.dtype} "
+                         f"{tuple(shape)}")
+    if blocks.device != dev:
+        raise ValueError(f"chronoquant_sparse_sdpa: blocks on {blocks.device}, the cache on {dev}")
+    top = shape[3]
+    if not 1 <= top <= MAX_TOP:
+        raise ValueError(f"chronoquant_sparse_sdpa: lists of 1 to {MAX_TOP} blocks, got {top}")
     if int(block_tokens) < 16 or int(block_tokens) % 16:
         raise ValueError(f"block_tokens must be a positive multiple of 16, got {block_tokens}")
-    starts = _check_starts(starts, B, st.device, "chronoquant_sparse_sdpa")
+    starts = _check_starts(starts, B, dev, "chronoquant_sparse_sdpa")
     if not blocks.is_contiguous():
         blocks = blocks.contiguous()
-    top = blocks.shape[3]
-    sb, sh, sq, _ = q.stride()
-    L, d = _lib.lib(), ctypes.byref(st.descriptor())
-    out = torch.empty((B, Hq, S, D), dtype=torch.float32 if return_lse else q.dtype, device=st.device)
-    lse = torch.empty((B, Hq, S), dtype=torch.float32, device=st.device) if return_lse else None
-    with on_device(st.device):
-        need = ctypes.c_size_t(0)
-        _lib.check(L.cq_sparse_attention_workspace(d, T, Hq, S, top, block_tokens, ctypes.byref(need)),
-                   "chronoquant_sparse_sdpa")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=st.device)
-        _lib.check(L.cq_sparse_attention(d, T, None, q.data_ptr(), cq_dtype(q), Hq, S, sb, sh, sq, float(scale),
-                                         None if starts is None else starts.data_ptr(), blocks.data_ptr(), top,
-                                         block_tokens, out.data_ptr(), cq_dtype(out),
-                                         None if lse is None else lse.data_ptr(), ws.data_ptr(), need.value,
-                                         stream_ptr(st.device)), "chronoquant_sparse_sdpa")
+    d = ctypes.byref(st.descriptor())
+    if return_lse:
+        out = q.new_empty((B, Hq, S, st.D), dtype=torch.float32)
+        lse = q.new_empty((B, Hq, S), dtype=torch.float32)
+    else:
+        out, lse = q.new_empty((B, Hq, S, st.D)), None
+    with on_device(dev):
+        need = _attention_workspace(st, d, T, Hq, S, top, block_tokens)
+        ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+        _lib.check(_lib.lib().cq_sparse_attention(
+            d, T, None, q.data_ptr(), dt, Hq, S, sb, sh, sq, float(scale), None if starts is None else
+            starts.data_ptr(), blocks.data_ptr(), top, block_tokens, out.data_ptr(), _lib.CQ_F32 if return_lse else dt,
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need, stream_ptr(dev)),
+            "chronoquant_sparse_sdpa")
     return (out, lse) if return_lse else out
