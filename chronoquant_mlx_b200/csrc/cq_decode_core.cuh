@@ -92,12 +92,6 @@ __device__ __forceinline__ float q_scaled(const QuerySrc &s, int g, int d) {
 
 // Loads a unit's query: K-code-order fragments into registers, natural-order
 // fragments (for the anchors) into the warp's table qn[8][32 lanes] (uint2).
-//
-// RAW: K codes enter the score MMAs as 1024 + n and 1024 + 16n (fewest
-// operations; the sums reach 1032 sum|q|, whose fp32 rounding shows in the
-// scores); otherwise as 64 + n = code + 72 (two shifts more per word, sums of
-// at most 79 sum|q|, a 13 times smaller error).
-template <bool RAW = true>
 __device__ __forceinline__ void load_q(const QuerySrc &p, int lane, QFrag &f, uint2 *qn) {
   const int g = lane >> 2, t = lane & 3;
   const bool real = g < p.gqa;
@@ -108,14 +102,14 @@ __device__ __forceinline__ void load_q(const QuerySrc &p, int lane, QFrag &f, ui
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = real ? q_scaled(p, g, d0 + i) : 0.f;
-    constexpr float hi = RAW ? 0.0625f : 1.f;
-    constexpr uint32_t c0 = RAW ? ptx::RAW_CODE0_LO : ptx::HALF2_72, c1 = RAW ? ptx::RAW_CODE0_HI : ptx::HALF2_72;
     f.qb[J][0] = ptx::pack_half2(v[0], v[4]);
-    f.qb[J][1] = ptx::pack_half2(v[1] * hi, v[5] * hi);
+    f.qb[J][1] = ptx::pack_half2(v[1] * 0.0625f, v[5] * 0.0625f);
     f.qb[J][2] = ptx::pack_half2(v[2], v[6]);
-    f.qb[J][3] = ptx::pack_half2(v[3] * hi, v[7] * hi);
-    ptx::mma_f16_16816(cc, c0, c0, c1, c1, f.qb[J][0], f.qb[J][1]);
-    ptx::mma_f16_16816(cc, c0, c0, c1, c1, f.qb[J][2], f.qb[J][3]);
+    f.qb[J][3] = ptx::pack_half2(v[3] * 0.0625f, v[7] * 0.0625f);
+    ptx::mma_f16_16816(cc, ptx::RAW_CODE0_LO, ptx::RAW_CODE0_LO, ptx::RAW_CODE0_HI, ptx::RAW_CODE0_HI, f.qb[J][0],
+                       f.qb[J][1]);
+    ptx::mma_f16_16816(cc, ptx::RAW_CODE0_LO, ptx::RAW_CODE0_LO, ptx::RAW_CODE0_HI, ptx::RAW_CODE0_HI, f.qb[J][2],
+                       f.qb[J][3]);
   }
   f.qc = make_float2(cc[0], cc[1]);
 #pragma unroll
@@ -130,7 +124,9 @@ __device__ __forceinline__ void load_q(const QuerySrc &p, int lane, QFrag &f, ui
 
 // q . anchor (log2 units) for the first nK (<= 16) K anchors of a slot, as
 // one MMA tile with rows = anchors; table [16][8] fp32 at `qa`.
-__device__ __forceinline__ void compute_qa(uint32_t kfK, float *qa, int nK, const uint2 *qn, int lane) {
+// frag(kk): the query's B fragment of channels 16 kk .. 16 kk + 15.
+template <class Frag>
+__device__ __forceinline__ void compute_qa_from(uint32_t kfK, float *qa, int nK, Frag frag, int lane) {
   const int g = lane >> 2, t = lane & 3;
   const int mi = lane >> 3, rr = lane & 7;
   float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -141,13 +137,72 @@ __device__ __forceinline__ void compute_qa(uint32_t kfK, float *qa, int nK, cons
     uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
     ptx::ldmatrix_x4(a0, a1, a2, a3, base + kk * 32);
     ptx::ldmatrix_x4(b0, b1, b2, b3, base + kk * 32 + 32);
-    const uint2 q0 = qn[kk * 32 + lane], q1 = qn[(kk + 1) * 32 + lane];
+    const uint2 q0 = frag(kk), q1 = frag(kk + 1);
     ptx::mma_f16_16816(c0, a0, a1, a2, a3, q0.x, q0.y);
     ptx::mma_f16_16816(c1, b0, b1, b2, b3, q1.x, q1.y);
   }
   float *row0 = qa + g * 8 + 2 * t;
   *(float2 *)row0 = make_float2((c0[0] + c1[0]) * LOG2E, (c0[1] + c1[1]) * LOG2E);
   *(float2 *)(row0 + 64) = make_float2((c0[2] + c1[2]) * LOG2E, (c0[3] + c1[3]) * LOG2E);
+}
+
+__device__ __forceinline__ void compute_qa(uint32_t kfK, float *qa, int nK, const uint2 *qn, int lane) {
+  compute_qa_from(kfK, qa, nK, [&](int kk) { return qn[kk * 32 + lane]; }, lane);
+}
+
+// A query kept as a tile in shared memory instead: fp16 [8 heads][kQRow bytes],
+// rows 16 bytes apart modulo 128, from which fragments are read without bank
+// conflicts.  It is filled with 8-byte loads where the rows allow them.
+constexpr int kQRow = HD * 2 + 16, kQTileBytes = 8 * kQRow;
+
+__device__ __forceinline__ void load_q_tile(const QuerySrc &p, int lane, QFrag &f, unsigned char *tile) {
+  const bool quads = (((uintptr_t)p.q & 7) | (p.base & 3) | (p.sh & 3)) == 0;
+  const float sc = round_dt(p.scale, p.dtype);
+  uint2 raw[8];
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    raw[g] = make_uint2(0u, 0u);
+    if (g < p.gqa) {
+      const uint16_t *src = (const uint16_t *)p.q + p.base + g * p.sh + 4 * lane;
+      if (quads)
+        raw[g] = *(const uint2 *)src;
+      else
+        raw[g] = make_uint2((uint32_t)src[0] | (uint32_t)src[1] << 16, (uint32_t)src[2] | (uint32_t)src[3] << 16);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint16_t u = (uint16_t)((i & 2 ? raw[g].y : raw[g].x) >> (i & 1 ? 16 : 0));
+      const float x = p.dtype == CQ_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
+      v[i] = round_dt(x * sc, p.dtype);  // q * scale in the query dtype (attention.py:46)
+    }
+    *(uint2 *)(tile + g * kQRow + 8 * lane) = make_uint2(ptx::pack_half2(v[0], v[1]), ptx::pack_half2(v[2], v[3]));
+  }
+  __syncwarp();
+  const int g = lane >> 2, t = lane & 3;
+  float cc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int J = 0; J < 4; ++J) {  // the K-code order, as load_q<false>
+    const uint4 w = *(const uint4 *)(tile + g * kQRow + 64 * t + 16 * J);
+    f.qb[J][0] = __byte_perm(w.x, w.z, 0x5410u);
+    f.qb[J][1] = __byte_perm(w.x, w.z, 0x7632u);
+    f.qb[J][2] = __byte_perm(w.y, w.w, 0x5410u);
+    f.qb[J][3] = __byte_perm(w.y, w.w, 0x7632u);
+    ptx::mma_f16_16816(cc, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, f.qb[J][0], f.qb[J][1]);
+    ptx::mma_f16_16816(cc, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, f.qb[J][2], f.qb[J][3]);
+  }
+  f.qc = make_float2(cc[0], cc[1]);
+}
+
+__device__ __forceinline__ void compute_qa_tile(uint32_t kfK, float *qa, int nK, const unsigned char *tile, int lane) {
+  const unsigned char *at = tile + (lane >> 2) * kQRow + 4 * (lane & 3);
+  compute_qa_from(
+      kfK, qa, nK,
+      [&](int kk) { return make_uint2(*(const uint32_t *)(at + 32 * kk), *(const uint32_t *)(at + 32 * kk + 16)); },
+      lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -222,7 +277,10 @@ __device__ __forceinline__ float lds_half_as_float(uint32_t a) {
 // factor for head g in `fh` (for the P of the chunk's earlier groups).
 // MASK: 0 every token of the chunk counts, 1 tokens below nvalid, 2 tokens
 // from vlo on and below nvalid (one of this group's at least).
-// RAW: as load_q's.
+// RAW: K codes enter the score MMAs as 1024 + n and 1024 + 16n (load_q's
+// fragments: fewest operations; the sums reach 1032 sum|q|, whose fp32 rounding
+// shows in the scores); otherwise as 64 + n = code + 72 (load_q_tile's: two
+// shifts more per word, sums of at most 79 sum|q|, a 13 times smaller error).
 template <class G, int MASK, bool RAW = true>
 __device__ __forceinline__ bool k_group(WarpState &st, const KAddr &A, const QFrag &f, int t0, int nvalid, int lane,
                                         uint2 (&bp)[2], __half2 &fh, int vlo = 0) {

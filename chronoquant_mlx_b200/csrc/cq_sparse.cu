@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "cq_prefill.cuh"
+#include "cq_ptx.cuh"
 #include "cq_sparse.cuh"
 
 namespace cq {
@@ -49,20 +50,21 @@ __device__ __forceinline__ float key_f16(const TokLoc &L, int d, int D, int orde
   return __half2float(__hadd_rn(a, __hmul_rn(__int2half_rn(code), __float2half_rn(L.scale))));
 }
 
-// The least whole number c with c * s >= x (s > 0, |x| <= 126 s up to
-// rounding): the rounded quotient, corrected by the exact sign of x - c * s.
-__device__ __forceinline__ float ceil_code(float x, float s) {
-  const float c = rintf(__fdiv_rn(x, s));
+// The least whole number c with c * s >= x (s > 0, |x| <= 126 s up to rounding;
+// r about 1 / s): rint(x * r) is one of the two whole numbers next to x / s, and
+// the exact sign of x - c * s tells which.
+__device__ __forceinline__ float ceil_code(float x, float s, float r) {
+  const float c = rintf(x * r);
   return fmaf(-c, s, x) > 0.f ? c + 1.f : c;
 }
 
-// One block's codes and scale from the per-channel range held by `threads`
-// threads (channel d of thread d); amax: the block's largest |x|.
+// One channel's codes from its range; s: the block's scale (max|x| / 126).
 __device__ __forceinline__ void store_codes(int8_t *codes, int d, int D, float lo, float hi, float s) {
   float l = 0.f, h = 0.f;
   if (s > 0.f) {
-    h = ceil_code(hi, s);
-    l = -ceil_code(-lo, s);
+    const float r = 1.f / s;
+    h = ceil_code(hi, s, r);
+    l = -ceil_code(-lo, s, r);
   }
   codes[d] = (int8_t)fminf(fmaxf(l, -127.f), 127.f);
   codes[D + d] = (int8_t)fminf(fmaxf(h, -127.f), 127.f);
@@ -121,7 +123,7 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
 // is 0, so whatever its row reads (the row before it, inside the chunk block)
 // becomes the anchor itself (the chunk's first token reads row 0).
 template <int D>
-__global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, int64_t n_warps) {
+__global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, unsigned n_warps) {
   constexpr int LPR = D / 32, RPI = 32 / LPR;  // lanes per row, rows at once
   constexpr int W = D / 8;                     // words of a code row
   const int lane = threadIdx.x & 31;
@@ -136,29 +138,33 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, in
     }
     t0 = T - A.S;
   }
-  const int64_t wi = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  // positions in 32 bits (the launch keeps them there): 64-bit divisions cost as much as a chunk's codes
+  const unsigned wi = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (wi >= n_warps) return;
-  const int64_t unit = wi / A.nb, j = t0 / A.bt + (wi - unit * A.nb);
-  const int64_t ta = j * A.bt, tb = min(T, ta + A.bt);
-  if (ta >= T) return;
-  const int b = (int)(unit / cv.H), h = (int)(unit - (int64_t)b * cv.H);
+  const unsigned unit = wi / (unsigned)A.nb;
+  const int j = (int)((unsigned)t0 / (unsigned)A.bt + (wi - unit * (unsigned)A.nb));
+  const int ta = j * A.bt, tb = (int)min((unsigned)T, (unsigned)ta + (unsigned)A.bt);
+  if (ta >= (int)T) return;
+  const int b = (int)(unit / (unsigned)cv.H), h = (int)(unit - (unsigned)b * cv.H);
   const int row = lane / LPR, part = lane % LPR;  // which of the rows at once, which 32 channels
   const __half2 inf = __float2half2_rn(INFINITY);
   __half2 lo[16], hi[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) lo[k] = inf, hi[k] = __hneg2(inf);
 
-  int64_t t = ta;
+  const int ct = c.pc + c.ac;  // tokens per chunk
+  int t = ta;
   while (t < tb) {  // one anchor's tokens at a time: they lie in one chunk of one page
-    const int64_t lp = t / cv.P;
-    const int tl = (int)(t - lp * cv.P);
-    const int a = tl / c.stride;
-    const int64_t te = min(tb, t - (tl - a * c.stride) + c.stride);
+    const int lp = (int)((unsigned)t / (unsigned)cv.P);
+    const int tl = t - lp * cv.P;
+    const int a = (int)((unsigned)tl / (unsigned)c.stride);
+    const int te = min(tb, t - (tl - a * c.stride) + c.stride);
     const int64_t pg = page_of(cv, b, lp);
-    const int ct = c.pc + c.ac, jc = tl / ct, x0 = tl - jc * ct;  // chunk, position in it
-    const __half *arow = c.kf + kf_index(c, cv.H, D, pg, h, a) + part * 32;
+    const int jc = (int)((unsigned)tl / (unsigned)ct), x0 = tl - jc * ct;  // chunk, position in it
+    const int xa = (int)((unsigned)x0 / (unsigned)c.stride);               // its anchor in the chunk
+    const __half *arow = c.kf + (pg * cv.H + h) * c.kf_hs + jc * c.kf_cs + xa * D + part * 32;
     const uint32_t *crow = c.codes + (pg * cv.H + h) * c.cd_hs + jc * c.cd_cs + part * 4;
-    const int i0 = x0 - x0 / c.stride - 1 + row;  // this lane's first code row
+    const int i0 = x0 - xa - 1 + row;  // this lane's first code row
     const __half *sc = c.scales + (pg * cv.H + h) * c.sc_hs + jc * c.sc_cs + x0 + row;
     // the anchor's channels in the code words' pairs: (d, d + 4) of each 8
     __half2 an[16];
@@ -172,7 +178,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, in
         an[4 * w + k] = *(const __half2 *)&pr;
       }
     }
-    const int n = (int)(te - t);
+    const int n = te - t;
     for (int r0 = 0; r0 < n; r0 += 2 * RPI) {
       uint4 code[2];
       __half s1[2];
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, in
   }
   amax = warp_max(amax);
   const float s = __fdiv_rn(amax, 126.f);
-  const int64_t at = unit * A.max_blocks + j;
+  const int64_t at = (int64_t)unit * A.max_blocks + j;
   int8_t *codes = A.codes + at * 2 * D;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
@@ -316,64 +322,79 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
 // A lane loads 16 bytes of a block at a time; the order of the sum's terms is
 // permuted alike in both operands, so these are two steps' B fragments as they
 // come.  A CTA quantises `tiles` row tiles into shared memory once (rows 64
-// bytes apart modulo 128: no bank conflicts), then each warp keeps the codes of
-// two column tiles in registers and passes over the rows.
+// bytes apart modulo 128: no bank conflicts), then each warp takes columns in
+// `passes`, keeping two column tiles' codes in registers over the rows.  The
+// maximum over a group's heads goes by halves: each exchange also halves the
+// values a lane holds, so every lane ends with its own ones to store.
 constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
 
-template <int KS>
-__global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(SelectArgs A, int tiles, int gp, int passes) {
-  constexpr int D = KS * 32, STR = 2 * D + 64;
+template <int KS, int GP>
+__global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(SelectArgs A, int tiles, int passes) {
+  constexpr int D = KS * 32, STR = 2 * D + 64, TPT = 16 / GP;  // query tokens per row tile
   extern __shared__ __align__(16) unsigned char s_a[];  // [tiles * 16][STR], then fp32 [tiles * 16]
   float *s_sg = (float *)(s_a + tiles * 16 * STR);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int tpt = 16 / gp;  // query tokens per row tile
   const int64_t unit = blockIdx.z;
   const int b = (int)(unit / A.H), h = (int)(unit - (int64_t)b * A.H);
-  const int i0 = blockIdx.y * tiles * tpt;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int i0 = blockIdx.y * tiles * TPT;
+  ptx::grid_dependency_wait();
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
   if (T == 0) return;
-  for (int r = warp; r < tiles * 16; r += kScoreWarps) {
-    const int i = i0 + r / gp, hd = r & (gp - 1);
-    const bool real = i < A.q_len && hd < A.G;
-    const int64_t qb = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq;
-    float x[KS], amax = 0.f;
+  // query rows of this warp: r, r + 8, ...; four rows' loads in flight
+  for (int r0 = warp; r0 < tiles * 16; r0 += 4 * kScoreWarps) {
+    float x[4][KS];
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      x[k] = real ? finite_query(load_as_float(A.q, qb + lane * KS + k, A.q_dtype)) : 0.f;
-      amax = fmaxf(amax, fabsf(x[k]));
-    }
-    const QueryScale qs(warp_max(amax));
-    int8_t *row = (int8_t *)s_a + r * STR + lane * KS;
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * kScoreWarps, i = i0 + r / GP, hd = r & (GP - 1);
+      const bool real = r < tiles * 16 && i < A.q_len && hd < A.G;
+      const int64_t qb = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int c = qs.code(x[k]);
-      row[k] = (int8_t)min(c, 0);
-      row[D + k] = (int8_t)max(c, 0);
+      for (int k = 0; k < KS; ++k) x[u][k] = real ? load_as_float(A.q, qb + lane * KS + k, A.q_dtype) : 0.f;
     }
-    if (lane == 0) s_sg[r] = qs.s;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * kScoreWarps;
+      if (r >= tiles * 16) break;
+      float amax = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        x[u][k] = finite_query(x[u][k]);
+        amax = fmaxf(amax, fabsf(x[u][k]));
+      }
+      const QueryScale qs(warp_max(amax));
+      int8_t *row = (int8_t *)s_a + r * STR + lane * KS;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int c = qs.code(x[u][k]);
+        row[k] = (int8_t)min(c, 0);
+        row[D + k] = (int8_t)max(c, 0);
+      }
+      if (lane == 0) s_sg[r] = qs.s;
+    }
   }
   __syncthreads();
   // the last block any of this CTA's tokens sees
-  const int i_last = min(A.q_len, i0 + tiles * tpt) - 1;
-  const int64_t j_end = min(A.n, (T - A.q_len + i_last) / A.bt + 1);
-  const int real_tiles = (i_last - i0) / tpt + 1;
+  const int i_last = min(A.q_len, i0 + tiles * TPT) - 1;
+  const int j_end = (int)min(A.n, (T - A.q_len + i_last) / A.bt + 1);
+  const int real_tiles = (i_last - i0) / TPT + 1;
   const int8_t *codes = A.codes + unit * A.max_blocks * 2 * D;
   const float *scales = A.scales + unit * A.max_blocks;
+  const bool pad0 = (g & (GP - 1)) >= A.G, pad1 = ((g + 8) & (GP - 1)) >= A.G;
   for (int pass = 0; pass < passes; ++pass) {
-    const int64_t j0 = (((int64_t)blockIdx.x * passes + pass) * kScoreWarps + warp) * kScoreCols;
+    const int j0 = (int)((blockIdx.x * passes + pass) * kScoreWarps + warp) * kScoreCols;
     if (j0 >= j_end) break;
     uint4 bf[2][KS];
     float sj[2][2];
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb) {
-      const int8_t *src = codes + min(j0 + nb * 8 + g, A.n - 1) * 2 * D + 16 * t;
+      const int8_t *src = codes + (int64_t)min(j0 + nb * 8 + g, (int)A.n - 1) * 2 * D + 16 * t;
 #pragma unroll
       for (int k = 0; k < KS; ++k) bf[nb][k] = *(const uint4 *)(src + 64 * k);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) sj[nb][e] = scales[min(j0 + nb * 8 + 2 * t + e, A.n - 1)];
+      for (int e = 0; e < 2; ++e) sj[nb][e] = scales[min(j0 + nb * 8 + 2 * t + e, (int)A.n - 1)];
     }
-    for (int rt = 0; rt < real_tiles; ++rt) {
+    float *dst = A.score + (unit * A.q_len + i0) * A.ns + j0;  // of this row tile's first token
+    for (int rt = 0; rt < real_tiles; ++rt, dst += TPT * A.ns) {
       int acc[2][4] = {};
       const unsigned char *a = s_a + (rt * 16 + g) * STR + 16 * t;
 #pragma unroll
@@ -385,31 +406,67 @@ __global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(Selec
           mma_s8_16832(acc[nb], x.z, y.z, x.w, y.w, bf[nb][k].z, bf[nb][k].w);
         }
       }
-      const float sg[2] = {s_sg[rt * 16 + g], s_sg[rt * 16 + g + 8]};
-      const bool pad0 = (g & (gp - 1)) >= A.G, pad1 = ((g + 8) & (gp - 1)) >= A.G;
+      const float sg0 = s_sg[rt * 16 + g], sg1 = s_sg[rt * 16 + g + 8];
+      // v[column tile][row half][column]: scores of rows g and g + 8
+      float v[2][2][2];
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
-        float v[4];
+      for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          v[e] = pad0 ? -INFINITY : __fmul_rn(__fmul_rn(sg[0], sj[nb][e]), (float)acc[nb][e]);
-          v[2 + e] = pad1 ? -INFINITY : __fmul_rn(__fmul_rn(sg[1], sj[nb][e]), (float)acc[nb][2 + e]);
+          const float x = __fmul_rn(__fmul_rn(sg0, sj[nb][e]), (float)acc[nb][e]);
+          const float y = __fmul_rn(__fmul_rn(sg1, sj[nb][e]), (float)acc[nb][2 + e]);
+          v[nb][0][e] = pad0 ? -INFINITY : __fadd_rn(x, 0.f);  // -0 becomes +0: equal scores have equal keys
+          v[nb][1][e] = pad1 ? -INFINITY : __fadd_rn(y, 0.f);
         }
-        if (gp == 16) v[0] = fmaxf(v[0], v[2]), v[1] = fmaxf(v[1], v[3]);
-        for (int o = 4; o < 4 * min(gp, 8); o <<= 1)
+      auto swap_max = [&](float &keep, float give, int o) {
+        keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      };
+      int nb0 = 0, hf0 = 0;  // which of the values this lane holds
+      if constexpr (GP == 16) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = fmaxf(v[e], __shfl_xor_sync(0xffffffffu, v[e], o));
-        if ((g & (min(gp, 8) - 1)) == 0) {
-          const int64_t col = j0 + nb * 8 + 2 * t;
-          const int ia = i0 + rt * tpt + g / gp, ib = ia + 8 / gp;  // the tokens of rows g and g + 8
-          float *dst = A.score + (unit * A.q_len + ia) * A.ns + col;
-          if (col < A.ns) {
-            if (ia < A.q_len) *(float2 *)dst = make_float2(__fadd_rn(v[0], 0.f), __fadd_rn(v[1], 0.f));
-            if (gp < 16 && ib < A.q_len)
-              *(float2 *)(dst + (int64_t)(8 / gp) * A.ns) = make_float2(__fadd_rn(v[2], 0.f), __fadd_rn(v[3], 0.f));
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) v[nb][0][e] = fmaxf(v[nb][0][e], v[nb][1][e]);
+      }
+      if constexpr (GP >= 2) {  // heads in lane bit 2: keep one column tile
+        nb0 = g & 1;
+#pragma unroll
+        for (int hf = 0; hf < (GP == 16 ? 1 : 2); ++hf)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float a0 = v[0][hf][e], a1 = v[1][hf][e];
+            v[0][hf][e] = nb0 ? a1 : a0;
+            swap_max(v[0][hf][e], nb0 ? a0 : a1, 4);
           }
+      }
+      if constexpr (GP == 4 || GP == 8) {  // heads in lane bit 3: keep one row half
+        hf0 = (g >> 1) & 1;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float a0 = v[0][0][e], a1 = v[0][1][e];
+          v[0][0][e] = hf0 ? a1 : a0;
+          swap_max(v[0][0][e], hf0 ? a0 : a1, 8);
         }
       }
+      if constexpr (GP == 16)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 8));
+      if constexpr (GP >= 8)  // heads in lane bit 4
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 16));
+      // token (in the tile) of the lane's row g, and of row g + 8: 8 / GP further on
+      const int ta = g / GP, i = i0 + rt * TPT;
+      constexpr int NBV = GP >= 2 ? 1 : 2, HFV = GP == 1 || GP == 2 ? 2 : 1;
+#pragma unroll
+      for (int nb = 0; nb < NBV; ++nb)
+#pragma unroll
+        for (int hf = 0; hf < HFV; ++hf) {
+          const int tok = ta + (HFV == 2 ? hf : hf0) * (8 / GP), col = (NBV == 2 ? nb : nb0) * 8 + 2 * t;
+          bool mine = i + tok < A.q_len && j0 + col < (int)A.ns;
+          if (GP >= 8) mine = mine && !(g & 4);
+          if (GP == 16) mine = mine && !(g & 2);
+          if (mine) *(float2 *)(dst + tok * A.ns + col) = make_float2(v[nb][hf][0], v[nb][hf][1]);
+        }
     }
   }
 }
@@ -456,35 +513,78 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 }
 
 // The `top` best visible blocks of a (unit, query token) row with every key in a
-// register: W warps hold KPT keys a thread.  The key of the last block taken is
-// found bit by bit (counts of keys at or above a candidate), and stops early
-// where a candidate has exactly `top`; the list is written in index order, of
-// equal keys the lowest indexes.
+// register: W warps hold KPT keys a thread.  The threshold key is found bit by
+// bit from the highest one on which the row's keys differ (a candidate holds if
+// at least `top` keys reach it).  As soon as no more than kShort keys reach the
+// threshold so far they are gathered in index order in shared memory, and one
+// warp goes on with those alone; where that never happens (long lists, many
+// equal keys) the search runs to the last bit over the registers.  The list is
+// written in index order, of equal keys the lowest indexes.
+constexpr int kShort = 256;
+
+// Exclusive prefix of `n` (at most 32 * PER) packed counts in shared memory, in
+// place, by one warp; returns the sum.
+template <int PER>
+__device__ __forceinline__ int warp_prefix(int *v, int n, int lane) {
+  int sum = 0;
+#pragma unroll
+  for (int e = 0; e < PER; ++e)
+    if (lane * PER + e < n) sum += v[lane * PER + e];
+  int before = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  const int all = __shfl_sync(0xffffffffu, before, 31);
+  before -= sum;
+#pragma unroll
+  for (int e = 0; e < PER; ++e)
+    if (lane * PER + e < n) {
+      const int x = v[lane * PER + e];
+      v[lane * PER + e] = before;
+      before += x;
+    }
+  return all;
+}
+
 template <int KPT, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W, int64_t rows) {
+__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
+  __shared__ uint32_t s_key[kShort];
+  __shared__ int s_idx[kShort];
   __shared__ int s_cnt[2][32];
   __shared__ int s_pre[KPT * 32];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  ptx::grid_dependency_wait();
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
-  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
-  const int64_t row = W == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   if (T == 0) {
     if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
     return;
   }
-  if (row >= rows) return;  // whole CTAs, or single warps that never meet others
   const int i = (int)(row % A.q_len);
   const int b = (int)(row / ((int64_t)A.q_len * A.H));
   const int64_t p = T - A.q_len + i, st = first_token(A.starts, b);
   const int fb = (int)min(st / A.bt, (int64_t)INT32_MAX), lb = (int)(p / A.bt);
   const int nv = st > p ? 0 : lb - fb + 1;
   const float *score = A.score + row * A.ns;
+  int32_t *out = A.blocks + row * A.top;
+  float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
   const int tid = warp * 32 + lane, step = W * 32;
+  for (int k = min(nv, A.top) + tid; k < A.top; k += step) {
+    out[k] = -1;
+    if (out_s) out_s[k] = -INFINITY;
+  }
   uint32_t key[KPT];  // 0: no block (visible ones are above it)
+  uint32_t all_or = 0, all_and = 0xffffffffu;
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
     const int x = k * step + tid;
     key[k] = x >= nv ? 0u : (x < A.first || x >= nv - A.recent) ? 0xffffffffu : order_key(score[fb + x]);
+    if (key[k] != 0u && key[k] != 0xffffffffu) {
+      all_or |= key[k];
+      all_and &= key[k];
+    }
   }
   int par = 0;
   auto total = [&](int c) {  // over the row's threads
@@ -497,19 +597,95 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     return c;
   };
   uint32_t thr = 1;  // keys at or above it are taken, those equal to it from the lowest index on
+  int reach = nv;    // keys that reach it
+  int bit = -1;
   if (nv > A.top) {
-    thr = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    // the bits above the highest differing one are those of every key that is not forced
+    all_or = __reduce_or_sync(0xffffffffu, all_or);
+    all_and = __reduce_and_sync(0xffffffffu, all_and);
+    if (W > 1) {
+      if (lane == 0) s_pre[warp] = (int)all_or, s_cnt[0][warp] = (int)all_and;
+      __syncthreads();
+      all_or = __reduce_or_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[lane] : 0u);
+      all_and = __reduce_and_sync(0xffffffffu, lane < W ? (uint32_t)s_cnt[0][lane] : 0xffffffffu);
+      __syncthreads();
+    }
+    const uint32_t differ = all_or & ~all_and;  // first + recent <= top < nv: some key is not forced
+    bit = differ ? 31 - __clz(differ) : -1;
+    thr = bit < 0 ? all_and : all_and & ~((2u << bit) - 1u);
+    const bool shorten = A.top <= kShort;
+    for (; bit >= 0 && reach != A.top && !(shorten && reach <= kShort); --bit) {
       const uint32_t cand = thr | (1u << bit);
       int c = 0;
 #pragma unroll
       for (int k = 0; k < KPT; ++k) c += key[k] >= cand;
       c = total(c);
-      if (c >= A.top) thr = cand;
-      if (c == A.top) break;
+      if (c >= A.top) thr = cand, reach = c;
     }
   }
-  // per key slot k and warp: keys above the threshold (low half) and equal to it (high half)
+  if (reach <= kShort && reach > 0) {  // gather the keys that reach the threshold, in index order
+    int running = 0;
+    if (W > 1) {
+#pragma unroll
+      for (int k = 0; k < KPT; ++k) {
+        const unsigned in = __ballot_sync(0xffffffffu, key[k] >= max(thr, 1u));
+        if (lane == 0) s_pre[k * W + warp] = __popc(in);
+      }
+      __syncthreads();
+      if (warp == 0) warp_prefix<KPT>(s_pre, KPT * W, lane);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const bool in = key[k] >= max(thr, 1u);
+      const unsigned m = __ballot_sync(0xffffffffu, in);
+      const int at = (W > 1 ? s_pre[k * W + warp] : running) + __popc(m & ((1u << lane) - 1u));
+      running += __popc(m);
+      if (in) {
+        s_key[at] = key[k];
+        s_idx[at] = fb + k * step + tid;
+      }
+    }
+    if (W > 1)
+      __syncthreads();
+    else
+      __syncwarp();
+    if (warp != 0) return;
+    constexpr int N = kShort / 32;
+    uint32_t kk[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) kk[k] = k * 32 + lane < reach ? s_key[k * 32 + lane] : 0u;
+    for (; bit >= 0 && reach > A.top; --bit) {
+      const uint32_t cand = thr | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) c += kk[k] >= cand;
+      c = __reduce_add_sync(0xffffffffu, c);
+      if (c >= A.top) thr = cand, reach = c;
+    }
+    // reach > top now means equal keys at the threshold: the lowest indexes of them
+    int gt_all = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) gt_all += __popc(__ballot_sync(0xffffffffu, kk[k] > thr));
+    const int need = reach > A.top ? A.top - gt_all : kShort;
+    int gt_run = 0, eq_run = 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const bool gt = kk[k] > thr, eq = kk[k] == thr;
+      const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+      const unsigned below = (1u << lane) - 1u;
+      const int e0 = eq_run + __popc(be & below);
+      if (gt || (eq && e0 < need)) {
+        const int at = gt_run + __popc(bg & below) + min(e0, need), j = s_idx[k * 32 + lane];
+        out[at] = j;
+        if (out_s) out_s[at] = score[j];
+      }
+      gt_run += __popc(bg);
+      eq_run += __popc(be);
+    }
+    return;
+  }
+  // the rest from the registers: per key slot k and warp, keys above the threshold (low half) and equal to it (high)
   int mine = 0, all_gt = 0;
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
@@ -522,38 +698,17 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     }
     all_gt += __popc(gt);
   }
-  int running = 0;
   if (W > 1) {
     __syncthreads();
-    if (warp == 0) {  // exclusive prefix in index order: KPT * W <= KPT * 32 entries
-      int sum = 0;
-      for (int e = 0; e < KPT; ++e) {
-        const int at = lane * KPT + e;
-        if (at < KPT * W) sum += s_pre[at];
-      }
-      int before = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
-      }
-      if (lane == 31) s_cnt[0][0] = before;
-      before -= sum;
-      for (int e = 0; e < KPT; ++e) {
-        const int at = lane * KPT + e;
-        if (at < KPT * W) {
-          const int x = s_pre[at];
-          s_pre[at] = before;
-          before += x;
-        }
-      }
+    if (warp == 0) {
+      const int all = warp_prefix<KPT>(s_pre, KPT * W, lane);
+      if (lane == 0) s_cnt[0][0] = all;
     }
     __syncthreads();
     all_gt = s_cnt[0][0] & 0xffff;
   }
   const int need = A.top - all_gt;  // equal keys to take
-  int32_t *out = A.blocks + row * A.top;
-  float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
+  int running = 0;
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
     const bool gt = key[k] > thr, eq = key[k] == thr;
@@ -567,10 +722,6 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
       if (out_s) out_s[at] = score[j];
     }
     if (W == 1) running += __shfl_sync(0xffffffffu, mine, k);
-  }
-  for (int k = min(nv, A.top) + tid; k < A.top; k += step) {
-    out[k] = -1;
-    if (out_s) out_s[k] = -INFINITY;
   }
 }
 
@@ -819,11 +970,11 @@ static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const cha
   const int D = A.cv.D, rows = D == 64 ? 16 : D == 128 ? 8 : 4;  // code rows a warp takes at once
   if ((D == 64 || D == 128 || D == 256) && c.order == CQ_ORDER_NATURAL && c.stok && c.stride % rows == 0 &&
       c.stride > 1 && A.bt % rows == 0 && aligned16(c.codes) && aligned16(c.kf) && (c.cd_hs | c.cd_cs) % 4 == 0 &&
-      (c.kf_hs | c.kf_cs) % 8 == 0) {
+      (c.kf_hs | c.kf_cs) % 8 == 0 && A.T + A.bt < (1LL << 31)) {
     auto *fn = D == 64    ? sparse::block_bounds_rows_kernel<64>
                : D == 128 ? sparse::block_bounds_rows_kernel<128>
                           : sparse::block_bounds_rows_kernel<256>;
-    fn<<<(unsigned)((grid + 3) / 4), 128, 0, st>>>(A, grid);
+    fn<<<(unsigned)((grid + 3) / 4), 128, 0, st>>>(A, (unsigned)grid);
     return check_launch(what);
   }
   const int threads = (A.cv.D + 31) & ~31;
@@ -903,26 +1054,30 @@ static int launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, c
 static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
   using namespace sparse;
   const int64_t rows = (int64_t)A.B * A.H * A.q_len, units = (int64_t)A.B * A.H;
-  void (*fn)(SelectArgs, int, int, int) = A.D == 64    ? block_score_mma_kernel<2>
-                                          : A.D == 96  ? block_score_mma_kernel<3>
-                                          : A.D == 128 ? block_score_mma_kernel<4>
-                                          : A.D == 256 ? block_score_mma_kernel<8>
-                                                       : nullptr;
-  if (fn && A.G <= 16 && aligned16(A.codes) && aligned16(A.score) && units < 65536) {
-    int gp = 1;
-    while (gp < A.G) gp *= 2;
-    const int tpt = 16 / gp, row_tiles = (A.q_len + tpt - 1) / tpt;
-    // row tiles per CTA: their quantisation is shared by its columns; 48 KB hold 8 of them up to head size 128
-    const int tiles = std::min(row_tiles, A.D > 128 ? 4 : 8);
+  if ((A.D == 64 || A.D == 96 || A.D == 128 || A.D == 256) && A.G <= 16 && aligned16(A.codes) && aligned16(A.score) &&
+      units < 65536 && A.n < (1LL << 30)) {
+    int lg = 0;
+    while ((1 << lg) < A.G) ++lg;
+    using Fn = void (*)(SelectArgs, int, int);
+#define CQ_SCORE(KS)                                                                                           \
+  {block_score_mma_kernel<KS, 1>, block_score_mma_kernel<KS, 2>, block_score_mma_kernel<KS, 4>,                \
+   block_score_mma_kernel<KS, 8>, block_score_mma_kernel<KS, 16>}
+    static const Fn table[4][5] = {CQ_SCORE(2), CQ_SCORE(3), CQ_SCORE(4), CQ_SCORE(8)};
+#undef CQ_SCORE
+    const Fn fn = table[A.D == 64 ? 0 : A.D == 96 ? 1 : A.D == 128 ? 2 : 3][lg];
+    const int tpt = 16 >> lg, row_tiles = (A.q_len + tpt - 1) / tpt;
+    // A CTA's rows are quantised once for all its columns, so it takes many columns as soon as there are two
+    // CTAs per SM without splitting them; few row tiles, so that this happens early
+    const int tiles = std::min(row_tiles, 4);
     const int64_t groups = (row_tiles + tiles - 1) / tiles;
+    CQ_REQUIRE(groups < 65536, CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
     const int per = kScoreWarps * kScoreCols;
     const int64_t cols = (A.n + per - 1) / per;
-    // several passes per CTA where there are CTAs enough without
-    const int passes = (int)std::max<int64_t>(1, std::min<int64_t>(cols, cols * groups * units / (8 * sm_count())));
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(cols, 2 * sm_count() / (groups * units)));
+    const int passes = (int)((cols + split - 1) / split);
     const dim3 grid((unsigned)((cols + passes - 1) / passes), (unsigned)groups, (unsigned)units);
-    CQ_REQUIRE(groups < 65536, CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
     return launch_after(fn, grid, kScoreWarps * 32, (size_t)tiles * 16 * (2 * A.D + 64 + 4), st, "cq_block_select", A,
-                        tiles, gp, passes);
+                        tiles, passes);
   }
   const int64_t grid = (rows * A.n * 32 + 255) / 256;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many scores");
@@ -933,24 +1088,19 @@ static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
 static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t st) {
   using namespace sparse;
   CQ_REQUIRE(rows < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
-  // a warp per row where rows abound, else several warps with few keys a thread
-  const bool many = rows >= 16 * sm_count() && A.n <= 32 * 32;
-  int kpt = many ? 8 : 4;
-  while (kpt < (many ? 32 : 16) && A.n > (int64_t)kpt * 32 * (many ? 1 : 32)) kpt *= 2;
+  // A CTA per row, four keys a thread; where rows abound eight (up to four warps), whose rounds cost fewer meetings
+  int kpt = rows >= 4 * sm_count() && A.n > 128 ? 8 : 4;
+  while (kpt < 16 && A.n > (int64_t)kpt * 32 * 32) kpt *= 2;
   const int64_t W = (A.n + kpt * 32 - 1) / (kpt * 32);
   if (W > 32) {
     block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
     return check_launch("cq_block_select");
   }
-  void (*fn)(SelectArgs, int, int64_t) = many ? (kpt == 8    ? block_topk_regs_kernel<8, 128>
-                                                 : kpt == 16 ? block_topk_regs_kernel<16, 128>
-                                                             : block_topk_regs_kernel<32, 128>)
-                                              : (kpt == 4   ? block_topk_regs_kernel<4, 1024>
-                                                 : kpt == 8 ? block_topk_regs_kernel<8, 1024>
-                                                            : block_topk_regs_kernel<16, 1024>);
-  const int threads = W == 1 ? 128 : (int)W * 32;
-  const int64_t grid = W == 1 ? (rows + 3) / 4 : rows;
-  return launch_after(fn, dim3((unsigned)grid), threads, 0, st, "cq_block_select", A, (int)W, rows);
+  void (*fn)(SelectArgs, int) = W <= 4 ? (kpt == 4 ? block_topk_regs_kernel<4, 128> : block_topk_regs_kernel<8, 128>)
+                                : kpt == 4 ? block_topk_regs_kernel<4, 1024>
+                                : kpt == 8 ? block_topk_regs_kernel<8, 1024>
+                                           : block_topk_regs_kernel<16, 1024>;
+  return launch_after(fn, dim3((unsigned)rows), (int)W * 32, 0, st, "cq_block_select", A, (int)W);
 }
 
 extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens,

@@ -87,12 +87,12 @@ __device__ __forceinline__ void copy_part(uint32_t buf, uint64_t *bar, const cha
 template <class G, int MASK>
 __device__ __forceinline__ bool sparse_chunk(WarpState &st, const QFrag &f, int vlo, int vhi, unsigned char *region,
                                              uint64_t *bar, int sk, uint32_t ph, const char *next, float *qa,
-                                             const uint2 *qn, int lane) {
+                                             const unsigned char *qt, int lane) {
   constexpr int NG = G::NT / 2;  // 32-token groups
   const uint32_t ra = ptx::smem_u32(region);
   const uint32_t kb = ra + (G::SPLIT ? 0 : sk * G::SLOT), vb = ra + (G::SPLIT ? G::KB : sk * G::SLOT + G::O_KF1);
   if (!ptx::mbar_wait_bounded(&bar[sk], ph, WAIT_BUDGET)) return false;
-  compute_qa(kb + G::O_KF0, qa, MASK ? ((vhi - 1) >> G::LSK) + 1 : G::AK, qn, lane);
+  compute_qa_tile(kb + G::O_KF0, qa, MASK ? ((vhi - 1) >> G::LSK) + 1 : G::AK, qt, lane);
   __syncwarp();
   uint2 bp[NG][2];
   {
@@ -168,7 +168,7 @@ __device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int6
   const int32_t *list = p.blocks + unit * p.top;
   const uint32_t ra = ptx::smem_u32(region);
   float *qa = (float *)(region + G::BUF);
-  uint2 *qn = (uint2 *)(region + G::BUF + kQaBytes);
+  unsigned char *qt = region + G::BUF + kQaBytes;
   WarpState st;
   reset(st);
   QFrag f;
@@ -215,8 +215,9 @@ __device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int6
       }
     }
     if (todo && !have_q) {  // under the first copies' latency
-      load_q<false>(QuerySrc{p.q, b * p.q_sb + (int64_t)h * p.gqa * p.q_sh + i * p.q_sq, p.q_sh, p.q_dtype, p.gqa, p.scale}, lane,
-             f, qn);
+      load_q_tile(QuerySrc{p.q, b * p.q_sb + (int64_t)h * p.gqa * p.q_sh + i * p.q_sq, p.q_sh, p.q_dtype, p.gqa,
+                           p.scale},
+                  lane, f, qt);
       __syncwarp();
       have_q = true;
     }
@@ -226,8 +227,8 @@ __device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int6
       const int lo = __shfl_sync(0xffffffffu, vlo, l), hi = __shfl_sync(0xffffffffu, vhi, l);
       const char *next = take(issue);
       const bool ok = (lo == 0 && hi == G::C)
-                          ? sparse_chunk<G, 0>(st, f, 0, G::C, region, bar, sk, ph, next, qa, qn, lane)
-                          : sparse_chunk<G, 2>(st, f, lo, hi, region, bar, sk, ph, next, qa, qn, lane);
+                          ? sparse_chunk<G, 0>(st, f, 0, G::C, region, bar, sk, ph, next, qa, qt, lane)
+                          : sparse_chunk<G, 2>(st, f, lo, hi, region, bar, sk, ph, next, qa, qt, lane);
       if (!ok) {  // a copy never landed: record it, let what is in flight land (bounded), stop (results invalid)
         atomicExch(&g_sparse_fast_error, ERR_TIMEOUT_FULL);
         for (int k = 0; k < 2; ++k) ptx::mbar_wait_bounded(&bar[k], ph, WAIT_BUDGET);
@@ -247,7 +248,7 @@ __device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int6
 template <class G>
 __global__ void __launch_bounds__(kSW * 32, 2) sparse_kernel(const __grid_constant__ SparseParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  constexpr int kBars = kSW * 4 * 8, kWarpBytes = G::BUF + kQaBytes + kQnBytes;
+  constexpr int kBars = kSW * 4 * 8, kWarpBytes = G::BUF + kQaBytes + kQTileBytes;
   static_assert(G::BUF >= kPartFloats * 4 && kWarpBytes % 16 == 0, "a partial lies in the copy buffers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint64_t *bar = (uint64_t *)smem + warp * 4;
@@ -363,7 +364,7 @@ template <int SK, int SV, int VP = 4>
 static SparseGeo sparse_geo() {
   using G = Geo<SK, SV, VP>;
   return SparseGeo{geo_spec<G>(), sparse_kernel<G>,
-                   kSW * 4 * 8 + kPartFloats * 4 + kSW * (G::BUF + kQaBytes + kQnBytes)};
+                   kSW * 4 * 8 + kPartFloats * 4 + kSW * (G::BUF + kQaBytes + kQTileBytes)};
 }
 
 // The decode kernel's stride pairs and bit-plane formats.
