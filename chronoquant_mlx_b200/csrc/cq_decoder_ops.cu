@@ -125,8 +125,9 @@ __device__ __forceinline__ float2 rope_angle(int64_t p, float inv_freq) {
   // 2 pi as the sum of two doubles: the remainder keeps its digits for any angle below 2^53 turns
   const double hi = 6.283185307179586, lo = 2.4492935982947064e-16;
   const double n = rint(ang * (1.0 / hi));
+  const double r = fma(-n, lo, fma(-n, hi, ang));
   float sn, cs;
-  sincosf((float)fma(-n, lo, fma(-n, hi, ang)), &sn, &cs);
+  sincospif((float)(r * (2.0 / hi)), &sn, &cs);  // of r = pi x: no reduction left to do
   return make_float2(cs, sn);
 }
 
@@ -178,91 +179,131 @@ __device__ __forceinline__ void store_quad(void *p, int64_t i, const float4 v) {
 // adjacent pairs, 8l and 8l + 4; lanes past the rotated channels take theirs in
 // order and keep them.  So a head needs no exchange between lanes but the sum of
 // squares.  A CTA takes `tile` tokens (a power of two): their angles once, in
-// shared memory, then each group of lanes keeps one token and its angles in
-// registers and walks its share of the heads, UN heads' loads in flight.
-// Neighbouring groups hold neighbouring tokens, whose output rows are contiguous.
-template <int DT, int D>
-__global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_quads_kernel(RopeArgs A, int tile) {
-  constexpr int LPH = D / 8, groups = kRopeWarps * 32 / LPH, UN = 4;
+// shared memory; then each group of lanes keeps one token and walks its share
+// of the query heads, then of the key heads, UN heads' loads in flight, with the
+// products of norm weight and sine or cosine in registers: a pair (x, y) of a
+// head with root r becomes r (x wc - y ws'), r (y wc' + x ws).  Neighbouring
+// groups hold neighbouring tokens, whose output rows are contiguous.
+struct PairTurn {  // coefficients of one pair: out0 = x * xc - y * ys, out1 = y * yc + x * xs
+  float xc, ys, yc, xs;
+};
+
+template <int DT, int D, int TILE>
+__global__ void __launch_bounds__(kRopeWarps * 32, 3) qk_norm_rope_quads_kernel(RopeArgs A) {
+  constexpr int LPH = D / 8, groups = kRopeWarps * 32 / LPH, DH = groups / TILE, UN = 4;
   using Raw = typename Quad<DT>::Raw;
-  extern __shared__ float2 s_cs[];  // [tile][D / 2]
-  const int64_t tok0 = (int64_t)blockIdx.x * tile, n_tok = (int64_t)A.B * A.S;
+  constexpr int ES = sizeof(Raw) / 4, ISTEP = DH * D * ES;  // bytes between two of a group's heads in a row
+  __shared__ float2 s_cs[TILE][D / 2];
+  const unsigned tok0 = blockIdx.x * TILE, n_tok = (unsigned)A.B * (unsigned)A.S;  // below 2^31
   const int half = A.rot / 2;
-  for (int i = threadIdx.x; i < tile * half; i += blockDim.x) {
-    const int tt = i / half, k = i - tt * half;
-    const int64_t tok = min(tok0 + tt, n_tok - 1), b = tok / A.S, s = tok - b * A.S;
-    s_cs[tt * (D / 2) + k] = rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]);
+  for (int i = threadIdx.x; i < TILE * (D / 2); i += kRopeWarps * 32) {
+    const int tt = i / (D / 2), k = i - tt * (D / 2);
+    const unsigned tok = min(tok0 + tt, n_tok - 1), b = tok / (unsigned)A.S, s = tok - b * (unsigned)A.S;
+    if (k < half) s_cs[tt][k] = rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]);
   }
   const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH;
-  const int tt = group & (tile - 1), h0 = group / tile, dh = groups / tile;
+  const int tt = group & (TILE - 1), h0 = group / TILE;
   const bool turns = l < A.rot / 8, halves = !A.adjacent && turns, live = tok0 + tt < n_tok;
   const int da = halves ? 4 * l : 8 * l, db = halves ? half + 4 * l : 8 * l + 4;
-  const int64_t tok = min(tok0 + tt, n_tok - 1), b = tok / A.S, s = tok - b * A.S;
-  const int64_t src = b * A.sb + s * A.ss;
-  const int H = A.Hq + A.Hkv;
-  Raw ra[UN], rc[UN];
+  const unsigned tok = min(tok0 + tt, n_tok - 1), b = tok / (unsigned)A.S, s = tok - b * (unsigned)A.S;
+#pragma unroll 1
+  for (int part = (int)blockIdx.y; part < 2; part += (int)gridDim.y) {  // query heads, then key heads (or a CTA each)
+    const int H = part ? A.Hkv : A.Hq;
+    const char *in = (const char *)A.qkv + (b * A.sb + s * A.ss + (int64_t)((part ? A.Hq : 0) + h0) * D) * ES;
+    const char *ia = in + da * ES, *ib = in + db * ES;
+    const int64_t row = (int64_t)A.S * D * ES, ostep = DH * row;
+    char *out = (char *)(part ? A.k_out : A.q_out) + ((int64_t)b * H + h0) * row + (int64_t)s * (D * ES);
+    char *oa = out + da * ES, *ob = out + db * ES;
+    Raw ra[UN], rc[UN];
 #pragma unroll
-  for (int u = 0; u < UN; ++u) {
-    const int64_t at = src + (int64_t)min(h0 + u * dh, H - 1) * D;
-    ra[u] = load_quad<DT>(A.qkv, at + da);
-    rc[u] = load_quad<DT>(A.qkv, at + db);
-  }
-  __syncthreads();
-  float4 p01 = make_float4(1.f, 0.f, 1.f, 0.f), p23 = p01;  // cos, sin of the lane's four pairs
-  if (turns) {
-    const float4 *cs = (const float4 *)(s_cs + tt * (D / 2) + 4 * l);
-    p01 = cs[0];
-    p23 = cs[1];
-  }
-  for (int base = 0; base < H; base += dh * UN) {  // the same trips for every lane: the sums are shuffles
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      const int h = base + h0 + u * dh;
-      float4 a = widen<DT>(ra[u]), c = widen<DT>(rc[u]);
-      {  // this slot's next head
-        const int64_t at = src + (int64_t)min(h + dh * UN, H - 1) * D;
-        if (base + dh * UN < H) {
-          ra[u] = load_quad<DT>(A.qkv, at + da);
-          rc[u] = load_quad<DT>(A.qkv, at + db);
-        }
-      }
-      const bool is_q = h < A.Hq;
-      if (A.wq) {
-        float sq = a.x * a.x;
-        sq = fmaf(a.y, a.y, sq);
-        sq = fmaf(a.z, a.z, sq);
-        sq = fmaf(a.w, a.w, sq);
-        sq = fmaf(c.x, c.x, sq);
-        sq = fmaf(c.y, c.y, sq);
-        sq = fmaf(c.z, c.z, sq);
-        sq = fmaf(c.w, c.w, sq);
-#pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        const float r = rsqrtf(sq * (1.f / D) + A.eps);
-        const void *w = is_q ? A.wq : A.wk;
-        const float4 wa = widen<DT>(load_quad<DT>(w, da)), wb = widen<DT>(load_quad<DT>(w, db));
-        a = make_float4(a.x * r * wa.x, a.y * r * wa.y, a.z * r * wa.z, a.w * r * wa.w);
-        c = make_float4(c.x * r * wb.x, c.y * r * wb.y, c.z * r * wb.z, c.w * r * wb.w);
-      }
-      if (h >= H || !live) continue;
-      float4 x = a, y = c;
-      if (!turns) {  // channels past the rotated ones
-      } else if (!A.adjacent) {
-        x = make_float4(a.x * p01.x - c.x * p01.y, a.y * p01.z - c.y * p01.w, a.z * p23.x - c.z * p23.y,
-                        a.w * p23.z - c.w * p23.w);
-        y = make_float4(c.x * p01.x + a.x * p01.y, c.y * p01.z + a.y * p01.w, c.z * p23.x + a.z * p23.y,
-                        c.w * p23.z + a.w * p23.w);
+    for (int u = 0; u < UN; ++u)
+      if (h0 + u * DH < H) {
+        ra[u] = *(const Raw *)(ia + u * ISTEP);
+        rc[u] = *(const Raw *)(ib + u * ISTEP);
       } else {
-        x = make_float4(a.x * p01.x - a.y * p01.y, a.y * p01.x + a.x * p01.y, a.z * p01.z - a.w * p01.w,
-                        a.w * p01.z + a.z * p01.w);
-        y = make_float4(c.x * p23.x - c.y * p23.y, c.y * p23.x + c.x * p23.y, c.z * p23.z - c.w * p23.w,
-                        c.w * p23.z + c.z * p23.w);
+        ra[u] = rc[u] = Raw{};
       }
-      void *out = is_q ? A.q_out : A.k_out;
-      const int64_t head = is_q ? b * A.Hq + h : b * A.Hkv + (h - A.Hq);
-      const int64_t dst = (head * A.S + s) * D;
-      store_quad<DT>(out, dst + da, x);
-      store_quad<DT>(out, dst + db, y);
+    if (part == (int)blockIdx.y) __syncthreads();  // the angles
+    PairTurn p[4];
+    {
+      const void *w = part ? A.wk : A.wq;
+      float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa;
+      if (w) wa = widen<DT>(load_quad<DT>(w, da)), wb = widen<DT>(load_quad<DT>(w, db));
+      float4 c01 = make_float4(1.f, 0.f, 1.f, 0.f), c23 = c01;  // cos, sin of the lane's four pairs
+      if (turns) {
+        const float4 *cs = (const float4 *)&s_cs[tt][4 * l];
+        c01 = cs[0];
+        c23 = cs[1];
+      }
+      auto turn = [](float wx, float wy, float cs, float sn) { return PairTurn{wx * cs, wy * sn, wy * cs, wx * sn}; };
+      if (!A.adjacent) {  // pairs (a.i, c.i)
+        p[0] = turn(wa.x, wb.x, c01.x, c01.y);
+        p[1] = turn(wa.y, wb.y, c01.z, c01.w);
+        p[2] = turn(wa.z, wb.z, c23.x, c23.y);
+        p[3] = turn(wa.w, wb.w, c23.z, c23.w);
+      } else {  // pairs (a.x, a.y) (a.z, a.w) (c.x, c.y) (c.z, c.w)
+        p[0] = turn(wa.x, wa.y, c01.x, c01.y);
+        p[1] = turn(wa.z, wa.w, c01.z, c01.w);
+        p[2] = turn(wb.x, wb.y, c23.x, c23.y);
+        p[3] = turn(wb.z, wb.w, c23.z, c23.w);
+      }
+    }
+    for (int base = 0; base < H; base += DH * UN) {  // the same trips for every lane: the sums are shuffles
+      ia += UN * ISTEP;
+      ib += UN * ISTEP;
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int h = base + h0 + u * DH;
+        const float4 a = widen<DT>(ra[u]), c = widen<DT>(rc[u]);
+        if (h + DH * UN < H) {  // this slot's next head
+          ra[u] = *(const Raw *)(ia + u * ISTEP);
+          rc[u] = *(const Raw *)(ib + u * ISTEP);
+        }
+        float r = 1.f;
+        if (A.wq) {
+          float sq = a.x * a.x, s2 = c.x * c.x;
+          sq = fmaf(a.y, a.y, sq);
+          s2 = fmaf(c.y, c.y, s2);
+          sq = fmaf(a.z, a.z, sq);
+          s2 = fmaf(c.z, c.z, s2);
+          sq = fmaf(a.w, a.w, sq);
+          s2 = fmaf(c.w, c.w, s2);
+          sq += s2;
+#pragma unroll
+          for (int o = 1; o < LPH; o <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+          r = rsqrtf(fmaf(sq, 1.f / D, A.eps));
+        }
+        float4 x, y;
+        auto pair = [&](const PairTurn &t, float u0, float u1, float &o0, float &o1) {
+          o0 = (u0 * t.xc - u1 * t.ys) * r;
+          o1 = (u1 * t.yc + u0 * t.xs) * r;
+        };
+        if (!turns) {  // channels past the rotated ones, alone (no product with their neighbours)
+          if (!A.adjacent) {
+            x = make_float4(a.x * p[0].xc * r, a.y * p[1].xc * r, a.z * p[2].xc * r, a.w * p[3].xc * r);
+            y = make_float4(c.x * p[0].yc * r, c.y * p[1].yc * r, c.z * p[2].yc * r, c.w * p[3].yc * r);
+          } else {
+            x = make_float4(a.x * p[0].xc * r, a.y * p[0].yc * r, a.z * p[1].xc * r, a.w * p[1].yc * r);
+            y = make_float4(c.x * p[2].xc * r, c.y * p[2].yc * r, c.z * p[3].xc * r, c.w * p[3].yc * r);
+          }
+        } else if (!A.adjacent) {
+          pair(p[0], a.x, c.x, x.x, y.x);
+          pair(p[1], a.y, c.y, x.y, y.y);
+          pair(p[2], a.z, c.z, x.z, y.z);
+          pair(p[3], a.w, c.w, x.w, y.w);
+        } else {
+          pair(p[0], a.x, a.y, x.x, x.y);
+          pair(p[1], a.z, a.w, x.z, x.w);
+          pair(p[2], c.x, c.y, y.x, y.y);
+          pair(p[3], c.z, c.w, y.z, y.w);
+        }
+        if (h < H && live) {
+          store_quad<DT>(oa, 0, x);
+          store_quad<DT>(ob, 0, y);
+        }
+        oa += ostep;
+        ob += ostep;
+      }
     }
   }
 }
@@ -402,17 +443,17 @@ extern "C" int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t
                        (uintptr_t)k_norm_w | (uintptr_t)(seq_stride * (int64_t)es) |
                        (uintptr_t)(row_stride * (int64_t)es)) & (unit - 1)) == 0;
   if (quads) {
-    // tokens per CTA: their angles are computed once for all heads, so several where there are CTAs enough
-    const int tile = n >= 8 * 1024 ? 8 : n >= 4 * 1024 ? 4 : 1;
-    const int64_t grid = (n + tile - 1) / tile;
-    const size_t smem = (size_t)tile * (head_dim / 2) * sizeof(float2);
+    // 8 tokens per CTA where there are CTAs enough (their rows are written next to each other), else one, its query
+    // and key heads in CTAs of their own
+    const bool tiled = n >= 8 * 2 * sm_count();
+    const dim3 grid((unsigned)(tiled ? (n + 7) / 8 : n), tiled ? 1 : 2);
 #define CQ_ROPE(DT)                                                                                         \
-  (head_dim == 64    ? dec::qk_norm_rope_quads_kernel<DT, 64>                                               \
-   : head_dim == 128 ? dec::qk_norm_rope_quads_kernel<DT, 128>                                              \
-                     : dec::qk_norm_rope_quads_kernel<DT, 256>)
+  (head_dim == 64    ? (tiled ? dec::qk_norm_rope_quads_kernel<DT, 64, 8> : dec::qk_norm_rope_quads_kernel<DT, 64, 1>)   \
+   : head_dim == 128 ? (tiled ? dec::qk_norm_rope_quads_kernel<DT, 128, 8> : dec::qk_norm_rope_quads_kernel<DT, 128, 1>) \
+                     : (tiled ? dec::qk_norm_rope_quads_kernel<DT, 256, 8> : dec::qk_norm_rope_quads_kernel<DT, 256, 1>))
     auto *fn = dtype == CQ_F16 ? CQ_ROPE(CQ_F16) : dtype == CQ_BF16 ? CQ_ROPE(CQ_BF16) : CQ_ROPE(CQ_F32);
 #undef CQ_ROPE
-    fn<<<(unsigned)grid, dec::kRopeWarps * 32, smem, st>>>(A, tile);
+    fn<<<grid, dec::kRopeWarps * 32, 0, st>>>(A);
     return check_launch("cq_qk_norm_rope_rows");
   }
   auto *fn = dtype == CQ_F16    ? dec::qk_norm_rope_rows_kernel<CQ_F16>

@@ -113,19 +113,38 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
 }
 
 // The same for the common layouts: head sizes D of 64, 128 or 256, K codes in
-// natural order with token-indexed scales, rows 16-byte aligned, strides that
-// are a multiple of the rows a warp takes at once.  A warp per block: D / 32
-// lanes hold a token's code row (16 bytes, 32 channels each), so 32 / (D / 32)
-// tokens at a time; every code pair becomes the fp16 pair code * scale + anchor
-// with the roundings of reconstruct and goes through packed min and max.  The
-// lanes that hold the same channels then meet by halves: each step a lane hands
-// over half of its channels and keeps the other half.  An I-frame's scale slot
-// is 0, so whatever its row reads (the row before it, inside the chunk block)
-// becomes the anchor itself (the chunk's first token reads row 0).
+// natural order with token-indexed scales, rows 4-byte aligned, strides that are
+// a multiple of the rows a warp takes at once.  A warp per block: a lane holds
+// one code word (8 channels) of a row, D / 8 lanes a row, so 256 / D tokens at
+// a time.  Keys of one anchor are anchor + p, p = code * scale rounded to fp16;
+// rounding the sum keeps the order of p, so the packed minimum and maximum run
+// over p and the anchor is added once at the end.  The kernel is bound by
+// instructions, the ALU's first (half rate: mask, half a shift, minimum and
+// maximum of a code pair): with one word a lane the lanes' meeting at the end,
+// the anchors and the addresses cost a third of what they cost with four (2012
+// instructions per 64 tokens of two anchors then).  An I-frame's scale slot is
+// 0, so whatever its row reads (the row before it, inside the chunk block; the
+// chunk's first token reads row 0) gives p = 0, the anchor itself.
+
+// p of a code word's 4 pairs (channels k and k + 4) into the running minimum and maximum.
+__device__ __forceinline__ void range_of_word(uint32_t word, __half2 scale, __half2 (&lo)[4], __half2 (&hi)[4]) {
+  const __half2 m1032 = __float2half2_rn(-1032.f), sixteenth = __float2half2_rn(0.0625f), m72 = __float2half2_rn(-72.f);
+  const uint32_t w8 = word >> 8;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // nibbles k and k + 4 as 1024 + n, or as 1024 + 16 n, then the codes n - 8, exactly
+    const uint32_t v = ptx::lop3_and_or(k < 2 ? word : w8, k & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+    const __half2 code = k & 1 ? __hfma2(ptx::u2h2(v), sixteenth, m72) : __hadd2_rn(ptx::u2h2(v), m1032);
+    const __half2 p = __hmul2_rn(code, scale);
+    lo[k] = __hmin2(lo[k], p);  // a NaN is left out
+    hi[k] = __hmax2(hi[k], p);
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, unsigned n_warps) {
-  constexpr int LPR = D / 32, RPI = 32 / LPR;  // lanes per row, rows at once
-  constexpr int W = D / 8;                     // words of a code row
+  constexpr int W = D / 8, RPI = 32 / W;  // words (lanes) per row, rows at once
+  constexpr int UN = 8;                   // steps whose loads are in flight
   const int lane = threadIdx.x & 31;
   const CacheView &cv = A.cv;
   const CompView &c = cv.c[0];
@@ -138,7 +157,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
     }
     t0 = T - A.S;
   }
-  // positions in 32 bits (the launch keeps them there): 64-bit divisions cost as much as a chunk's codes
+  // positions in 32 bits (the launch keeps them there)
   const unsigned wi = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (wi >= n_warps) return;
   const unsigned unit = wi / (unsigned)A.nb;
@@ -146,88 +165,73 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
   const int ta = j * A.bt, tb = (int)min((unsigned)T, (unsigned)ta + (unsigned)A.bt);
   if (ta >= (int)T) return;
   const int b = (int)(unit / (unsigned)cv.H), h = (int)(unit - (unsigned)b * cv.H);
-  const int row = lane / LPR, part = lane % LPR;  // which of the rows at once, which 32 channels
-  const __half2 inf = __float2half2_rn(INFINITY);
-  __half2 lo[16], hi[16];
+  const int row = lane / W, word = lane % W;  // which of the rows at once, which 8 channels
+  const __half2 inf = __float2half2_rn(INFINITY), ninf = __float2half2_rn(-INFINITY);
+  __half2 lo[4], hi[4];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) lo[k] = inf, hi[k] = __hneg2(inf);
+  for (int k = 0; k < 4; ++k) lo[k] = inf, hi[k] = ninf;
 
   const int ct = c.pc + c.ac;  // tokens per chunk
   int t = ta;
   while (t < tb) {  // one anchor's tokens at a time: they lie in one chunk of one page
     const int lp = (int)((unsigned)t / (unsigned)cv.P);
     const int tl = t - lp * cv.P;
-    const int a = (int)((unsigned)tl / (unsigned)c.stride);
-    const int te = min(tb, t - (tl - a * c.stride) + c.stride);
-    const int64_t pg = page_of(cv, b, lp);
     const int jc = (int)((unsigned)tl / (unsigned)ct), x0 = tl - jc * ct;  // chunk, position in it
     const int xa = (int)((unsigned)x0 / (unsigned)c.stride);               // its anchor in the chunk
-    const __half *arow = c.kf + (pg * cv.H + h) * c.kf_hs + jc * c.kf_cs + xa * D + part * 32;
-    const uint32_t *crow = c.codes + (pg * cv.H + h) * c.cd_hs + jc * c.cd_cs + part * 4;
+    const int n = min(tb - t, (xa + 1) * c.stride - x0);
+    const int64_t ph = page_of(cv, b, lp) * cv.H + h;
+    const uint4 an = *(const uint4 *)(c.kf + ph * c.kf_hs + jc * c.kf_cs + xa * D + word * 8);
     const int i0 = x0 - xa - 1 + row;  // this lane's first code row
-    const __half *sc = c.scales + (pg * cv.H + h) * c.sc_hs + jc * c.sc_cs + x0 + row;
-    // the anchor's channels in the code words' pairs: (d, d + 4) of each 8
-    __half2 an[16];
+    const uint32_t *crow = c.codes + ph * c.cd_hs + jc * c.cd_cs + i0 * W + word;
+    const __half *sc = c.scales + ph * c.sc_hs + jc * c.sc_cs + x0 + row;
+    __half2 plo[4], phi[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint4 u = *(const uint4 *)(arow + 8 * w);
-      const uint32_t p[4] = {u.x, u.y, u.z, u.w};  // (0,1) (2,3) (4,5) (6,7)
+    for (int k = 0; k < 4; ++k) plo[k] = inf, phi[k] = ninf;
+    for (int r = 0; r < n; r += UN * RPI) {
+      uint32_t code[UN];
+      __half s1[UN];
+      if (r + UN * RPI <= n) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t pr = __byte_perm(p[k >> 1], p[2 + (k >> 1)], (k & 1) ? 0x7632u : 0x5410u);
-        an[4 * w + k] = *(const __half2 *)&pr;
-      }
-    }
-    const int n = te - t;
-    for (int r0 = 0; r0 < n; r0 += 2 * RPI) {
-      uint4 code[2];
-      __half s1[2];
+        for (int u = 0; u < UN; ++u) {
+          code[u] = u == 0 && i0 + r < 0 ? 0u : crow[(r + u * RPI) * W];
+          s1[u] = sc[r + u * RPI];
+        }
+      } else {  // rows past the end give NaN, which is left out
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int r = r0 + u * RPI;
-        if (r + row < n) {
-          code[u] = *(const uint4 *)(crow + max(i0 + r, 0) * W);
-          s1[u] = sc[r];
+        for (int u = 0; u < UN; ++u) {
+          const bool in = r + u * RPI + row < n;
+          code[u] = !in || i0 + r + u * RPI < 0 ? 0u : crow[(r + u * RPI) * W];
+          s1[u] = in ? sc[r + u * RPI] : __ushort_as_half(0x7fffu);
         }
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (r0 + u * RPI + row >= n) continue;
-        const __half2 sv = __half2half2(s1[u]);
-        const uint32_t word[4] = {code[u].x, code[u].y, code[u].z, code[u].w};
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // nibbles k and k + 4 as 1024 + n, minus 1032: the codes, exactly
-            const uint32_t v = ((word[w] >> (4 * k)) & 0x000f000fu) | 0x64006400u;
-            const __half2 code2 = __hsub2(*(const __half2 *)&v, __float2half2_rn(1032.f));
-            const __half2 key = __hadd2_rn(an[4 * w + k], __hmul2_rn(code2, sv));
-            lo[4 * w + k] = __hmin2(lo[4 * w + k], key);  // a NaN is left out
-            hi[4 * w + k] = __hmax2(hi[4 * w + k], key);
-          }
-      }
+      for (int u = 0; u < UN; ++u) range_of_word(code[u], __half2half2(s1[u]), plo, phi);
     }
-    t = te;
+    const uint32_t p[4] = {an.x, an.y, an.z, an.w};  // channels (0,1) (2,3) (4,5) (6,7)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t pr = __byte_perm(p[k >> 1], p[2 + (k >> 1)], (k & 1) ? 0x7632u : 0x5410u);
+      lo[k] = __hmin2(lo[k], __hadd2_rn(ptx::u2h2(pr), plo[k]));
+      hi[k] = __hmax2(hi[k], __hadd2_rn(ptx::u2h2(pr), phi[k]));
+    }
+    t += n;
   }
-  // lanes of the same channels: rows meet by halves until a lane holds 16 / RPI pairs
+  // lanes of the same channels: rows meet by halves, each keeping half of its pairs, until a lane holds 4 / RPI pairs
   int k0 = 0;  // first pair this lane still holds
   auto meet = [&](auto pairs, int o) {
-    constexpr int n = decltype(pairs)::value / 2;
+    constexpr int m = decltype(pairs)::value / 2;
     const bool up = lane & o;
 #pragma unroll
-    for (int k = 0; k < n; ++k) {
-      const __half2 la = lo[k], lb = lo[k + n], ha = hi[k], hb = hi[k + n];
+    for (int k = 0; k < m; ++k) {
+      const __half2 la = lo[k], lb = lo[k + m], ha = hi[k], hb = hi[k + m];
       lo[k] = __hmin2(up ? lb : la, __shfl_xor_sync(0xffffffffu, up ? la : lb, o));
       hi[k] = __hmax2(up ? hb : ha, __shfl_xor_sync(0xffffffffu, up ? ha : hb, o));
     }
-    if (up) k0 += n;
+    if (up) k0 += m;
   };
-  meet(std::integral_constant<int, 16>(), 16);
-  meet(std::integral_constant<int, 8>(), 8);
-  if constexpr (LPR <= 4) meet(std::integral_constant<int, 4>(), 4);
-  if constexpr (LPR <= 2) meet(std::integral_constant<int, 2>(), 2);
-  constexpr int NP = RPI >= 16 ? 1 : 16 / RPI;  // pairs a lane ends with
+  if constexpr (RPI >= 2) meet(std::integral_constant<int, 4>(), 16);
+  if constexpr (RPI >= 4) meet(std::integral_constant<int, 2>(), 8);
+  constexpr int NP = 4 / RPI;  // pairs a lane ends with
   float l[2 * NP], u[2 * NP], amax = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
   int8_t *codes = A.codes + at * 2 * D;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int pair = k0 + k, d = part * 32 + (pair >> 2) * 8 + (pair & 3);
+    const int d = word * 8 + k0 + k;
     store_codes(codes, d, D, l[2 * k], u[2 * k], s);
     store_codes(codes, d + 4, D, l[2 * k + 1], u[2 * k + 1], s);
   }
@@ -967,10 +971,9 @@ static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const cha
   const int64_t grid = (int64_t)A.cv.B * A.cv.H * A.nb;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_INVALID, std::string(what) + ": grid too large");
   const CompView &c = A.cv.c[0];
-  const int D = A.cv.D, rows = D == 64 ? 16 : D == 128 ? 8 : 4;  // code rows a warp takes at once
+  const int D = A.cv.D, rows = D == 64 ? 4 : D == 128 ? 2 : 1;  // code rows a warp takes at once
   if ((D == 64 || D == 128 || D == 256) && c.order == CQ_ORDER_NATURAL && c.stok && c.stride % rows == 0 &&
-      c.stride > 1 && A.bt % rows == 0 && aligned16(c.codes) && aligned16(c.kf) && (c.cd_hs | c.cd_cs) % 4 == 0 &&
-      (c.kf_hs | c.kf_cs) % 8 == 0 && A.T + A.bt < (1LL << 31)) {
+      c.stride > 1 && A.bt % rows == 0 && aligned16(c.kf) && (c.kf_hs | c.kf_cs) % 8 == 0 && A.T + A.bt < (1LL << 31)) {
     auto *fn = D == 64    ? sparse::block_bounds_rows_kernel<64>
                : D == 128 ? sparse::block_bounds_rows_kernel<128>
                           : sparse::block_bounds_rows_kernel<256>;
