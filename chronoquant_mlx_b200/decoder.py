@@ -29,10 +29,17 @@ every layer's cache, partial attention with log-sum-exp, one NCCL all-gather
 per layer, cq_lse_merge_packed).  Combined, a rank keeps its tensor-parallel
 share of the weights and, for its kv-heads, its token range of the context.
 
-``fill_context`` writes a synthetic context (seeded random K/V per layer,
-encoded by the cache's own append kernel) instead of running a 32k-token
-prompt through the model; a decode step's cost does not depend on the
-values.
+``prefill`` runs a prompt through the model in chunks (per-token head norm and
+rotation in ``qk_norm_rope``, causal query-chunk attention over the compressed
+cache) and leaves the decoder ready to step.  ``fill_context`` writes a
+synthetic context (seeded random K/V per layer, encoded by the cache's own
+append kernel) instead of running a 32k-token prompt through the model; a
+decode step's cost does not depend on the values.
+
+``sparse``: each step attends to the ``top`` blocks of the history that the
+layer's ``BlockIndex`` picks for it instead of to all of it (sparse.py): the
+step appends the token, refreshes its block's key ranges, selects and attends,
+all in the captured graph.
 """
 
 from __future__ import annotations
@@ -45,7 +52,10 @@ import torch
 
 from . import _lib
 from ._tensors import cq_dtype, stream_ptr
+from .attention import chronoquant_sdpa
 from .cache import ChronoQuantCache
+from .rope import qk_norm_rope
+from .sparse import BlockIndex, chronoquant_sparse_sdpa
 
 
 @dataclass
@@ -104,7 +114,7 @@ class Qwen3StyleDecoder:
 
     def __init__(self, cfg: DecoderConfig, batch: int, max_len: int, cache_kwargs: dict | None = None,
                  device="cuda", dtype=torch.bfloat16, seed: int = 0, tp_group=None, seq_group=None,
-                 peer_sum: bool = True):
+                 peer_sum: bool = True, sparse: dict | None = None):
         """``tp_group``: a torch.distributed (NCCL) group over which the layers
         are tensor-parallel by kv-head: this rank keeps kv_heads/N kv-heads
         with their query heads and ffn/N of each FFN; the o_proj and down
@@ -126,7 +136,22 @@ class Qwen3StyleDecoder:
         Both together (``mesh_groups``): the layers are tensor-parallel over
         ``tp_group`` and each rank's kv-heads hold its token range of the
         context; the tail ranks (the last of every sequence group) encode the
-        new tokens."""
+        new tokens.
+
+        ``sparse``: block-sparse attention with ``block_tokens`` (default 64),
+        ``top`` (required), ``first`` (1) and ``recent`` (2) as
+        ``BlockIndex.select`` takes them; None attends to the whole history.
+        Not together with ``seq_group``."""
+        if sparse is not None:
+            if seq_group is not None:
+                raise NotImplementedError("sparse attention under a sequence split is not supported")
+            unknown = set(sparse) - {"block_tokens", "top", "first", "recent"}
+            if unknown or "top" not in sparse:
+                raise ValueError(f"sparse takes block_tokens, top, first and recent (top is required), got {sparse}")
+            sparse = {"block_tokens": 64, "first": 1, "recent": 2, **sparse}
+            if sparse["recent"] < 1:
+                raise ValueError("sparse: recent must be at least 1 (a step attends to its own block)")
+        self.sparse = sparse
         self.cfg, self.B, self.max_len = cfg, batch, max_len
         self.device, self.dtype = torch.device(device), dtype
         self.group, self.seq_group = tp_group, seq_group
@@ -212,11 +237,73 @@ class Qwen3StyleDecoder:
         self.pos.fill_(T0)
         self._prepare_attention()
 
+    # -- prompts -----------------------------------------------------------------
+    def prefill(self, ids: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
+        """Run the prompt ``ids`` [B, S] through the model after whatever the
+        caches hold, ``chunk`` tokens at a time, and encode its K/V.  Returns the
+        last token's logits [B, vocab]; the next step starts from their argmax.
+        A step captured before is dropped (it holds the old lengths): capture again."""
+        if self.seq_group is not None:
+            raise NotImplementedError("prefill under a sequence split is not supported")
+        if ids.dim() != 2 or ids.shape[0] != self.B or ids.shape[1] < 1 or chunk < 1:
+            raise ValueError(f"prefill: ids must be [{self.B}, S] with S >= 1, got {tuple(ids.shape)}")
+        t0 = self.layers[0]["cache"].offset
+        if t0 + ids.shape[1] > self.max_len:
+            raise ValueError(f"prefill past max_len {self.max_len}")
+        ids = ids.to(self.device)
+        self.graph = None
+        for a in range(0, ids.shape[1], chunk):
+            xn = self._chunk_body(ids[:, a:a + chunk], t0 + a)
+        logits = xn.view(self.B, -1, self.cfg.hidden)[:, -1] @ self.lm_head.t()
+        self.ids.copy_(logits.argmax(-1))
+        self.pos.fill_(t0 + ids.shape[1])
+        self._prepare_attention()
+        return logits
+
+    def _chunk_body(self, ids: torch.Tensor, t0: int) -> torch.Tensor:
+        """One chunk of prompt tokens through every layer; final-normed rows [B * n, hidden]."""
+        c, B, n = self.cfg, self.B, ids.shape[1]
+        lib, st, dt = _lib.lib(), stream_ptr(self.device), cq_dtype(self.embed)
+        D, hq, hk = c.head_dim, self.heads, self.kv_heads
+        pos = torch.arange(t0, t0 + n, device=self.device)
+        x = self.embed[ids.reshape(-1)]
+        xn = self._norm(x, self.layers[0]["ln1"])
+        for i, L in enumerate(self.layers):
+            qkv = (xn @ L["wqkv"].t()).view(B, n, (hq + 2 * hk) * D)
+            q, k = qk_norm_rope(qkv, hq, hk, self.inv_freq, pos, L["q_norm"], L["k_norm"], eps=c.eps)
+            v = qkv[..., (hq + hk) * D:].view(B, n, hk, D).transpose(1, 2)
+            L["cache"].update_and_fetch(k, v)
+            a = self._chunk_attention(L, q).transpose(1, 2).reshape(B * n, hq * D)
+            x += self._reduce(a @ L["wo"].t())
+            gu = self._norm(x, L["ln2"]) @ L["wgu"].t()
+            h = torch.empty((B * n, self.ffn), device=self.device, dtype=self.dtype)
+            _lib.check(lib.cq_silu_mul(gu.data_ptr(), h.data_ptr(), B * n, self.ffn, dt, st), "decoder")
+            x += self._reduce(h @ L["wdown"].t())
+            xn = self._norm(x, self.layers[i + 1]["ln1"] if i + 1 < len(self.layers) else self.final_norm)
+        return xn
+
+    def _chunk_attention(self, L: dict, q: torch.Tensor) -> torch.Tensor:
+        """Causal attention of a chunk's queries, the newest tokens of the layer's cache."""
+        cache, scale = L["cache"], 1.0 / math.sqrt(self.cfg.head_dim)
+        sp = self.sparse
+        if sp is None or cache.offset <= sp["top"] * sp["block_tokens"]:
+            return chronoquant_sdpa(q, None, None, cache, scale, mask="causal" if q.shape[2] > 1 else None)
+        index = self._index(L)
+        blocks = index.select(q, sp["top"], first=sp["first"], recent=sp["recent"])
+        return chronoquant_sparse_sdpa(q, cache, scale, blocks, sp["block_tokens"])
+
+    def _index(self, L: dict) -> BlockIndex:
+        if "index" not in L:
+            L["index"] = BlockIndex(L["cache"], self.sparse["block_tokens"])
+        return L["index"]
+
     def _prepare_attention(self) -> None:
         """Per-layer descriptors, device-resident lengths and one shared
         workspace (layers run in order on one stream)."""
         lib = _lib.lib()
         need_max = 0
+        if self.sparse is not None:
+            self._prepare_sparse()
         for L in self.layers:
             st = L["cache"].store
             st.ensure(self.max_len, self.max_len)
@@ -237,6 +324,46 @@ class Qwen3StyleDecoder:
             self.lse_part = self.part[R * D:].view(self.B, self.heads)
             self.parts_all = torch.empty((W, R * (D + 1)), dtype=torch.float32, device=self.device)
 
+    def _prepare_sparse(self) -> None:
+        """Every layer's index, up to date and as large as its cache may grow,
+        one block list and one workspace for all."""
+        sp, lib = self.sparse, _lib.lib()
+        need = ctypes.c_size_t(0)
+        most = 1
+        for L in self.layers:
+            L["cache"].store.ensure(self.max_len, self.max_len)
+            index = self._index(L)
+            index.reserve(self.max_len)
+            index.update()
+            d = ctypes.byref(L["cache"].store.descriptor())
+            _lib.check(lib.cq_sparse_attention_workspace(d, self.max_len, self.heads, 1, sp["top"], sp["block_tokens"],
+                                                         ctypes.byref(need)), "decoder")
+            most = max(most, need.value)
+        _lib.check(lib.cq_block_select_workspace(self.B, self.kv_heads, 1, self.max_len, sp["block_tokens"],
+                                                 ctypes.byref(need)), "decoder")
+        self.sparse_ws = torch.empty(max(most, need.value), dtype=torch.uint8, device=self.device)
+        self.blocks = torch.empty((self.B, self.kv_heads, 1, sp["top"]), dtype=torch.int32, device=self.device)
+
+    def _sparse_attention(self, L: dict, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Encode this step's k/v, refresh the newest block's key ranges, list
+        the blocks each kv-head's queries attend to and attend over them."""
+        lib, sp, st, index = _lib.lib(), self.sparse, stream_ptr(self.device), L["index"]
+        ks, vs, qs, bt = k.stride(), v.stride(), q.stride(), sp["block_tokens"]
+        d, n = ctypes.byref(L["desc"]), L["len"].data_ptr()
+        codes, scales, cap = index.codes.data_ptr(), index.scales.data_ptr(), index.codes.shape[2]
+        ws, wsb = self.sparse_ws.data_ptr(), self.sparse_ws.numel()
+        _lib.check(lib.cq_append_at(d, k.data_ptr(), ks[0], ks[1], 0, v.data_ptr(), vs[0], vs[1], 0, cq_dtype(k), n, 1,
+                                    st), "decoder")
+        _lib.check(lib.cq_block_bounds_at(d, n, self.max_len, 1, bt, codes, scales, cap, st), "decoder")
+        _lib.check(lib.cq_block_select(codes, scales, cap, bt, self.B, self.kv_heads, self.cfg.head_dim, self.max_len, n,
+                                       q.data_ptr(), cq_dtype(q), self.heads, 1, qs[0], qs[1], 0, None, sp["first"],
+                                       sp["recent"], sp["top"], self.blocks.data_ptr(), None, ws, wsb, st), "decoder")
+        _lib.check(lib.cq_sparse_attention(d, self.max_len, n, q.data_ptr(), cq_dtype(q), self.heads, 1, qs[0], qs[1],
+                                           0, 1.0 / math.sqrt(self.cfg.head_dim), None, self.blocks.data_ptr(),
+                                           sp["top"], bt, self.attn_out.data_ptr(), cq_dtype(self.attn_out), None, ws,
+                                           wsb, st), "decoder")
+        return self.attn_out
+
     # -- one decode step --------------------------------------------------------
     def _attention(self, L: dict, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Encode this step's k/v [B, Hkv, D] into the layer's cache and attend
@@ -244,6 +371,8 @@ class Qwen3StyleDecoder:
         Under a sequence split the tail rank does that and the others attend
         their fixed range (cq_attention_at); each writes an fp32 partial with
         its log-sum-exp, and the gathered partials are merged (cq_lse_merge_packed)."""
+        if self.sparse is not None:
+            return self._sparse_attention(L, q, k, v)
         lib = _lib.lib()
         ks, vs, qs = k.stride(), v.stride(), q.stride()
         scale = 1.0 / math.sqrt(self.cfg.head_dim)
@@ -372,6 +501,8 @@ class Qwen3StyleDecoder:
         between); returns the last step's logits.  The caches' host-side
         offsets follow the device lengths afterwards."""
         start = self.layers[0]["cache"].offset
+        if self.graph is None:
+            raise RuntimeError("decode replays a captured step: call capture() first")
         if start + steps > self.max_len:
             raise ValueError(f"decode past max_len {self.max_len}")
         for _ in range(steps):
@@ -379,6 +510,8 @@ class Qwen3StyleDecoder:
         if self.tail:  # under a sequence split only the tail rank's caches grow
             for L in self.layers:
                 L["cache"].offset += steps
+                if self.sparse is not None:
+                    L["index"].covered = L["cache"].offset
         return self.logits
 
     def close(self) -> None:

@@ -1,0 +1,157 @@
+"""The decoder's prompt path and its block-sparse steps.
+
+Bars as in test_decoder.py: the same kernels in another order within 1e-3
+relative (L2) of each other; the prompt path against one-token steps within
+2e-2 (bf16 activations, other GEMM shapes, the query-chunk attention's fp16
+reconstruction against the decode kernel's fp32 one)."""
+
+import math
+
+import pytest
+import torch
+
+from chronoquant_mlx_b200 import BlockIndex, chronoquant_sparse_sdpa
+from chronoquant_mlx_b200.decoder import DecoderConfig, Qwen3StyleDecoder
+
+gpu = pytest.mark.gpu
+
+CFG = DecoderConfig(layers=2, hidden=512, heads=8, kv_heads=2, head_dim=128, ffn=1024, vocab=1000)
+FT = dict(stride_k=64, stride_v=32, delta_bits_v=3, dead_zone_v=0.05)
+
+
+def rel(a, b):
+    return float((a.float() - b.float()).norm() / b.float().norm())
+
+
+def prompt(B, S, seed=0):
+    return torch.randint(0, CFG.vocab, (B, S), generator=torch.Generator().manual_seed(seed))
+
+
+@gpu
+@pytest.mark.parametrize("kw", [dict(), FT])
+def test_prefill_matches_steps(kw):
+    """A 70-token prompt in one chunk, in chunks of 33, and its last 3 tokens as
+    single steps (eager and captured): the same logits, greedy ids and caches."""
+    ids = prompt(2, 70)
+    a, b, c = (Qwen3StyleDecoder(CFG, 2, 120, kw, seed=3) for _ in range(3))
+    la = a.prefill(ids)
+    lb = b.prefill(ids, chunk=33)
+    assert rel(lb, la) < 2e-2
+    c.prefill(ids[:, :67])
+    for t in range(67, 69):
+        c.ids.copy_(ids[:, t])
+        c.step_eager()
+        for L in c.layers:  # eager steps advance the device length; the host's follows
+            L["cache"].offset += 1
+    c.capture()
+    c.ids.copy_(ids[:, 69])
+    lc = c.decode(1)
+    assert rel(lc, la) < 2e-2
+    assert a.layers[1]["cache"].offset == b.layers[1]["cache"].offset == c.layers[1]["cache"].offset == 70
+    assert int(a.pos) == int(c.pos) == 70 and int(a.layers[0]["len"][0]) == int(c.layers[0]["len"][0]) == 70
+    assert torch.equal(a.ids, la.argmax(-1))
+    # the first layer's K/V depend on the ids and positions alone, up to the rounding of two norm kernels
+    for x, y in zip(a.layers[0]["cache"].reconstruct_history(), c.layers[0]["cache"].reconstruct_history()):
+        assert rel(x, y) < 1e-2
+    c.prefill(prompt(2, 2))
+    with pytest.raises(RuntimeError):  # the captured step held the lengths of before
+        c.decode(1)
+    more = prompt(2, 5, seed=1)  # a second prompt behind the first
+    assert rel(a.prefill(more), Qwen3StyleDecoder(CFG, 2, 120, kw, seed=3).prefill(torch.cat((ids, more), 1))) < 2e-2
+
+
+@gpu
+@pytest.mark.parametrize("kw", [dict(), FT, dict(stride_k=12, stride_v=4)])
+def test_sparse_step_over_every_block_is_the_dense_step(kw):
+    """With room for every block the sparse decoder is the dense one: eager
+    steps for every layout, captured ones too, across a block's end."""
+    T0 = 317
+    dense_ok = kw.get("stride_k") != 12  # the dense step needs the decode kernel's layouts
+    d = Qwen3StyleDecoder(CFG, 2, T0 + 10, kw, seed=3)
+    s = Qwen3StyleDecoder(CFG, 2, T0 + 10, kw, seed=3, sparse=dict(top=6))
+    for m in (d, s):
+        m.fill_context(T0)
+    if not dense_ok:
+        d._attention = None
+    s.capture() if dense_ok else None
+    for i in range(6):
+        ids = torch.tensor([5 + i, 77 - i], device="cuda")
+        s.ids.copy_(ids)
+        d.ids.copy_(ids)
+        ls = (s.decode(1) if dense_ok else s.step_eager()).float().clone()
+        if dense_ok:
+            assert rel(ls, d.step_eager()) < 1e-2
+        assert torch.isfinite(ls).all()
+        n = T0 + i + 1
+        want = list(range(-(-n // 64))) + [-1] * (6 - -(-n // 64))
+        assert s.blocks[0, 0, 0].tolist() == want
+    assert int(s.layers[1]["len"][0]) == T0 + 6
+
+
+@gpu
+def test_sparse_steps_follow_their_index():
+    """Captured sparse steps with few blocks: every layer attends to what a
+    fresh index over its cache selects (the eager path's own calls), and
+    graph and eager agree."""
+    T0, kw, sp = 900, FT, dict(top=5, block_tokens=64, first=1, recent=1)
+    g = Qwen3StyleDecoder(CFG, 2, T0 + 80, kw, seed=7, sparse=sp)
+    e = Qwen3StyleDecoder(CFG, 2, T0 + 80, kw, seed=7)
+    for m in (g, e):
+        m.fill_context(T0)
+    g.capture()
+
+    def attend(L, q, k, v):
+        cache = L["cache"]
+        cache.update_and_fetch(k.unsqueeze(2), v.unsqueeze(2))
+        blocks = BlockIndex(cache, 64).select(q.unsqueeze(2), 5, first=1, recent=1)
+        L["blocks"] = blocks
+        return chronoquant_sparse_sdpa(q.unsqueeze(2), cache, 1 / math.sqrt(128), blocks, 64).squeeze(2)
+
+    for i in range(70):  # past a block's end
+        ids = torch.tensor([i, 3 * i], device="cuda")
+        g.ids.copy_(ids)
+        e.ids.copy_(ids)
+        lg, le = g.decode(1).float().clone(), e.step_eager(attend).float()
+        assert rel(lg, le) <= 1e-3, i
+        assert torch.equal(g.blocks, e.layers[-1]["blocks"]), i  # the last layer's lists
+    for L in g.layers:
+        whole = BlockIndex(L["cache"], 64).update()
+        n = whole.n_blocks
+        assert L["index"].covered == T0 + 70 and torch.equal(L["index"].codes[:, :, :n], whole.codes[:, :, :n])
+    # an eager call on the same index afterwards goes on from there
+    assert g.layers[0]["index"].select(torch.zeros((2, 8, 1, 128), device="cuda").bfloat16(), 5).shape == (2, 2, 1, 5)
+
+
+@gpu
+def test_sparse_prefill():
+    """A long prompt through the sparse path: its first chunk is dense, the
+    later ones select; the result is close to the dense model's, the lists hold
+    their own block."""
+    ids = prompt(1, 600, seed=2)
+    dense = Qwen3StyleDecoder(CFG, 1, 700, FT, seed=3).prefill(ids, chunk=200)
+    m = Qwen3StyleDecoder(CFG, 1, 700, FT, seed=3, sparse=dict(top=8, block_tokens=64))
+    got = m.prefill(ids, chunk=200)
+    assert torch.isfinite(got).all() and rel(got, dense) < 0.5  # 8 of 10 blocks: another, nearby function
+    all_blocks = Qwen3StyleDecoder(CFG, 1, 700, FT, seed=3, sparse=dict(top=8, block_tokens=96 * 2))
+    assert rel(all_blocks.prefill(ids, chunk=200), dense) < 2e-2
+
+
+def test_refusals():
+    for sparse in (dict(), dict(first=1), dict(top=4, blocks=3), dict(top=4, recent=0)):
+        with pytest.raises(ValueError):
+            Qwen3StyleDecoder(CFG, 1, 64, sparse=sparse, device="cpu")
+    with pytest.raises(NotImplementedError):
+        Qwen3StyleDecoder(CFG, 1, 64, sparse=dict(top=4), seq_group=object(), device="cpu")
+
+
+@gpu
+def test_prefill_refusals():
+    m = Qwen3StyleDecoder(CFG, 2, 64, seed=3)
+    for ids in (prompt(1, 4), prompt(2, 4)[:, :0], prompt(2, 4)[0], prompt(2, 65)):
+        with pytest.raises(ValueError):
+            m.prefill(ids)
+    with pytest.raises(RuntimeError):
+        m.decode(1)
+    m.seq_group = object()
+    with pytest.raises(NotImplementedError):
+        m.prefill(prompt(2, 4))
