@@ -152,6 +152,28 @@ def lib():
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """Load (once) and return the extension module of the checked C++ entry
+    points, bound to the library that ``lib()`` loads."""
+    global _calls
+    if _calls is None:
+        lib()
+        with _lock:
+            if _calls is None:
+                import torch  # noqa: F401  (the module links against torch's libraries)
+                try:
+                    from . import _calls as m
+                except ImportError as e:
+                    raise ImportError(f"the _calls extension is not built or does not load ({e}); build it with "
+                                      "`python -m chronoquant_mlx_b200.build`") from e
+                m.load(LIB_PATH, CudaLibError)
+                _calls = m
+    return _calls
+
+
 def check(status: int, what: str = "") -> None:
     """Raise on a non-zero status from the C ABI."""
     if status == CQ_OK:

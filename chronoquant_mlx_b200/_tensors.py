@@ -2,13 +2,9 @@
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
-
-_HERE = contextlib.nullcontext()
 
 _DT = {torch.float16: _lib.CQ_F16, torch.bfloat16: _lib.CQ_BF16, torch.float32: _lib.CQ_F32}
 
@@ -40,11 +36,3 @@ def stream_ptr(device: torch.device | None = None) -> int:
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
-
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one (a launch goes to the
-    current device; switching costs more than a launch, so it is done only
-    where another one is current)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return torch.cuda.device(device)

@@ -5,6 +5,9 @@
 Each ``csrc/*.cu`` compiles to an object under ``_build/`` (in parallel), then
 they link into ``chronoquant_mlx_b200/libchronoquant_b200.so``.  Objects are
 rebuilt when their source or any ``csrc/*.cuh`` / ``include/*.h`` is newer.
+``csrc/cq_calls.cpp`` (host code: the checked Python entry points of the sparse
+operators) compiles with g++ against torch's headers into the extension module
+``chronoquant_mlx_b200/_calls.so``.
 
 ``--checks`` builds the debug variant ``libchronoquant_b200_checks.so``
 (objects under ``_build/checks/``) with ``-DCQ_CHECKS``: every page lookup
@@ -29,6 +32,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libchronoquant_b200.so")
 OUT_CHECKS = os.path.join(HERE, "libchronoquant_b200_checks.so")
 BUILD = os.path.join(ROOT, "_build")
+CALLS_SRC = os.path.join(CSRC, "cq_calls.cpp")
+CALLS_OUT = os.path.join(HERE, "_calls.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -45,6 +50,37 @@ def nvcc() -> str:
 def _newest_header() -> float:
     hs = glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
     return max((os.path.getmtime(h) for h in hs), default=0.0)
+
+
+def build_calls(force: bool = False) -> str:
+    """The extension module of cq_calls.cpp (rebuilt when it, the C header or torch's version is newer)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    stamp = os.path.join(BUILD, "calls.torch")
+    header = os.path.join(ROOT, "include", "chronoquant_b200.h")
+    version = f"{torch.__version__} {sysconfig.get_python_version()}"
+    built_for = open(stamp).read() if os.path.exists(stamp) else ""
+    if (not force and built_for == version and os.path.exists(CALLS_OUT)
+            and os.path.getmtime(CALLS_OUT) >= max(os.path.getmtime(CALLS_SRC), os.path.getmtime(header))):
+        return CALLS_OUT
+    os.makedirs(BUILD, exist_ok=True)
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    inc = [f for d in (*cpp_extension.include_paths(), cuda, sysconfig.get_paths()["include"]) for f in ("-isystem", d)]
+    tmp = CALLS_OUT + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, CALLS_SRC, "-o", tmp, "-L", lib,
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {CALLS_SRC}:\n{r.stderr}")
+    os.replace(tmp, CALLS_OUT)
+    with open(stamp, "w") as f:
+        f.write(version)
+    return CALLS_OUT
 
 
 def build(force: bool = False, jobs: int = 8, verbose: bool = False, checks: bool = False) -> str:
@@ -69,7 +105,9 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False, checks: boo
         return obj
 
     with ThreadPoolExecutor(max_workers=jobs) as ex:
+        calls = ex.submit(build_calls, force)
         objs = list(ex.map(compile_one, srcs))
+    calls.result()
     newest_obj = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(out) or os.path.getmtime(out) < newest_obj:
         tmp = out + ".tmp"
