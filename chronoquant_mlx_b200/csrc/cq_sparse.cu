@@ -329,7 +329,10 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
 // bytes apart modulo 128: no bank conflicts), then each warp takes columns in
 // `passes`, keeping two column tiles' codes in registers over the rows.  The
 // maximum over a group's heads goes by halves: each exchange also halves the
-// values a lane holds, so every lane ends with its own ones to store.
+// values a lane holds, so every lane ends with its own ones to store.  Bound by
+// the tensor pipe: mma.sync runs at about 512 multiply-adds a clock and SM here,
+// for int8 as for fp16 (2048 rows x 1024 blocks x 256 codes x 8 units: 34 us;
+// with the codes as fp16, whose fragments cost conversions, 47 us).
 constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
 
 template <int KS, int GP>
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(Selec
   __syncthreads();
   // the last block any of this CTA's tokens sees
   const int i_last = min(A.q_len, i0 + tiles * TPT) - 1;
-  const int j_end = (int)min(A.n, (T - A.q_len + i_last) / A.bt + 1);
+  const int j_end = (int)min((unsigned)A.n, (unsigned)(T - A.q_len + i_last) / (unsigned)A.bt + 1u);  // T below 2^31
   const int real_tiles = (i_last - i0) / TPT + 1;
   const int8_t *codes = A.codes + unit * A.max_blocks * 2 * D;
   const float *scales = A.scales + unit * A.max_blocks;
@@ -517,14 +520,17 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 }
 
 // The `top` best visible blocks of a (unit, query token) row with every key in a
-// register: W warps hold KPT keys a thread.  The threshold key is found bit by
-// bit from the highest one on which the row's keys differ (a candidate holds if
-// at least `top` keys reach it).  As soon as no more than kShort keys reach the
-// threshold so far they are gathered in index order in shared memory, and one
-// warp goes on with those alone; where that never happens (long lists, many
-// equal keys) the search runs to the last bit over the registers.  The list is
-// written in index order, of equal keys the lowest indexes.
-constexpr int kShort = 256;
+// register: W warps hold KPT keys a thread.  The threshold key is found from the
+// highest bit on which the row's keys differ: with up to four warps bit by bit
+// (count the keys that reach a candidate), with more of them, whose meetings
+// cost more, eight bits at a time by a histogram of the keys still in question.
+// As soon as no more than kShort keys reach the threshold so far, those are
+// gathered in index order in shared memory, and one warp goes on with them
+// alone, bit by bit (ranking them against each other instead took 3 us more).
+// Where that never happens (long lists, many equal keys) the search runs to the
+// last bit.  The list is written in index order, of equal keys the lowest
+// indexes.
+constexpr int kShort = 128;
 
 // Exclusive prefix of `n` (at most 32 * PER) packed counts in shared memory, in
 // place, by one warp; returns the sum.
@@ -556,24 +562,27 @@ template <int KPT, int THREADS>
 __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
   __shared__ uint32_t s_key[kShort];
   __shared__ int s_idx[kShort];
-  __shared__ int s_cnt[2][32];
-  __shared__ int s_pre[KPT * 32];
+  __shared__ int s_hist[THREADS > 128 ? 256 : 1];
+  __shared__ int s_cnt[4];
+  __shared__ int s_pre[KPT * 32 < 64 ? 64 : KPT * 32];
   ptx::grid_dependency_wait();
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
+  const unsigned row = blockIdx.x;
   if (T == 0) {
     if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
     return;
   }
-  const int i = (int)(row % A.q_len);
-  const int b = (int)(row / ((int64_t)A.q_len * A.H));
-  const int64_t p = T - A.q_len + i, st = first_token(A.starts, b);
-  const int fb = (int)min(st / A.bt, (int64_t)INT32_MAX), lb = (int)(p / A.bt);
+  // 32-bit positions (the launch keeps T there): a 64-bit division takes a hundred instructions
+  const unsigned unit = row / (unsigned)A.q_len, bt = (unsigned)A.bt;
+  const int b = (int)(unit / (unsigned)A.H);
+  const unsigned p = (unsigned)(T - A.q_len) + (row - unit * (unsigned)A.q_len);
+  const unsigned st = (unsigned)min(first_token(A.starts, b), (int64_t)INT32_MAX);
+  const int fb = (int)(st / bt), lb = (int)(p / bt);
   const int nv = st > p ? 0 : lb - fb + 1;
-  const float *score = A.score + row * A.ns;
-  int32_t *out = A.blocks + row * A.top;
-  float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
+  const float *score = A.score + (int64_t)row * A.ns;
+  int32_t *out = A.blocks + (int64_t)row * A.top;
+  float *out_s = A.block_scores ? A.block_scores + (int64_t)row * A.top : nullptr;
   const int tid = warp * 32 + lane, step = W * 32;
   for (int k = min(nv, A.top) + tid; k < A.top; k += step) {
     out[k] = -1;
@@ -590,16 +599,6 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
       all_and &= key[k];
     }
   }
-  int par = 0;
-  auto total = [&](int c) {  // over the row's threads
-    c = __reduce_add_sync(0xffffffffu, c);
-    if (W == 1) return c;
-    if (lane == 0) s_cnt[par][warp] = c;
-    __syncthreads();
-    c = __reduce_add_sync(0xffffffffu, lane < W ? s_cnt[par][lane] : 0);
-    par ^= 1;
-    return c;
-  };
   uint32_t thr = 1;  // keys at or above it are taken, those equal to it from the lowest index on
   int reach = nv;    // keys that reach it
   int bit = -1;
@@ -608,23 +607,70 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     all_or = __reduce_or_sync(0xffffffffu, all_or);
     all_and = __reduce_and_sync(0xffffffffu, all_and);
     if (W > 1) {
-      if (lane == 0) s_pre[warp] = (int)all_or, s_cnt[0][warp] = (int)all_and;
+      if (lane == 0) s_pre[2 * warp] = (int)all_or, s_pre[2 * warp + 1] = (int)all_and;
       __syncthreads();
-      all_or = __reduce_or_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[lane] : 0u);
-      all_and = __reduce_and_sync(0xffffffffu, lane < W ? (uint32_t)s_cnt[0][lane] : 0xffffffffu);
-      __syncthreads();
+      all_or = __reduce_or_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane] : 0u);
+      all_and = __reduce_and_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane + 1] : 0xffffffffu);
+      __syncthreads();  // s_pre is written again below
     }
     const uint32_t differ = all_or & ~all_and;  // first + recent <= top < nv: some key is not forced
     bit = differ ? 31 - __clz(differ) : -1;
     thr = bit < 0 ? all_and : all_and & ~((2u << bit) - 1u);
     const bool shorten = A.top <= kShort;
-    for (; bit >= 0 && reach != A.top && !(shorten && reach <= kShort); --bit) {
-      const uint32_t cand = thr | (1u << bit);
-      int c = 0;
+    int above = A.first + A.recent;  // keys above those in question (all of them visible: nv > top)
+    if (above == A.top) thr = 0xffffffffu, reach = A.top, bit = -1;  // the forced blocks fill the list
+    if constexpr (THREADS <= 128) {
+      int par = 0;
+      for (; bit >= 0 && reach != A.top && !(shorten && reach <= kShort); --bit) {
+        const uint32_t cand = thr | (1u << bit);
+        int c = 0;
 #pragma unroll
-      for (int k = 0; k < KPT; ++k) c += key[k] >= cand;
-      c = total(c);
-      if (c >= A.top) thr = cand, reach = c;
+        for (int k = 0; k < KPT; ++k) c += key[k] >= cand;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (W > 1) {
+          if (lane == 0) s_pre[par * 4 + warp] = c;
+          __syncthreads();
+          c = __reduce_add_sync(0xffffffffu, lane < W ? s_pre[par * 4 + lane] : 0);
+          par ^= 1;
+        }
+        if (c >= A.top) thr = cand, reach = c;
+      }
+      if (W > 1) __syncthreads();  // s_pre is written again below
+    }
+    while (THREADS > 128 && bit >= 0 && reach != A.top && !(shorten && reach <= kShort)) {
+      const int shift = max(bit - 7, 0), bins = 2 << (bit - shift);  // up to 8 bits
+      for (int k = tid; k < 256; k += step) s_hist[k] = 0;
+      __syncthreads();
+      const uint32_t prefix = bit >= 31 ? 0u : thr >> (bit + 1);
+#pragma unroll
+      for (int k = 0; k < KPT; ++k)
+        if (key[k] != 0u && key[k] != 0xffffffffu && (bit >= 31 || key[k] >> (bit + 1) == prefix))
+          atomicAdd(&s_hist[(key[k] >> shift) & (bins - 1)], 1);
+      __syncthreads();
+      if (warp == 0) {  // the highest bin that brings the count to `top`: lane l holds bins 8l .. 8l + 7
+        int c[8], sum = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += c[e] = s_hist[lane * 8 + e];
+        int from = sum;  // of this lane's bins and all above
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_down_sync(0xffffffffu, from, o);
+          if (lane + o < 32) from += x;
+        }
+        int over = above + from - sum;  // keys above this lane's bins
+        if (over < A.top && over + sum >= A.top) {  // one lane
+          int e = 7;
+          while (over + c[e] < A.top) over += c[e--];
+          s_cnt[0] = lane * 8 + e;
+          s_cnt[1] = over;
+          s_cnt[2] = over + c[e];
+        }
+      }
+      __syncthreads();
+      thr |= (uint32_t)s_cnt[0] << shift;
+      above = s_cnt[1];
+      reach = s_cnt[2];
+      bit = shift - 1;
     }
   }
   if (reach <= kShort && reach > 0) {  // gather the keys that reach the threshold, in index order
@@ -706,10 +752,10 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     __syncthreads();
     if (warp == 0) {
       const int all = warp_prefix<KPT>(s_pre, KPT * W, lane);
-      if (lane == 0) s_cnt[0][0] = all;
+      if (lane == 0) s_cnt[0] = all;
     }
     __syncthreads();
-    all_gt = s_cnt[0][0] & 0xffff;
+    all_gt = s_cnt[0] & 0xffff;
   }
   const int need = A.top - all_gt;  // equal keys to take
   int running = 0;
@@ -1058,7 +1104,7 @@ static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
   using namespace sparse;
   const int64_t rows = (int64_t)A.B * A.H * A.q_len, units = (int64_t)A.B * A.H;
   if ((A.D == 64 || A.D == 96 || A.D == 128 || A.D == 256) && A.G <= 16 && aligned16(A.codes) && aligned16(A.score) &&
-      units < 65536 && A.n < (1LL << 30)) {
+      units < 65536 && A.T < (1LL << 31)) {
     int lg = 0;
     while ((1 << lg) < A.G) ++lg;
     using Fn = void (*)(SelectArgs, int, int);
@@ -1095,7 +1141,7 @@ static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t s
   int kpt = rows >= 4 * sm_count() && A.n > 128 ? 8 : 4;
   while (kpt < 16 && A.n > (int64_t)kpt * 32 * 32) kpt *= 2;
   const int64_t W = (A.n + kpt * 32 - 1) / (kpt * 32);
-  if (W > 32) {
+  if (W > 32 || A.T >= (1LL << 31)) {
     block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
     return check_launch("cq_block_select");
   }
@@ -1156,7 +1202,7 @@ extern "C" int cq_sparse_attention_workspace(const cq_paged_cache *cache, int64_
   int r = sparse_checks(cache, T, n_q_heads, q_len, top, block_tokens);
   if (r) return r;
   CQ_REQUIRE(bytes, CQ_ERR_INVALID, "cq_sparse_attention_workspace: bytes is null");
-  if (sparse_fast_supported(*cache, n_q_heads, block_tokens)) {
+  if (sparse_fast_supported(*cache, T, n_q_heads, block_tokens)) {
     *bytes = 0;
     return CQ_OK;
   }
@@ -1178,7 +1224,7 @@ extern "C" int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const
   CQ_REQUIRE(out_dtype == CQ_F16 || out_dtype == CQ_BF16 || out_dtype == CQ_F32, CQ_ERR_UNSUPPORTED,
              "cq_sparse_attention: bad out dtype");
   const int64_t rows = (int64_t)cache->batch * n_q_heads * q_len;
-  if (sparse_fast_supported(*cache, n_q_heads, block_tokens))
+  if (sparse_fast_supported(*cache, T, n_q_heads, block_tokens))
     return run_sparse_fast(*cache, T, len_dev, q, q_dtype, n_q_heads, q_len, q_sb, q_sh, q_sq, scale, starts, blocks,
                            top, block_tokens, out, out_dtype, lse_out, (cudaStream_t)stream);
   const int splits = sparse::pick_list_splits(rows, top), D = cache->head_dim;

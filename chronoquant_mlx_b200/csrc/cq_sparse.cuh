@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 
 // Attention over listed blocks on the chunk-block layout (cq_sparse_fast.cu);
 // it needs no workspace.
-bool sparse_fast_supported(const cq_paged_cache &c, int n_q_heads, int block_tokens);
+bool sparse_fast_supported(const cq_paged_cache &c, int64_t T, int n_q_heads, int block_tokens);
 int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
                     int n_q_heads, int q_len, int64_t q_sb, int64_t q_sh, int64_t q_sq, float scale,
                     const int64_t *starts, const int32_t *blocks, int top, int block_tokens, void *out, int out_dtype,

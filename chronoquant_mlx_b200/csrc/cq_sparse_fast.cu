@@ -42,7 +42,7 @@ struct SparseParams {
   const int32_t *blocks;
   int cpb;        // chunks per block
   int w, s;       // warps per unit in a CTA, CTAs per unit
-  int64_t units;
+  unsigned units;
   void *out;
   int out_dtype;
   float *lse_out;
@@ -158,14 +158,16 @@ __device__ __forceinline__ bool sparse_chunk(WarpState &st, const QFrag &f, int 
 
 // The chunks of rank r of unit (b, h, i); the partial is left in `region`.
 template <class G>
-__device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int64_t unit, int r, unsigned char *region,
+__device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, unsigned unit, int r, unsigned char *region,
                                           uint64_t *bar, int lane) {
+  // positions and units in 32 bits (the launch keeps them there)
   const int W = p.w * p.s, n = p.top * p.cpb;
-  const int i = (int)(unit % p.q_len);
-  const int64_t bh = unit / p.q_len;
-  const int b = (int)(bh / p.cv.H), h = (int)(bh - (int64_t)b * p.cv.H);
-  const int64_t pos = T - p.q_len + i, st0 = sparse::first_token(p.starts, b);
-  const int32_t *list = p.blocks + unit * p.top;
+  const unsigned bh = unit / (unsigned)p.q_len;
+  const int i = (int)(unit - bh * (unsigned)p.q_len);
+  const int b = (int)(bh / (unsigned)p.cv.H), h = (int)(bh - (unsigned)b * (unsigned)p.cv.H);
+  const int pos = (int)T - p.q_len + i, st0 = (int)min(sparse::first_token(p.starts, b), (int64_t)INT32_MAX);
+  const int last = (int)((unsigned)pos / (unsigned)p.bt);  // the query's own block
+  const int32_t *list = p.blocks + (int64_t)unit * p.top;
   const uint32_t ra = ptx::smem_u32(region);
   float *qa = (float *)(region + G::BUF);
   unsigned char *qt = region + G::BUF + kQaBytes;
@@ -182,16 +184,16 @@ __device__ __forceinline__ void unit_main(const SparseParams &p, int64_t T, int6
     const int64_t x = base + (int64_t)lane * W;
     if (x < n) {
       const int slot = (int)x / p.cpb, c = (int)x - slot * p.cpb;
-      const int64_t j = list[slot];
-      if (j >= 0 && (slot == 0 || j > list[slot - 1])) {
-        const int64_t t0 = j * p.bt + c * G::C;
-        const int64_t lo = max((int64_t)0, st0 - t0), hi = min((int64_t)G::C, pos + 1 - t0);
+      const int j = list[slot];
+      if (j >= 0 && j <= last && (slot == 0 || j > list[slot - 1])) {
+        const int t0 = j * p.bt + c * G::C;
+        const int lo = max(0, st0 - t0), hi = min(G::C, pos + 1 - t0);
         if (lo < hi) {
-          const int64_t lp = t0 / p.cv.P;
-          const int jc = (int)(t0 - lp * p.cv.P) / G::C;
+          const int lp = (int)((unsigned)t0 / (unsigned)p.cv.P);
+          const int jc = (t0 - lp * p.cv.P) / G::C;
           src = p.blk + (table_page(p.cv, b, lp) * p.cv.H + h) * p.phs + (int64_t)jc * G::SLOT;
-          vlo = (int)lo;
-          vhi = (int)hi;
+          vlo = lo;
+          vhi = hi;
         }
       }
     }
@@ -263,7 +265,7 @@ __global__ void __launch_bounds__(kSW * 32, 2) sparse_kernel(const __grid_consta
   const int64_t T = sparse::launch_length(p.T, p.len_dev, p.q_len);
   if (T == 0 && blockIdx.x == 0 && threadIdx.x == 0) atomicExch(&g_sparse_fast_error, ERR_LENGTH);
   const int upc = kSW / p.w, gi = warp / p.w, rank = (int)(blockIdx.x % p.s);
-  const int64_t unit = (int64_t)(blockIdx.x / p.s) * upc + gi;
+  const unsigned unit = blockIdx.x / (unsigned)p.s * upc + gi;
   const bool live = unit < p.units;
   unsigned char *region = regions + warp * kWarpBytes;
   if (live && T > 0) {
@@ -278,11 +280,10 @@ __global__ void __launch_bounds__(kSW * 32, 2) sparse_kernel(const __grid_consta
   const int gt = p.w * 32, tid = threadIdx.x - gi * gt, Gq = p.gqa;
   const float *parts = (const float *)(regions + gi * p.w * kWarpBytes);
   constexpr int PS = kWarpBytes / 4;
-  const int64_t bh = live ? unit / p.q_len : 0;
-  const int qi = live ? (int)(unit - bh * p.q_len) : 0;
-  const int64_t Hq = (int64_t)p.cv.H * Gq, b = bh / p.cv.H, h = bh - b * p.cv.H;
+  const unsigned bh = unit / (unsigned)p.q_len;  // output rows [b][h * Gq + g][i]: (bh * Gq + g) * q_len + i
+  const int qi = (int)(unit - bh * (unsigned)p.q_len);
   auto finish = [&](int g, int d, float4 a, float M, float L) {
-    const int64_t row = (b * Hq + h * Gq + g) * p.q_len + qi;
+    const int64_t row = ((int64_t)bh * Gq + g) * p.q_len + qi;
     const float inv = L > 0.f ? 1.f / L : 0.f;
     store_from_float(p.out, row * HD + d, a.x * inv, p.out_dtype);
     store_from_float(p.out, row * HD + d + 1, a.y * inv, p.out_dtype);
@@ -412,10 +413,10 @@ static int pick_warps(int64_t units, int n, int sms) {
 
 }  // namespace fast
 
-bool sparse_fast_supported(const cq_paged_cache &c, int n_q_heads, int block_tokens) {
+bool sparse_fast_supported(const cq_paged_cache &c, int64_t T, int n_q_heads, int block_tokens) {
   int64_t phs;
   int index;
-  return fast::sparse_layout(c, n_q_heads, block_tokens, &phs, &index) != nullptr;
+  return T + block_tokens < (1LL << 31) && fast::sparse_layout(c, n_q_heads, block_tokens, &phs, &index) != nullptr;
 }
 
 int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
@@ -444,7 +445,9 @@ int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, 
   p.starts = starts;
   p.blocks = blocks;
   p.cpb = block_tokens / geo->C;
-  p.units = (int64_t)c.batch * c.kv_heads * q_len;
+  const int64_t units = (int64_t)c.batch * c.kv_heads * q_len;
+  CQ_REQUIRE(units < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_sparse_attention: too many query tokens");
+  p.units = (unsigned)units;
   p.out = out;
   p.out_dtype = out_dtype;
   p.lse_out = lse_out;

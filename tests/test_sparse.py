@@ -245,6 +245,8 @@ SELECT = [  # B, H, G, S, T, bt, top, first, recent
     (1, 1, 1, 1, 1, 16, 1, 0, 0), (1, 2, 4, 1, 40, 16, 2, 1, 1), (2, 2, 4, 1, 1000, 32, 8, 1, 2),
     (1, 2, 4, 7, 700, 64, 5, 1, 2), (1, 1, 8, 33, 300, 16, 6, 0, 1), (2, 1, 3, 2, 513, 32, 40, 2, 3),
     (1, 2, 2, 1, 5000, 16, 64, 1, 2), (1, 1, 4, 16, 16, 16, 3, 1, 1), (3, 1, 16, 1, 700, 64, 4, 0, 0),
+    (1, 2, 2, 3, 900, 16, 5, 2, 3), (1, 1, 1, 2, 9000, 16, 7, 7, 0), (1, 1, 2, 1, 20000, 16, 300, 1, 2),
+    (1, 2, 4, 600, 6000, 16, 20, 1, 2), (1, 1, 32, 2, 3000, 16, 9, 1, 1),
 ]
 
 
@@ -265,7 +267,40 @@ def test_select_equals_definition(shape, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("D", [8, 64, 72, 256])
+@pytest.mark.parametrize("T,top", [(140000, 64), (140000, 700), (270000, 40), (270000, 3000)])
+def test_select_long_rows(T, top):
+    """8750 blocks (a row in the registers of 18 warps) and 16875 (the radix
+    kernel), with lists shorter and longer than what one warp finishes."""
+    cache = make_cache(1, 1, T, 64, seed=T)
+    q = queries(1, 2, 1, 64, torch.float16)
+    index = BlockIndex(cache, 16).update()
+    n = index.n_blocks
+    got, s = index.select(q, top, return_scores=True)
+    ref, ref_s = ref_select(index.codes[:, :, :n].double(), index.scales[:, :, :n], q, T, 16, top, 1, 2)
+    assert torch.equal(got.cpu(), ref) and torch.equal(s.cpu(), ref_s)
+
+
+@gpu
+@pytest.mark.parametrize("blocks", [200, 700, 9000, 17000])
+def test_select_many_equal_scores(blocks):
+    """Two kinds of block only, more of each than any short list: whole
+    classes of equal keys at the threshold, the lowest indexes of them."""
+    k = torch.ones((1, 1, blocks * 16, 64), device="cuda").half()
+    k.view(1, 1, blocks, 16, 64)[:, :, ::3] = 2
+    cache = ChronoQuantCache()
+    cache.update_and_fetch(k, k)
+    index = BlockIndex(cache, 16)
+    q = torch.ones((1, 1, 1, 64), device="cuda").half()
+    for top in (10, blocks // 3 + 5, 4000):
+        if top > min(4096, blocks):
+            continue
+        got = index.select(q, top, first=1, recent=2).flatten().tolist()
+        order = sorted(range(blocks), key=lambda j: (not (j == 0 or j >= blocks - 2), j % 3 != 0, j))
+        assert got == sorted(order[:top])
+
+
+@gpu
+@pytest.mark.parametrize("D", [8, 32, 64, 72, 96, 256])
 def test_select_head_dims(D):
     cache = make_cache(2, 2, 600, D, seed=D)
     q = queries(2, 6, 3, D, torch.float16)
