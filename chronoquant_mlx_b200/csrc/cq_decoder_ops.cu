@@ -178,9 +178,9 @@ __device__ __forceinline__ void store_quad(void *p, int64_t i, const float4 v) {
 // other: with halves, lane l < rot/8 the quads at 4l and rot/2 + 4l; with
 // adjacent pairs, 8l and 8l + 4; lanes past the rotated channels take theirs in
 // order and keep them.  So a head needs no exchange between lanes but the sum of
-// squares.  A CTA takes `tile` tokens (a power of two): their angles once, in
-// shared memory; then each group of lanes keeps one token and walks its share
-// of the query heads, then of the key heads, UN heads' loads in flight, with the
+// squares.  A CTA takes TILE tokens; each group of lanes keeps one token, works out
+// its lanes' four angles (no exchange, no barrier) and walks its share of the
+// query heads, then of the key heads, UN heads' loads in flight, with the
 // products of norm weight and sine or cosine in registers: a pair (x, y) of a
 // head with root r becomes r (x wc - y ws'), r (y wc' + x ws).  Neighbouring
 // groups hold neighbouring tokens, whose output rows are contiguous.
@@ -189,23 +189,20 @@ struct PairTurn {  // coefficients of one pair: out0 = x * xc - y * ys, out1 = y
 };
 
 template <int DT, int D, int TILE>
-__global__ void __launch_bounds__(kRopeWarps * 32, 3) qk_norm_rope_quads_kernel(RopeArgs A) {
+__global__ void __launch_bounds__(kRopeWarps * 32, DT == CQ_F32 ? 3 : 4) qk_norm_rope_quads_kernel(RopeArgs A) {
   constexpr int LPH = D / 8, groups = kRopeWarps * 32 / LPH, DH = groups / TILE, UN = 4;
   using Raw = typename Quad<DT>::Raw;
   constexpr int ES = sizeof(Raw) / 4, ISTEP = DH * D * ES;  // bytes between two of a group's heads in a row
-  __shared__ float2 s_cs[TILE][D / 2];
   const unsigned tok0 = blockIdx.x * TILE, n_tok = (unsigned)A.B * (unsigned)A.S;  // below 2^31
   const int half = A.rot / 2;
-  for (int i = threadIdx.x; i < TILE * (D / 2); i += kRopeWarps * 32) {
-    const int tt = i / (D / 2), k = i - tt * (D / 2);
-    const unsigned tok = min(tok0 + tt, n_tok - 1), b = tok / (unsigned)A.S, s = tok - b * (unsigned)A.S;
-    if (k < half) s_cs[tt][k] = rope_angle(A.pos[b * A.p_sb + s * A.p_ss], A.inv_freq[k]);
-  }
   const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH;
   const int tt = group & (TILE - 1), h0 = group / TILE;
   const bool turns = l < A.rot / 8, halves = !A.adjacent && turns, live = tok0 + tt < n_tok;
   const int da = halves ? 4 * l : 8 * l, db = halves ? half + 4 * l : 8 * l + 4;
   const unsigned tok = min(tok0 + tt, n_tok - 1), b = tok / (unsigned)A.S, s = tok - b * (unsigned)A.S;
+  float2 cs[4];  // (cos, sin) of the lane's four pairs
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = make_float2(1.f, 0.f);
 #pragma unroll 1
   for (int part = (int)blockIdx.y; part < 2; part += (int)gridDim.y) {  // query heads, then key heads (or a CTA each)
     const int H = part ? A.Hkv : A.Hq;
@@ -223,29 +220,27 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) qk_norm_rope_quads_kernel(
       } else {
         ra[u] = rc[u] = Raw{};
       }
-    if (part == (int)blockIdx.y) __syncthreads();  // the angles
+    if (part == (int)blockIdx.y && turns) {  // under the first loads' latency
+      const int64_t at = A.pos[b * A.p_sb + s * A.p_ss];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cs[i] = rope_angle(at, A.inv_freq[4 * l + i]);
+    }
     PairTurn p[4];
     {
       const void *w = part ? A.wk : A.wq;
       float4 wa = make_float4(1.f, 1.f, 1.f, 1.f), wb = wa;
       if (w) wa = widen<DT>(load_quad<DT>(w, da)), wb = widen<DT>(load_quad<DT>(w, db));
-      float4 c01 = make_float4(1.f, 0.f, 1.f, 0.f), c23 = c01;  // cos, sin of the lane's four pairs
-      if (turns) {
-        const float4 *cs = (const float4 *)&s_cs[tt][4 * l];
-        c01 = cs[0];
-        c23 = cs[1];
-      }
-      auto turn = [](float wx, float wy, float cs, float sn) { return PairTurn{wx * cs, wy * sn, wy * cs, wx * sn}; };
+      auto turn = [](float wx, float wy, float2 a) { return PairTurn{wx * a.x, wy * a.y, wy * a.x, wx * a.y}; };
       if (!A.adjacent) {  // pairs (a.i, c.i)
-        p[0] = turn(wa.x, wb.x, c01.x, c01.y);
-        p[1] = turn(wa.y, wb.y, c01.z, c01.w);
-        p[2] = turn(wa.z, wb.z, c23.x, c23.y);
-        p[3] = turn(wa.w, wb.w, c23.z, c23.w);
+        p[0] = turn(wa.x, wb.x, cs[0]);
+        p[1] = turn(wa.y, wb.y, cs[1]);
+        p[2] = turn(wa.z, wb.z, cs[2]);
+        p[3] = turn(wa.w, wb.w, cs[3]);
       } else {  // pairs (a.x, a.y) (a.z, a.w) (c.x, c.y) (c.z, c.w)
-        p[0] = turn(wa.x, wa.y, c01.x, c01.y);
-        p[1] = turn(wa.z, wa.w, c01.z, c01.w);
-        p[2] = turn(wb.x, wb.y, c23.x, c23.y);
-        p[3] = turn(wb.z, wb.w, c23.z, c23.w);
+        p[0] = turn(wa.x, wa.y, cs[0]);
+        p[1] = turn(wa.z, wa.w, cs[1]);
+        p[2] = turn(wb.x, wb.y, cs[2]);
+        p[3] = turn(wb.z, wb.w, cs[3]);
       }
     }
     for (int base = 0; base < H; base += DH * UN) {  // the same trips for every lane: the sums are shuffles
