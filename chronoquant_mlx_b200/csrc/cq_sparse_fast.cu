@@ -392,17 +392,20 @@ static const SparseGeo *sparse_layout(const cq_paged_cache &c, int n_q_heads, in
 }
 
 // Warps per unit.  With W of them a unit takes about ceil(n / W) chunk times
-// plus a fixed part (lookups, query fragments, the merge), and the machine runs
-// 16 warps per SM at a time; the W with the least such time is taken.
+// plus a fixed part of about 2.5 (lookups, query fragments, the merge); the
+// machine runs 16 warps per SM at a time, and where that takes more than one
+// round the last one is half empty.  The W with the least such time is taken.
+// (4096 units of 32 chunks: 245, 221, 233, 261, 360 us with W = 1, 2, 4, 8, 16;
+// 128 units of 64: 42, 25.5, 25.0, 32 us with 4, 8, 16, 32; 8 units of 64: 17.3,
+// 12.2, 9.3, 7.9 us with 8, 16, 32, 64.)
 static int pick_warps(int64_t units, int n, int sms) {
-  const int fixed = 6;  // the fixed part in chunk times
-  const int64_t slots = (int64_t)sms * 2 * kSW;
+  const double slots = (double)sms * 2 * kSW;
   int best = 1;
   double best_t = 0;
   for (int W = 1; W <= kSW * kMaxCluster; W *= 2) {
     if (W > 1 && W > n) break;
-    const int64_t waves = (units * W + slots - 1) / slots;
-    const double t = (double)waves * ((n + W - 1) / W + fixed);
+    const double rounds = units * W / slots;
+    const double t = (rounds <= 1 ? 1 : rounds + 0.5) * ((n + W - 1) / W + 2.5);
     if (W == 1 || t < best_t) {
       best = W;
       best_t = t;

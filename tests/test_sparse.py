@@ -369,6 +369,8 @@ LAYOUTS = [dict(), dict(stride_k=64, stride_v=32, delta_bits_v=3), dict(stride_k
 SPARSE = [  # B, H, G, S, T, bt, top
     (1, 1, 1, 1, 1, 64, 1), (2, 2, 4, 1, 333, 64, 3), (1, 2, 8, 1, 2000, 64, 9), (1, 2, 4, 5, 700, 64, 4),
     (1, 1, 16, 2, 400, 128, 3), (2, 1, 3, 40, 257, 16, 5), (1, 2, 2, 1, 1500, 256, 4), (2, 1, 7, 3, 130, 48, 6),
+    (2, 2, 1, 21, 900, 64, 4), (1, 2, 2, 10, 1300, 64, 6), (1, 2, 3, 9, 1300, 64, 5), (1, 1, 4, 70, 1000, 64, 3),
+    (1, 1, 4, 2, 800, 64, 300),
 ]
 
 
@@ -467,6 +469,42 @@ def test_sparse_attention_padded_batch(kw):
     out = chronoquant_sparse_sdpa(q, cache, 0.09, blocks, index.block_tokens, starts=starts)
     check_attention(out, ref, vmax)
     assert not out[4].any() and not out[3, :, 0].any() and out[3, :, 1].any()
+
+
+@gpu
+@pytest.mark.parametrize("kw", [LAYOUTS[0], LAYOUTS[1], LAYOUTS[2], LAYOUTS[4], LAYOUTS[5]])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_infinite_values_stay_with_the_queries_that_see_them(kw, G):
+    """Query tokens that are computed together: a NaN or infinite value in a
+    block that only one of them lists, and in the newest token, which only the
+    last one sees, reaches that one's output and no other's."""
+    T, S = 500, 6
+    cache = make_cache(1, 1, T, 128, seed=3, **kw)
+    st = cache.state
+    st[1][0, 0, 64 // cache.stride_v, 5] = math.nan  # the V anchor of token 64: block 1
+    st[1][0, 0, 192 // cache.stride_v, 9] = math.inf  # of token 192: block 3
+    clean = ChronoQuantCache(**kw)
+    clean.state = [x.clone() for x in cache.state]
+    cache.state = st
+    q = queries(1, G, S, 128, torch.float16)
+    rows = [[0, 2, 7], [0, 1, 7], [2, 3, 7], [4, 5, 7], [0, 3, 7], [2, 4, 7]]
+    blocks = torch.tensor(rows, dtype=torch.int32, device="cuda").view(1, 1, S, 3)
+    got = chronoquant_sparse_sdpa(q, cache, 0.1, blocks, 64)
+    want = chronoquant_sparse_sdpa(q, clean, 0.1, blocks, 64)
+    for i, hit in enumerate((None, 5, 9, None, 9, None)):
+        if hit is None:
+            assert torch.equal(got[:, :, i], want[:, :, i])
+        else:
+            assert not torch.isfinite(got[0, :, i, hit]).any()
+    # the newest token: an I-frame at 448 with an infinite channel, seen by the last of 3 queries
+    short = ChronoQuantCache(**kw)
+    k, v = (torch.randn((1, 1, 449, 128), device="cuda").half() for _ in range(2))
+    if 448 % cache.stride_v == 0:
+        v[..., 448, 3] = math.inf
+        short.update_and_fetch(k, v)
+        qs, row = queries(1, G, 3, 128, torch.float16), torch.tensor([0, 3, 6, 7], dtype=torch.int32, device="cuda")
+        out = chronoquant_sparse_sdpa(qs, short, 0.1, row.expand(1, 1, 3, 4), 64)
+        assert torch.isfinite(out[:, :, :2]).all() and not torch.isfinite(out[0, :, 2, 3]).any()
 
 
 @gpu
