@@ -122,7 +122,7 @@ def _declare(lib):
         "cq_block_bounds_read": [P, P, I64, I64, I64, I64, I32, P, P],
         "cq_block_select": [P, P, I64, I32, I32, I32, I32, I64, P, P, ctypes.c_int, I32, I32, I64, I64, I64, P, I32,
                             I32, I32, P, P, P, SZ, P],
-        "cq_block_select_workspace": [I32, I32, I32, I64, I32, ctypes.POINTER(SZ)],
+        "cq_block_select_workspace": [I32, I32, I32, I32, I32, I64, I32, ctypes.POINTER(SZ)],
         "cq_sparse_attention": [C, I64, P, P, ctypes.c_int, I32, I32, I64, I64, I64, F, P, P, I32, I32, P,
                                 ctypes.c_int, P, P, SZ, P],
         "cq_sparse_attention_workspace": [C, I64, I32, I32, I32, I32, ctypes.POINTER(SZ)],

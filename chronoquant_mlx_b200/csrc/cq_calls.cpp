@@ -286,7 +286,7 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::Tensor starts = starts_of(a[8], ix.B, dev, "select");
     const bool want = PyObject_IsTrue(a[9]) == 1;
     size_t need = 0;
-    check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, q.S, T, bt, &need), "select");
+    check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, q.S, T, bt, &need), "select");
     at::Tensor blocks = at::empty({ix.B, ix.H, q.S, top}, ix.codes.options().dtype(at::kInt)), scores, ws;
     if (want) scores = at::empty({ix.B, ix.H, q.S, top}, ix.scales.options());
     if (need) ws = at::empty({(int64_t)need}, ix.codes.options());

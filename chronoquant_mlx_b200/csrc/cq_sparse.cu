@@ -335,33 +335,27 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
 // with the codes as fp16, whose fragments cost conversions, 47 us).
 constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
 
-template <int KS, int GP>
-__global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(SelectArgs A, int tiles, int passes) {
-  constexpr int D = KS * 32, STR = 2 * D + 64, TPT = 16 / GP;  // query tokens per row tile
-  extern __shared__ __align__(16) unsigned char s_a[];  // [tiles * 16][STR], then fp32 [tiles * 16]
-  float *s_sg = (float *)(s_a + tiles * 16 * STR);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int64_t unit = blockIdx.z;
-  const int b = (int)(unit / A.H), h = (int)(unit - (int64_t)b * A.H);
-  const int i0 = blockIdx.y * tiles * TPT;
-  ptx::grid_dependency_wait();
-  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
-  if (T == 0) return;
-  // query rows of this warp: r, r + 8, ...; four rows' loads in flight
-  for (int r0 = warp; r0 < tiles * 16; r0 += 4 * kScoreWarps) {
-    float x[4][KS];
+// Query rows [0, rows) of a unit from token i0 on into shared memory, by WARPS warps.
+template <int KS, int GP, int WARPS>
+__device__ __forceinline__ void quantise_rows(const SelectArgs &A, unsigned unit, int i0, int rows, unsigned char *s_a,
+                                              float *s_sg) {
+  constexpr int D = KS * 32, STR = 2 * D + 64, UN = WARPS > 8 ? 1 : 4;  // rows whose loads are in flight
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = (int)(unit / (unsigned)A.H), h = (int)(unit - (unsigned)b * (unsigned)A.H);
+  for (int r0 = warp; r0 < rows; r0 += UN * WARPS) {
+    float x[UN][KS];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int r = r0 + u * kScoreWarps, i = i0 + r / GP, hd = r & (GP - 1);
-      const bool real = r < tiles * 16 && i < A.q_len && hd < A.G;
+    for (int u = 0; u < UN; ++u) {
+      const int r = r0 + u * WARPS, i = i0 + r / GP, hd = r & (GP - 1);
+      const bool real = r < rows && i < A.q_len && hd < A.G;
       const int64_t qb = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq;
 #pragma unroll
       for (int k = 0; k < KS; ++k) x[u][k] = real ? load_as_float(A.q, qb + lane * KS + k, A.q_dtype) : 0.f;
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int r = r0 + u * kScoreWarps;
-      if (r >= tiles * 16) break;
+    for (int u = 0; u < UN; ++u) {
+      const int r = r0 + u * WARPS;
+      if (r >= rows) break;
       float amax = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -379,102 +373,131 @@ __global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(Selec
       if (lane == 0) s_sg[r] = qs.s;
     }
   }
+}
+
+// A warp's two column tiles: the B fragments of blocks j0 .. j0 + 15 and their scales.
+template <int KS>
+struct BlockCodes {
+  uint4 bf[2][KS];
+  float sj[2][2];
+  __device__ __forceinline__ BlockCodes(const SelectArgs &A, unsigned unit, int j0) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, last = (int)A.n - 1;
+    const int8_t *codes = A.codes + (int64_t)unit * A.max_blocks * (2 * KS * 32);
+    const float *scales = A.scales + (int64_t)unit * A.max_blocks;
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      const int8_t *src = codes + (int64_t)min(j0 + nb * 8 + g, last) * (2 * KS * 32) + 16 * t;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) bf[nb][k] = *(const uint4 *)(src + 64 * k);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) sj[nb][e] = scales[min(j0 + nb * 8 + 2 * t + e, last)];
+    }
+  }
+};
+
+// Scores of one row tile (its codes at a_tile, its scales at sg_tile; its first
+// token is i) against blocks j0 .. j0 + 15: token tok's go to dst[tok * ns].
+template <int KS, int GP>
+__device__ __forceinline__ void score_tile(const SelectArgs &A, const BlockCodes<KS> &f, const unsigned char *a_tile,
+                                           const float *sg_tile, int i, int j0, float *dst) {
+  constexpr int STR = 2 * KS * 32 + 64;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const bool pad0 = (g & (GP - 1)) >= A.G, pad1 = ((g + 8) & (GP - 1)) >= A.G;
+  int acc[2][4] = {};
+  const unsigned char *a = a_tile + g * STR + 16 * t;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const uint4 x = *(const uint4 *)(a + 64 * k), y = *(const uint4 *)(a + 8 * STR + 64 * k);
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb) {
+      mma_s8_16832(acc[nb], x.x, y.x, x.y, y.y, f.bf[nb][k].x, f.bf[nb][k].y);
+      mma_s8_16832(acc[nb], x.z, y.z, x.w, y.w, f.bf[nb][k].z, f.bf[nb][k].w);
+    }
+  }
+  const float sg0 = sg_tile[g], sg1 = sg_tile[g + 8];
+  // v[column tile][row half][column]: scores of rows g and g + 8
+  float v[2][2][2];
+#pragma unroll
+  for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = __fmul_rn(__fmul_rn(sg0, f.sj[nb][e]), (float)acc[nb][e]);
+      const float y = __fmul_rn(__fmul_rn(sg1, f.sj[nb][e]), (float)acc[nb][2 + e]);
+      v[nb][0][e] = pad0 ? -INFINITY : __fadd_rn(x, 0.f);  // -0 becomes +0: equal scores have equal keys
+      v[nb][1][e] = pad1 ? -INFINITY : __fadd_rn(y, 0.f);
+    }
+  auto swap_max = [&](float &keep, float give, int o) { keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o)); };
+  int nb0 = 0, hf0 = 0;  // which of the values this lane holds
+  if constexpr (GP == 16) {
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[nb][0][e] = fmaxf(v[nb][0][e], v[nb][1][e]);
+  }
+  if constexpr (GP >= 2) {  // heads in lane bit 2: keep one column tile
+    nb0 = g & 1;
+#pragma unroll
+    for (int hf = 0; hf < (GP == 16 ? 1 : 2); ++hf)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float a0 = v[0][hf][e], a1 = v[1][hf][e];
+        v[0][hf][e] = nb0 ? a1 : a0;
+        swap_max(v[0][hf][e], nb0 ? a0 : a1, 4);
+      }
+  }
+  if constexpr (GP == 4 || GP == 8) {  // heads in lane bit 3: keep one row half
+    hf0 = (g >> 1) & 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float a0 = v[0][0][e], a1 = v[0][1][e];
+      v[0][0][e] = hf0 ? a1 : a0;
+      swap_max(v[0][0][e], hf0 ? a0 : a1, 8);
+    }
+  }
+  if constexpr (GP == 16)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 8));
+  if constexpr (GP >= 8)  // heads in lane bit 4
+#pragma unroll
+    for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 16));
+  // token (in the tile) of the lane's row g, and of row g + 8: 8 / GP further on
+  const int ta = g / GP;
+  constexpr int NBV = GP >= 2 ? 1 : 2, HFV = GP == 1 || GP == 2 ? 2 : 1;
+#pragma unroll
+  for (int nb = 0; nb < NBV; ++nb)
+#pragma unroll
+    for (int hf = 0; hf < HFV; ++hf) {
+      const int tok = ta + (HFV == 2 ? hf : hf0) * (8 / GP), col = (NBV == 2 ? nb : nb0) * 8 + 2 * t;
+      bool mine = i + tok < A.q_len && j0 + col < (int)A.ns;
+      if (GP >= 8) mine = mine && !(g & 4);
+      if (GP == 16) mine = mine && !(g & 2);
+      if (mine) *(float2 *)(dst + tok * A.ns + col) = make_float2(v[nb][hf][0], v[nb][hf][1]);
+    }
+}
+
+template <int KS, int GP>
+__global__ void __launch_bounds__(kScoreWarps * 32) block_score_mma_kernel(SelectArgs A, int tiles, int passes) {
+  constexpr int STR = 2 * KS * 32 + 64, TPT = 16 / GP;  // query tokens per row tile
+  extern __shared__ __align__(16) unsigned char s_a[];  // [tiles * 16][STR], then fp32 [tiles * 16]
+  float *s_sg = (float *)(s_a + tiles * 16 * STR);
+  const unsigned unit = blockIdx.z;
+  const int i0 = blockIdx.y * tiles * TPT;
+  ptx::grid_dependency_wait();
+  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+  if (T == 0) return;
+  quantise_rows<KS, GP, kScoreWarps>(A, unit, i0, tiles * 16, s_a, s_sg);
   __syncthreads();
   // the last block any of this CTA's tokens sees
   const int i_last = min(A.q_len, i0 + tiles * TPT) - 1;
   const int j_end = (int)min((unsigned)A.n, (unsigned)(T - A.q_len + i_last) / (unsigned)A.bt + 1u);  // T below 2^31
   const int real_tiles = (i_last - i0) / TPT + 1;
-  const int8_t *codes = A.codes + unit * A.max_blocks * 2 * D;
-  const float *scales = A.scales + unit * A.max_blocks;
-  const bool pad0 = (g & (GP - 1)) >= A.G, pad1 = ((g + 8) & (GP - 1)) >= A.G;
   for (int pass = 0; pass < passes; ++pass) {
-    const int j0 = (int)((blockIdx.x * passes + pass) * kScoreWarps + warp) * kScoreCols;
+    const int j0 = (int)((blockIdx.x * passes + pass) * kScoreWarps + (threadIdx.x >> 5)) * kScoreCols;
     if (j0 >= j_end) break;
-    uint4 bf[2][KS];
-    float sj[2][2];
-#pragma unroll
-    for (int nb = 0; nb < 2; ++nb) {
-      const int8_t *src = codes + (int64_t)min(j0 + nb * 8 + g, (int)A.n - 1) * 2 * D + 16 * t;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) bf[nb][k] = *(const uint4 *)(src + 64 * k);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) sj[nb][e] = scales[min(j0 + nb * 8 + 2 * t + e, (int)A.n - 1)];
-    }
-    float *dst = A.score + (unit * A.q_len + i0) * A.ns + j0;  // of this row tile's first token
-    for (int rt = 0; rt < real_tiles; ++rt, dst += TPT * A.ns) {
-      int acc[2][4] = {};
-      const unsigned char *a = s_a + (rt * 16 + g) * STR + 16 * t;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const uint4 x = *(const uint4 *)(a + 64 * k), y = *(const uint4 *)(a + 8 * STR + 64 * k);
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb) {
-          mma_s8_16832(acc[nb], x.x, y.x, x.y, y.y, bf[nb][k].x, bf[nb][k].y);
-          mma_s8_16832(acc[nb], x.z, y.z, x.w, y.w, bf[nb][k].z, bf[nb][k].w);
-        }
-      }
-      const float sg0 = s_sg[rt * 16 + g], sg1 = s_sg[rt * 16 + g + 8];
-      // v[column tile][row half][column]: scores of rows g and g + 8
-      float v[2][2][2];
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float x = __fmul_rn(__fmul_rn(sg0, sj[nb][e]), (float)acc[nb][e]);
-          const float y = __fmul_rn(__fmul_rn(sg1, sj[nb][e]), (float)acc[nb][2 + e]);
-          v[nb][0][e] = pad0 ? -INFINITY : __fadd_rn(x, 0.f);  // -0 becomes +0: equal scores have equal keys
-          v[nb][1][e] = pad1 ? -INFINITY : __fadd_rn(y, 0.f);
-        }
-      auto swap_max = [&](float &keep, float give, int o) {
-        keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o));
-      };
-      int nb0 = 0, hf0 = 0;  // which of the values this lane holds
-      if constexpr (GP == 16) {
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) v[nb][0][e] = fmaxf(v[nb][0][e], v[nb][1][e]);
-      }
-      if constexpr (GP >= 2) {  // heads in lane bit 2: keep one column tile
-        nb0 = g & 1;
-#pragma unroll
-        for (int hf = 0; hf < (GP == 16 ? 1 : 2); ++hf)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float a0 = v[0][hf][e], a1 = v[1][hf][e];
-            v[0][hf][e] = nb0 ? a1 : a0;
-            swap_max(v[0][hf][e], nb0 ? a0 : a1, 4);
-          }
-      }
-      if constexpr (GP == 4 || GP == 8) {  // heads in lane bit 3: keep one row half
-        hf0 = (g >> 1) & 1;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float a0 = v[0][0][e], a1 = v[0][1][e];
-          v[0][0][e] = hf0 ? a1 : a0;
-          swap_max(v[0][0][e], hf0 ? a0 : a1, 8);
-        }
-      }
-      if constexpr (GP == 16)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 8));
-      if constexpr (GP >= 8)  // heads in lane bit 4
-#pragma unroll
-        for (int e = 0; e < 2; ++e) v[0][0][e] = fmaxf(v[0][0][e], __shfl_xor_sync(0xffffffffu, v[0][0][e], 16));
-      // token (in the tile) of the lane's row g, and of row g + 8: 8 / GP further on
-      const int ta = g / GP, i = i0 + rt * TPT;
-      constexpr int NBV = GP >= 2 ? 1 : 2, HFV = GP == 1 || GP == 2 ? 2 : 1;
-#pragma unroll
-      for (int nb = 0; nb < NBV; ++nb)
-#pragma unroll
-        for (int hf = 0; hf < HFV; ++hf) {
-          const int tok = ta + (HFV == 2 ? hf : hf0) * (8 / GP), col = (NBV == 2 ? nb : nb0) * 8 + 2 * t;
-          bool mine = i + tok < A.q_len && j0 + col < (int)A.ns;
-          if (GP >= 8) mine = mine && !(g & 4);
-          if (GP == 16) mine = mine && !(g & 2);
-          if (mine) *(float2 *)(dst + tok * A.ns + col) = make_float2(v[nb][hf][0], v[nb][hf][1]);
-        }
-    }
+    const BlockCodes<KS> f(A, unit, j0);
+    float *dst = A.score + ((int64_t)unit * A.q_len + i0) * A.ns + j0;  // of this row tile's first token
+    for (int rt = 0; rt < real_tiles; ++rt, dst += TPT * A.ns)
+      score_tile<KS, GP>(A, f, s_a + rt * 16 * STR, s_sg + rt * 16, i0 + rt * TPT, j0, dst);
   }
 }
 
@@ -558,21 +581,24 @@ __device__ __forceinline__ int warp_prefix(int *v, int n, int lane) {
   return all;
 }
 
-template <int KPT, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
-  __shared__ uint32_t s_key[kShort];
-  __shared__ int s_idx[kShort];
-  __shared__ int s_hist[THREADS > 128 ? 256 : 1];
-  __shared__ int s_cnt[4];
-  __shared__ int s_pre[KPT * 32 < 64 ? 64 : KPT * 32];
-  ptx::grid_dependency_wait();
-  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+template <int KPT, bool HIST>
+struct TopkShared {
+  uint32_t key[kShort];
+  int idx[kShort];
+  int hist[HIST ? 256 : 1];
+  int cnt[4];
+  int pre[KPT * 32 < 64 ? 64 : KPT * 32];
+};
+
+// Row `row` (unit * q_len + query token) with its scores at `score`, by the CTA's
+// first W warps (named barrier 1); HIST: W may exceed four.
+template <int KPT, bool HIST>
+__device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigned row, const float *score, int W,
+                                         TopkShared<KPT, HIST> &sh) {
+  uint32_t *s_key = sh.key;
+  int *s_idx = sh.idx, *s_hist = sh.hist, *s_cnt = sh.cnt, *s_pre = sh.pre;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const unsigned row = blockIdx.x;
-  if (T == 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
-    return;
-  }
+  auto meet = [&]() { ptx::named_barrier_sync(1, W * 32); };
   // 32-bit positions (the launch keeps T there): a 64-bit division takes a hundred instructions
   const unsigned unit = row / (unsigned)A.q_len, bt = (unsigned)A.bt;
   const int b = (int)(unit / (unsigned)A.H);
@@ -580,7 +606,6 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
   const unsigned st = (unsigned)min(first_token(A.starts, b), (int64_t)INT32_MAX);
   const int fb = (int)(st / bt), lb = (int)(p / bt);
   const int nv = st > p ? 0 : lb - fb + 1;
-  const float *score = A.score + (int64_t)row * A.ns;
   int32_t *out = A.blocks + (int64_t)row * A.top;
   float *out_s = A.block_scores ? A.block_scores + (int64_t)row * A.top : nullptr;
   const int tid = warp * 32 + lane, step = W * 32;
@@ -608,10 +633,10 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     all_and = __reduce_and_sync(0xffffffffu, all_and);
     if (W > 1) {
       if (lane == 0) s_pre[2 * warp] = (int)all_or, s_pre[2 * warp + 1] = (int)all_and;
-      __syncthreads();
+      meet();
       all_or = __reduce_or_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane] : 0u);
       all_and = __reduce_and_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane + 1] : 0xffffffffu);
-      __syncthreads();  // s_pre is written again below
+      meet();  // s_pre is written again below
     }
     const uint32_t differ = all_or & ~all_and;  // first + recent <= top < nv: some key is not forced
     bit = differ ? 31 - __clz(differ) : -1;
@@ -619,7 +644,7 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     const bool shorten = A.top <= kShort;
     int above = A.first + A.recent;  // keys above those in question (all of them visible: nv > top)
     if (above == A.top) thr = 0xffffffffu, reach = A.top, bit = -1;  // the forced blocks fill the list
-    if constexpr (THREADS <= 128) {
+    if (!HIST || W <= 4) {
       int par = 0;
       for (; bit >= 0 && reach != A.top && !(shorten && reach <= kShort); --bit) {
         const uint32_t cand = thr | (1u << bit);
@@ -629,24 +654,24 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
         c = __reduce_add_sync(0xffffffffu, c);
         if (W > 1) {
           if (lane == 0) s_pre[par * 4 + warp] = c;
-          __syncthreads();
+          meet();
           c = __reduce_add_sync(0xffffffffu, lane < W ? s_pre[par * 4 + lane] : 0);
           par ^= 1;
         }
         if (c >= A.top) thr = cand, reach = c;
       }
-      if (W > 1) __syncthreads();  // s_pre is written again below
+      if (W > 1) meet();  // s_pre is written again below
     }
-    while (THREADS > 128 && bit >= 0 && reach != A.top && !(shorten && reach <= kShort)) {
+    while (HIST && W > 4 && bit >= 0 && reach != A.top && !(shorten && reach <= kShort)) {
       const int shift = max(bit - 7, 0), bins = 2 << (bit - shift);  // up to 8 bits
       for (int k = tid; k < 256; k += step) s_hist[k] = 0;
-      __syncthreads();
+      meet();
       const uint32_t prefix = bit >= 31 ? 0u : thr >> (bit + 1);
 #pragma unroll
       for (int k = 0; k < KPT; ++k)
         if (key[k] != 0u && key[k] != 0xffffffffu && (bit >= 31 || key[k] >> (bit + 1) == prefix))
           atomicAdd(&s_hist[(key[k] >> shift) & (bins - 1)], 1);
-      __syncthreads();
+      meet();
       if (warp == 0) {  // the highest bin that brings the count to `top`: lane l holds bins 8l .. 8l + 7
         int c[8], sum = 0;
 #pragma unroll
@@ -666,7 +691,7 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
           s_cnt[2] = over + c[e];
         }
       }
-      __syncthreads();
+      meet();
       thr |= (uint32_t)s_cnt[0] << shift;
       above = s_cnt[1];
       reach = s_cnt[2];
@@ -681,9 +706,9 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
         const unsigned in = __ballot_sync(0xffffffffu, key[k] >= max(thr, 1u));
         if (lane == 0) s_pre[k * W + warp] = __popc(in);
       }
-      __syncthreads();
+      meet();
       if (warp == 0) warp_prefix<KPT>(s_pre, KPT * W, lane);
-      __syncthreads();
+      meet();
     }
 #pragma unroll
     for (int k = 0; k < KPT; ++k) {
@@ -696,10 +721,7 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
         s_idx[at] = fb + k * step + tid;
       }
     }
-    if (W > 1)
-      __syncthreads();
-    else
-      __syncwarp();
+    meet();
     if (warp != 0) return;
     constexpr int N = kShort / 32;
     uint32_t kk[N];
@@ -749,12 +771,12 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
     all_gt += __popc(gt);
   }
   if (W > 1) {
-    __syncthreads();
+    meet();
     if (warp == 0) {
       const int all = warp_prefix<KPT>(s_pre, KPT * W, lane);
       if (lane == 0) s_cnt[0] = all;
     }
-    __syncthreads();
+    meet();
     all_gt = s_cnt[0] & 0xffff;
   }
   const int need = A.top - all_gt;  // equal keys to take
@@ -772,6 +794,52 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
       if (out_s) out_s[at] = score[j];
     }
     if (W == 1) running += __shfl_sync(0xffffffffu, mine, k);
+  }
+}
+
+template <int KPT, int THREADS>
+__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
+  __shared__ TopkShared<KPT, (THREADS > 128)> sh;
+  ptx::grid_dependency_wait();
+  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+  if (T == 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+    return;
+  }
+  topk_row<KPT, (THREADS > 128)>(A, T, blockIdx.x, A.score + (int64_t)blockIdx.x * A.ns, W, sh);
+}
+
+// Scores and lists of one unit by one CTA, for a decode step's few query tokens
+// (one row tile) and up to kOneBlocks blocks: the scores stay in shared memory,
+// one launch and no workspace.
+constexpr int kOneWarps = 16, kOneBlocks = 2048;
+
+template <int KS, int GP>
+__global__ void __launch_bounds__(kOneWarps * 32) block_select_one_kernel(SelectArgs A) {
+  constexpr int STR = 2 * KS * 32 + 64;
+  extern __shared__ __align__(16) unsigned char s_a[];  // int8 [16][STR], fp32 [16], fp32 scores [q_len][ns]
+  __shared__ TopkShared<4, true> sh;
+  float *s_sg = (float *)(s_a + 16 * STR), *s_score = s_sg + 16;
+  const unsigned unit = blockIdx.x;
+  ptx::grid_dependency_wait();
+  const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
+  if (T == 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+    return;
+  }
+  quantise_rows<KS, GP, kOneWarps>(A, unit, 0, 16, s_a, s_sg);
+  __syncthreads();
+  const int warp = threadIdx.x >> 5, j_end = (int)((unsigned)(T - 1) / (unsigned)A.bt) + 1;
+  for (int j0 = warp * kScoreCols; j0 < j_end; j0 += kOneWarps * kScoreCols) {
+    const BlockCodes<KS> f(A, unit, j0);
+    score_tile<KS, GP>(A, f, s_a, s_sg, 0, j0, s_score + j0);
+  }
+  __syncthreads();
+  const int W = (j_end + 127) / 128;  // four keys a thread
+  if (warp >= W) return;
+  for (int i = 0; i < A.q_len; ++i) {
+    if (i) ptx::named_barrier_sync(1, W * 32);
+    topk_row<4, true>(A, T, unit * (unsigned)A.q_len + i, s_score + i * A.ns, W, sh);
   }
 }
 
@@ -1066,18 +1134,46 @@ extern "C" int cq_block_bounds_read(const int8_t *codes, const float *scales, in
   return check_launch("cq_block_bounds_read");
 }
 
-static int select_sizes(int32_t batch, int32_t kv_heads, int32_t q_len, int64_t T, int32_t block_tokens,
-                        size_t *bytes) {
+// The form of a selection: the head groups' power of two (its log), whether the tensor-core kernels take it, whether
+// one CTA per unit does it all.
+struct SelectForm {
+  int lg = 0;
+  bool mma = false, one = false;
+  int64_t n = 0, ns = 0;
+  size_t bytes = 0;  // workspace
+};
+
+static int select_form(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t n_q_heads, int32_t q_len, int64_t T,
+                       int32_t block_tokens, SelectForm &f) {
   CQ_REQUIRE(batch >= 1 && kv_heads >= 1 && block_tokens >= 1, CQ_ERR_INVALID, "cq_block_select: bad sizes");
+  CQ_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, CQ_ERR_UNSUPPORTED,
+             "cq_block_select: head_dim must be a multiple of 8 in [8, 256]");
+  CQ_REQUIRE(n_q_heads >= 1 && n_q_heads % kv_heads == 0, CQ_ERR_INVALID,
+             "cq_block_select: n_q_heads must be a positive multiple of kv_heads");
   CQ_REQUIRE(q_len >= 1 && q_len <= T, CQ_ERR_INVALID, "cq_block_select: need 1 <= q_len <= T");
-  *bytes = (size_t)batch * kv_heads * q_len * (((T + block_tokens - 1) / block_tokens + 7) & ~7LL) * sizeof(float);
+  f.n = (T + block_tokens - 1) / block_tokens;
+  CQ_REQUIRE(f.n < (1LL << 30), CQ_ERR_INVALID, "cq_block_select: too many blocks");
+  f.ns = (f.n + 7) & ~7LL;
+  const int G = n_q_heads / kv_heads;
+  while ((1 << f.lg) < G) ++f.lg;
+  const int64_t units = (int64_t)batch * kv_heads;
+  f.mma = (head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256) && G <= 16 && units < 65536 &&
+          T < (1LL << 31);
+  // one CTA scores up to 256 blocks a pass; longer rows want the whole machine unless there are units for it
+  f.one = f.mma && (q_len << f.lg) <= 16 && f.n <= sparse::kOneBlocks && q_len * f.ns <= 8192 &&
+          (f.n <= 512 || 2 * units >= sm_count());
+  f.bytes = f.one ? 0 : (size_t)units * q_len * f.ns * sizeof(float);
   return CQ_OK;
 }
 
-extern "C" int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t q_len, int64_t T,
-                                         int32_t block_tokens, size_t *bytes) {
+extern "C" int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t n_q_heads,
+                                         int32_t q_len, int64_t T, int32_t block_tokens, size_t *bytes) {
   CQ_REQUIRE(bytes, CQ_ERR_INVALID, "cq_block_select_workspace: bytes is null");
-  return select_sizes(batch, kv_heads, q_len, T, block_tokens, bytes);
+  SelectForm f;
+  int r = select_form(batch, kv_heads, head_dim, n_q_heads, q_len, T, block_tokens, f);
+  if (r) return r;
+  *bytes = f.bytes;
+  return CQ_OK;
 }
 
 // A launch that may start while the kernel before it in the stream drains (it
@@ -1100,21 +1196,27 @@ static int launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, c
   return check_launch(what);
 }
 
-static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
+// One entry per head size (64, 96, 128, 256) and power of two of the group.
+static int size_index(int D) { return D == 64 ? 0 : D == 96 ? 1 : D == 128 ? 2 : 3; }
+#define CQ_BY_GROUP(K, KS) {K<KS, 1>, K<KS, 2>, K<KS, 4>, K<KS, 8>, K<KS, 16>}
+#define CQ_BY_SIZE(K) {CQ_BY_GROUP(K, 2), CQ_BY_GROUP(K, 3), CQ_BY_GROUP(K, 4), CQ_BY_GROUP(K, 8)}
+
+static int launch_one(const sparse::SelectArgs &A, const SelectForm &f, cudaStream_t st) {
+  using namespace sparse;
+  using Fn = void (*)(SelectArgs);
+  static const Fn table[4][5] = CQ_BY_SIZE(block_select_one_kernel);
+  const size_t smem = 16 * (2 * A.D + 64 + 4) + (size_t)A.q_len * A.ns * sizeof(float);  // below 43 KB
+  return launch_after(table[size_index(A.D)][f.lg], dim3((unsigned)(A.B * A.H)), kOneWarps * 32, smem, st,
+                      "cq_block_select", A);
+}
+
+static int launch_scores(const sparse::SelectArgs &A, const SelectForm &f, cudaStream_t st) {
   using namespace sparse;
   const int64_t rows = (int64_t)A.B * A.H * A.q_len, units = (int64_t)A.B * A.H;
-  if ((A.D == 64 || A.D == 96 || A.D == 128 || A.D == 256) && A.G <= 16 && aligned16(A.codes) && aligned16(A.score) &&
-      units < 65536 && A.T < (1LL << 31)) {
-    int lg = 0;
-    while ((1 << lg) < A.G) ++lg;
+  if (f.mma) {
     using Fn = void (*)(SelectArgs, int, int);
-#define CQ_SCORE(KS)                                                                                           \
-  {block_score_mma_kernel<KS, 1>, block_score_mma_kernel<KS, 2>, block_score_mma_kernel<KS, 4>,                \
-   block_score_mma_kernel<KS, 8>, block_score_mma_kernel<KS, 16>}
-    static const Fn table[4][5] = {CQ_SCORE(2), CQ_SCORE(3), CQ_SCORE(4), CQ_SCORE(8)};
-#undef CQ_SCORE
-    const Fn fn = table[A.D == 64 ? 0 : A.D == 96 ? 1 : A.D == 128 ? 2 : 3][lg];
-    const int tpt = 16 >> lg, row_tiles = (A.q_len + tpt - 1) / tpt;
+    static const Fn table[4][5] = CQ_BY_SIZE(block_score_mma_kernel);
+    const int tpt = 16 >> f.lg, row_tiles = (A.q_len + tpt - 1) / tpt;
     // A CTA's rows are quantised once for all its columns, so it takes many columns as soon as there are two
     // CTAs per SM without splitting them; few row tiles, so that this happens early
     const int tiles = std::min(row_tiles, 4);
@@ -1125,8 +1227,8 @@ static int launch_scores(const sparse::SelectArgs &A, cudaStream_t st) {
     const int64_t split = std::max<int64_t>(1, std::min<int64_t>(cols, 2 * sm_count() / (groups * units)));
     const int passes = (int)((cols + split - 1) / split);
     const dim3 grid((unsigned)((cols + passes - 1) / passes), (unsigned)groups, (unsigned)units);
-    return launch_after(fn, grid, kScoreWarps * 32, (size_t)tiles * 16 * (2 * A.D + 64 + 4), st, "cq_block_select", A,
-                        tiles, passes);
+    return launch_after(table[size_index(A.D)][f.lg], grid, kScoreWarps * 32,
+                        (size_t)tiles * 16 * (2 * A.D + 64 + 4), st, "cq_block_select", A, tiles, passes);
   }
   const int64_t grid = (rows * A.n * 32 + 255) / 256;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many scores");
@@ -1158,29 +1260,27 @@ extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t
                                int64_t q_sh, int64_t q_sq, const int64_t *starts, int32_t first, int32_t recent,
                                int32_t top, int32_t *blocks, float *block_scores, void *workspace,
                                size_t workspace_bytes, void *stream) {
-  size_t need = 0;
-  int r = select_sizes(batch, kv_heads, q_len, T, block_tokens, &need);
+  SelectForm f;
+  int r = select_form(batch, kv_heads, head_dim, n_q_heads, q_len, T, block_tokens, f);
   if (r) return r;
   CQ_REQUIRE(codes && scales && q && blocks, CQ_ERR_INVALID, "cq_block_select: null pointer");
-  CQ_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, CQ_ERR_UNSUPPORTED,
-             "cq_block_select: head_dim must be a multiple of 8 in [8, 256]");
+  CQ_REQUIRE(aligned16(codes), CQ_ERR_INVALID, "cq_block_select: codes must be 16-byte aligned");
   CQ_REQUIRE(q_dtype == CQ_F16 || q_dtype == CQ_BF16, CQ_ERR_UNSUPPORTED, "cq_block_select: q dtype must be f16/bf16");
-  CQ_REQUIRE(n_q_heads >= 1 && n_q_heads % kv_heads == 0, CQ_ERR_INVALID,
-             "cq_block_select: n_q_heads must be a positive multiple of kv_heads");
   CQ_REQUIRE(first >= 0 && recent >= 0 && top >= 1 && first <= top && recent <= top - first, CQ_ERR_INVALID,
              "cq_block_select: need first + recent <= top");
   CQ_REQUIRE(top <= sparse::kMaxTop, CQ_ERR_UNSUPPORTED, "cq_block_select: top must be <= 4096");
-  const int64_t n = (T + block_tokens - 1) / block_tokens;
-  CQ_REQUIRE(n <= max_blocks && n < (1LL << 30), CQ_ERR_INVALID, "cq_block_select: T beyond the summarised blocks");
-  CQ_REQUIRE(workspace && workspace_bytes >= need, CQ_ERR_WORKSPACE, "cq_block_select: workspace too small");
+  CQ_REQUIRE(f.n <= max_blocks, CQ_ERR_INVALID, "cq_block_select: T beyond the summarised blocks");
+  CQ_REQUIRE(f.bytes == 0 || (workspace && workspace_bytes >= f.bytes), CQ_ERR_WORKSPACE,
+             "cq_block_select: workspace too small");
+  CQ_REQUIRE(f.bytes == 0 || aligned16(workspace), CQ_ERR_INVALID, "cq_block_select: workspace must be 16-byte aligned");
   sparse::SelectArgs A{codes,  scales, max_blocks, block_tokens, batch, kv_heads, head_dim, n_q_heads / kv_heads,
                        q_len,  T,      len_dev,    q,            q_dtype, q_sb,   q_sh,     q_sq,
-                       starts, first,  recent,     top,          blocks,  block_scores,     n, (n + 7) & ~7LL, (float *)workspace};
-  const int64_t rows = (int64_t)batch * kv_heads * q_len;
+                       starts, first,  recent,     top,          blocks,  block_scores,     f.n, f.ns, (float *)workspace};
   cudaStream_t st = (cudaStream_t)stream;
-  r = launch_scores(A, st);
+  if (f.one) return launch_one(A, f, st);
+  r = launch_scores(A, f, st);
   if (r) return r;
-  return launch_topk(A, rows, st);
+  return launch_topk(A, (int64_t)batch * kv_heads * q_len, st);
 }
 
 static int sparse_checks(const cq_paged_cache *cache, int64_t T, int32_t n_q_heads, int32_t q_len, int32_t top,

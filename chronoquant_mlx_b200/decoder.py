@@ -339,8 +339,8 @@ class Qwen3StyleDecoder:
             _lib.check(lib.cq_sparse_attention_workspace(d, self.max_len, self.heads, 1, sp["top"], sp["block_tokens"],
                                                          ctypes.byref(need)), "decoder")
             most = max(most, need.value)
-        _lib.check(lib.cq_block_select_workspace(self.B, self.kv_heads, 1, self.max_len, sp["block_tokens"],
-                                                 ctypes.byref(need)), "decoder")
+        _lib.check(lib.cq_block_select_workspace(self.B, self.kv_heads, self.cfg.head_dim, self.heads, 1, self.max_len,
+                                                 sp["block_tokens"], ctypes.byref(need)), "decoder")
         self.sparse_ws = torch.empty(max(most, need.value), dtype=torch.uint8, device=self.device)
         self.blocks = torch.empty((self.B, self.kv_heads, 1, sp["top"]), dtype=torch.int32, device=self.device)
 

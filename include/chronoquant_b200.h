@@ -410,9 +410,10 @@ int cq_block_bounds_read(const int8_t *codes, const float *scales, int64_t units
  * block_scores (optional): fp32, the listed blocks' scores, -inf behind.  q as
  * in cq_attention.  T: tokens summarised; with len_dev (may be NULL) the
  * length is read from device memory and T is the largest it may be.
- * workspace: cq_block_select_workspace bytes, contents ignored. */
-int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t q_len, int64_t T, int32_t block_tokens,
-                              size_t *bytes);
+ * workspace: cq_block_select_workspace bytes (0 for a decode step's few rows,
+ * else 4 per query token, kv-head and block), 16-byte aligned, contents ignored. */
+int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t n_q_heads, int32_t q_len,
+                              int64_t T, int32_t block_tokens, size_t *bytes);
 int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens, int32_t batch,
                     int32_t kv_heads, int32_t head_dim, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
                     int32_t n_q_heads, int32_t q_len, int64_t q_sb, int64_t q_sh, int64_t q_sq, const int64_t *starts,

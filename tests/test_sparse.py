@@ -660,7 +660,7 @@ def _desc(**over):
 
 P = 0x10000  # a pointer that the refused calls never follow
 BOUNDS = dict(t0=0, T=1000, bt=64, codes=P, scales=P, max_blocks=16)
-SELECT_ARGS = dict(codes=P, scales=P, max_blocks=16, bt=64, B=2, H=8, D=128, T=1000, len=None, q=P, dt=0, Hq=32, S=1,
+SELECT_ARGS = dict(codes=P, scales=P, max_blocks=16, bt=64, B=2, H=8, D=72, T=1000, len=None, q=P, dt=0, Hq=32, S=1,
                    sb=4096, sh=128, sq=128, starts=None, first=1, recent=2, top=8, blocks=P, scores=None, ws=P,
                    nws=1 << 20)
 SPARSE_ARGS = dict(T=1000, len=None, q=P, dt=0, Hq=32, S=1, sb=4096, sh=128, sq=128, scale=1.0, starts=None, blocks=P,
@@ -684,7 +684,8 @@ def test_c_bounds_refusals(over, status):
     (dict(codes=None), -1), (dict(q=None), -1), (dict(blocks=None), -1), (dict(dt=2), -2), (dict(D=12), -2),
     (dict(D=264), -2), (dict(Hq=12), -1), (dict(Hq=0), -1), (dict(S=0), -1), (dict(S=1001), -1), (dict(top=0), -1),
     (dict(top=2), -1), (dict(first=-1), -1), (dict(recent=-1), -1), (dict(top=4097), -2), (dict(max_blocks=15), -1),
-    (dict(ws=None), -4), (dict(nws=8), -4), (dict(bt=0), -1), (dict(B=0), -1), (dict(recent=2 ** 31 - 1), -1)])
+    (dict(ws=None), -4), (dict(nws=8), -4), (dict(bt=0), -1), (dict(B=0), -1), (dict(recent=2 ** 31 - 1), -1),
+    (dict(codes=P + 8), -1), (dict(ws=P + 4), -1)])
 def test_c_select_refusals(over, status):
     assert _lib.lib().cq_block_select(*{**SELECT_ARGS, **over}.values(), None) == status
 
