@@ -330,9 +330,12 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
 // `passes`, keeping two column tiles' codes in registers over the rows.  The
 // maximum over a group's heads goes by halves: each exchange also halves the
 // values a lane holds, so every lane ends with its own ones to store.  Bound by
-// the tensor pipe: mma.sync runs at about 512 multiply-adds a clock and SM here,
-// for int8 as for fp16 (2048 rows x 1024 blocks x 256 codes x 8 units: 34 us;
-// with the codes as fp16, whose fragments cost conversions, 47 us).
+// latency and issue, not by the tensor pipe: a row tile against 16 blocks is
+// about 220 instructions, 16 of them products, and 14 warps an SM issue in 46 %
+// of the slots.  2048 rows x 1024 blocks x 256 codes x 8 units take 30 us; with
+// the codes as fp16, whose fragments cost conversions, 47 us.  One launch that
+// also lists, with the scores in shared memory, takes 64 us there against 54 us
+// for this kernel and the next: too few warps fit beside the scores.
 constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
 
 // Query rows [0, rows) of a unit from token i0 on into shared memory, by WARPS warps.
@@ -811,7 +814,9 @@ __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, 
 
 // Scores and lists of one unit by one CTA, for a decode step's few query tokens
 // (one row tile) and up to kOneBlocks blocks: the scores stay in shared memory,
-// one launch and no workspace.
+// one launch and no workspace.  Bound by latency (a launch, the codes' loads, the
+// search's meetings): one sequence of 8192 tokens 5.9 us, 8.5 us as two kernels;
+// 16 of 32768 tokens 7.7 us, 10.4 us as two kernels.
 constexpr int kOneWarps = 16, kOneBlocks = 2048;
 
 template <int KS, int GP>
@@ -1192,7 +1197,10 @@ static int launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, c
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
-  if (e != cudaSuccess) return set_error(CQ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the next call
+    return set_error(CQ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  }
   return check_launch(what);
 }
 

@@ -488,7 +488,10 @@ int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, 
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, geo->fn, p);
-  if (e != cudaSuccess) return set_error(CQ_ERR_CUDA, std::string("cq_sparse_attention: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // reported here, not by the next call
+    return set_error(CQ_ERR_CUDA, std::string("cq_sparse_attention: ") + cudaGetErrorString(e));
+  }
   return check_launch("cq_sparse_attention");
 }
 
