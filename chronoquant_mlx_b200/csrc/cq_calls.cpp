@@ -285,12 +285,12 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Queries q = queries(tensor(a[4], "queries"), ix.B, ix.H, ix.D, T, dev, "select");
     const at::Tensor starts = starts_of(a[8], ix.B, dev, "select");
     const bool want = PyObject_IsTrue(a[9]) == 1;
+    const Launch at_(ix.codes);
     size_t need = 0;
     check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, q.S, T, bt, &need), "select");
     at::Tensor blocks = at::empty({ix.B, ix.H, q.S, top}, ix.codes.options().dtype(at::kInt)), scores, ws;
     if (want) scores = at::empty({ix.B, ix.H, q.S, top}, ix.scales.options());
     if (need) ws = at::empty({(int64_t)need}, ix.codes.options());
-    const Launch at_(ix.codes);
     check(L.select((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.cap, bt,
                    (int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S,
                    q.sb, q.sh, q.sq, starts_ptr(starts), first, recent, top, blocks.mutable_data_ptr<int32_t>(),

@@ -417,6 +417,7 @@ extern "C" int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t
              "cq_qk_norm_rope_rows: give both norm weights or neither");
   CQ_REQUIRE(batch >= 0 && tokens >= 0 && n_q_heads >= 1 && n_kv_heads >= 1, CQ_ERR_INVALID,
              "cq_qk_norm_rope_rows: bad sizes");
+  CQ_REQUIRE(n_q_heads < (1 << 20) && n_kv_heads < (1 << 20), CQ_ERR_UNSUPPORTED, "cq_qk_norm_rope_rows: too many heads");
   CQ_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, CQ_ERR_UNSUPPORTED,
              "cq_qk_norm_rope_rows: head_dim must be a multiple of 8 in [8, 256]");
   CQ_REQUIRE(rot_dim >= 0 && rot_dim <= head_dim && rot_dim % 2 == 0, CQ_ERR_INVALID,

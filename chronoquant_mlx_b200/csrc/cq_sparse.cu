@@ -1078,9 +1078,10 @@ static int bounds_checks(const cq_paged_cache *cache, int64_t T, int32_t bt, con
   const std::string w(what);
   CQ_REQUIRE(codes && scales, CQ_ERR_INVALID, w + ": null pointer");
   CQ_REQUIRE(bt >= 1, CQ_ERR_INVALID, w + ": block_tokens must be >= 1");
-  CQ_REQUIRE(T >= 1 && (T + cache->page_tokens - 1) / cache->page_tokens <= cache->max_pages, CQ_ERR_INVALID,
+  CQ_REQUIRE(T >= 1 && T <= (int64_t)cache->max_pages * cache->page_tokens, CQ_ERR_INVALID,
              w + ": tokens beyond the mapped pages (or none)");
-  CQ_REQUIRE((T + bt - 1) / bt <= max_blocks, CQ_ERR_INVALID, w + ": max_blocks too small");
+  CQ_REQUIRE((T - 1) / bt < max_blocks, CQ_ERR_INVALID, w + ": max_blocks too small");
+  CQ_REQUIRE((T - 1) / bt < (1LL << 30), CQ_ERR_UNSUPPORTED, w + ": too many blocks");
   return CQ_OK;
 }
 
@@ -1132,8 +1133,8 @@ extern "C" int cq_block_bounds_read(const int8_t *codes, const float *scales, in
   CQ_REQUIRE(units >= 1 && first >= 0 && n >= 0 && n <= max_blocks - first && head_dim >= 8 && head_dim <= 256,
              CQ_ERR_INVALID, "cq_block_bounds_read: bad sizes");
   if (n == 0) return CQ_OK;
-  const int64_t grid = (units * n * 32 + 255) / 256;
-  CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_INVALID, "cq_block_bounds_read: grid too large");
+  CQ_REQUIRE(n <= (1LL << 33) / units, CQ_ERR_INVALID, "cq_block_bounds_read: grid too large");
+  const int64_t grid = (units * n + 7) / 8;  // a warp per block
   sparse::bounds_read_kernel<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(codes, scales, units, max_blocks, first,
                                                                               n, head_dim, out);
   return check_launch("cq_block_bounds_read");
@@ -1156,16 +1157,18 @@ static int select_form(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_
   CQ_REQUIRE(n_q_heads >= 1 && n_q_heads % kv_heads == 0, CQ_ERR_INVALID,
              "cq_block_select: n_q_heads must be a positive multiple of kv_heads");
   CQ_REQUIRE(q_len >= 1 && q_len <= T, CQ_ERR_INVALID, "cq_block_select: need 1 <= q_len <= T");
-  f.n = (T + block_tokens - 1) / block_tokens;
+  f.n = (T - 1) / block_tokens + 1;
   CQ_REQUIRE(f.n < (1LL << 30), CQ_ERR_INVALID, "cq_block_select: too many blocks");
   f.ns = (f.n + 7) & ~7LL;
   const int G = n_q_heads / kv_heads;
-  while ((1 << f.lg) < G) ++f.lg;
+  while ((1LL << f.lg) < G) ++f.lg;
   const int64_t units = (int64_t)batch * kv_heads;
+  CQ_REQUIRE(units < (1LL << 31) && units * q_len < (1LL << 31), CQ_ERR_UNSUPPORTED,
+             "cq_block_select: too many query tokens");
   f.mma = (head_dim == 64 || head_dim == 96 || head_dim == 128 || head_dim == 256) && G <= 16 && units < 65536 &&
           T < (1LL << 31);
   // one CTA scores up to 256 blocks a pass; longer rows want the whole machine unless there are units for it
-  f.one = f.mma && (q_len << f.lg) <= 16 && f.n <= sparse::kOneBlocks && q_len * f.ns <= 8192 &&
+  f.one = f.mma && ((int64_t)q_len << f.lg) <= 16 && f.n <= sparse::kOneBlocks && q_len * f.ns <= 8192 &&
           (f.n <= 512 || 2 * units >= sm_count());
   f.bytes = f.one ? 0 : (size_t)units * q_len * f.ns * sizeof(float);
   return CQ_OK;
@@ -1238,7 +1241,7 @@ static int launch_scores(const sparse::SelectArgs &A, const SelectForm &f, cudaS
     return launch_after(table[size_index(A.D)][f.lg], grid, kScoreWarps * 32,
                         (size_t)tiles * 16 * (2 * A.D + 64 + 4), st, "cq_block_select", A, tiles, passes);
   }
-  const int64_t grid = (rows * A.n * 32 + 255) / 256;
+  const int64_t grid = (rows * A.n + 7) / 8;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many scores");
   block_score_kernel<<<(unsigned)grid, 256, 0, st>>>(A);
   return check_launch("cq_block_select");
@@ -1246,7 +1249,6 @@ static int launch_scores(const sparse::SelectArgs &A, const SelectForm &f, cudaS
 
 static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t st) {
   using namespace sparse;
-  CQ_REQUIRE(rows < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
   // A CTA per row, four keys a thread; where rows abound eight (up to four warps), whose rounds cost fewer meetings
   int kpt = rows >= 4 * sm_count() && A.n > 128 ? 8 : 4;
   while (kpt < 16 && A.n > (int64_t)kpt * 32 * 32) kpt *= 2;
@@ -1298,8 +1300,11 @@ static int sparse_checks(const cq_paged_cache *cache, int64_t T, int32_t n_q_hea
   CQ_REQUIRE(n_q_heads >= 1 && n_q_heads % cache->kv_heads == 0, CQ_ERR_INVALID,
              "cq_sparse_attention: n_q_heads must be a positive multiple of kv_heads");
   CQ_REQUIRE(q_len >= 1 && q_len <= T, CQ_ERR_INVALID, "cq_sparse_attention: need 1 <= q_len <= T");
-  CQ_REQUIRE((T + cache->page_tokens - 1) / cache->page_tokens <= cache->max_pages, CQ_ERR_INVALID,
+  CQ_REQUIRE(T <= (int64_t)cache->max_pages * cache->page_tokens, CQ_ERR_INVALID,
              "cq_sparse_attention: T beyond mapped pages");
+  const int64_t heads = (int64_t)cache->batch * n_q_heads;
+  CQ_REQUIRE(heads < (1LL << 31) && heads * q_len < (1LL << 31), CQ_ERR_UNSUPPORTED,
+             "cq_sparse_attention: too many query tokens");
   CQ_REQUIRE(top >= 1 && bt >= 1, CQ_ERR_INVALID, "cq_sparse_attention: bad list length or block_tokens");
   CQ_REQUIRE(top <= sparse::kMaxTop, CQ_ERR_UNSUPPORTED, "cq_sparse_attention: at most 4096 blocks per list");
   return CQ_OK;

@@ -448,9 +448,7 @@ int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, 
   p.starts = starts;
   p.blocks = blocks;
   p.cpb = block_tokens / geo->C;
-  const int64_t units = (int64_t)c.batch * c.kv_heads * q_len;
-  CQ_REQUIRE(units < (1LL << 31), CQ_ERR_UNSUPPORTED, "cq_sparse_attention: too many query tokens");
-  p.units = (unsigned)units;
+  p.units = (unsigned)((int64_t)c.batch * c.kv_heads * q_len);  // below 2^31 (the caller's check of the query rows)
   p.out = out;
   p.out_dtype = out_dtype;
   p.lse_out = lse_out;
@@ -469,8 +467,10 @@ int run_sparse_fast(const cq_paged_cache &c, int64_t T, const int64_t *len_dev, 
     std::lock_guard<std::mutex> lk(mu);
     if (dev < 0 || dev >= 64 || !attr_set[dev][gi]) {
       cudaError_t e = cudaFuncSetAttribute(geo->fn, cudaFuncAttributeMaxDynamicSharedMemorySize, geo->smem);
-      if (e != cudaSuccess)
+      if (e != cudaSuccess) {
+        cudaGetLastError();
         return set_error(CQ_ERR_CUDA, std::string("cq_sparse_attention: ") + cudaGetErrorString(e));
+      }
       if (dev >= 0 && dev < 64) attr_set[dev][gi] = true;
     }
   }

@@ -167,3 +167,8 @@ def test_c_refusals(over, status):
 
 def test_c_nothing_to_do():
     assert _lib.lib().cq_qk_norm_rope_rows(*{**ARGS, "B": 0}.values(), None) == 0
+
+
+def test_c_too_many_heads():
+    for over in (dict(Hq=2 ** 31 - 1), dict(Hkv=2 ** 30)):
+        assert _lib.lib().cq_qk_norm_rope_rows(*{**ARGS, **over}.values(), None) == -2

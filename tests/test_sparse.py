@@ -704,3 +704,21 @@ def test_c_bounds_read_refusals():
                  (P, P, 16, 16, 13, 4, 128, P), (P, P, 0, 16, 0, 4, 128, P), (P, P, 16, 16, 0, 4, 300, P),
                  (P, P, 16, 16, 0, 4, 128, None)):
         assert L.cq_block_bounds_read(*args, None) == -1
+
+
+def test_c_sizes_past_32_bits_are_refused():
+    L, n, big = _lib.lib(), ctypes.c_size_t(), 2 ** 31 - 1
+    far = ctypes.byref(_desc(max_pages=big))  # maps 2^39 tokens
+    for T in (2 ** 62, 2 ** 63 - 1):  # sums with a page's or a block's tokens would wrap
+        assert L.cq_block_bounds(far, 0, T, 64, P, P, 2 ** 40, None) == -1
+        assert L.cq_block_bounds_at(far, P, T, 1, 64, P, P, 2 ** 40, None) == -1
+        assert L.cq_block_select(*{**SELECT_ARGS, "T": T, "max_blocks": 2 ** 62}.values(), None) == -1
+        assert L.cq_sparse_attention(far, *{**SPARSE_ARGS, "T": T}.values(), None) == -1
+    assert L.cq_block_bounds(far, 0, 2 ** 39 - 256, 64, P, P, 2 ** 40, None) == -2  # 2^33 blocks
+    # groups of 2^30 heads and more, and rows past 2^31
+    assert L.cq_block_select_workspace(1, 1, 128, big, 1, 64, 64, ctypes.byref(n)) == 0 and n.value
+    assert L.cq_block_select_workspace(big, big, 128, big, 1, 64, 64, ctypes.byref(n)) == -2
+    assert L.cq_block_select_workspace(1, 2, 128, 2, 2 ** 30, 2 ** 31, 64, ctypes.byref(n)) == -2
+    for over in (dict(Hq=2 ** 30), dict(S=2 ** 28, T=2 ** 29)):
+        assert L.cq_sparse_attention(far, *{**SPARSE_ARGS, **over}.values(), None) == -2
+    assert L.cq_block_bounds_read(P, P, 2 ** 40, 2 ** 40, 0, 2 ** 40, 128, P, None) == -1
