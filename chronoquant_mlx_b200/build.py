@@ -73,7 +73,7 @@ def build_calls(force: bool = False) -> str:
     tmp = CALLS_OUT + ".tmp"
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, CALLS_SRC, "-o", tmp, "-L", lib,
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-ldl"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {CALLS_SRC}:\n{r.stderr}")

@@ -2,11 +2,12 @@
 // operators in C++: argument checks, output allocation, stream lookup and the
 // call of the C library in one step.  A decode step's kernels run for 3 to 10 us;
 // checked in Python and called through ctypes such a call took 11 to 18 us of
-// host time, from here 5 to 7.  The module holds no kernels and keeps nothing
+// host time, from here 5.  The module holds no kernels and keeps nothing
 // between calls; the C functions come from the library that load() is given.
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -134,6 +135,11 @@ at::Tensor starts_of(PyObject *o, int64_t B, c10::Device device, const char *wha
 }
 const int64_t *starts_ptr(const at::Tensor &s) { return s.defined() ? s.const_data_ptr<int64_t>() : nullptr; }
 
+// An uninitialised contiguous tensor: torch's own CUDA allocation, without its dispatcher's way there.
+at::Tensor empty(at::IntArrayRef size, at::ScalarType type, c10::Device device) {
+  return at::detail::empty_cuda(size, type, device, c10::nullopt);
+}
+
 PyObject *pair(at::Tensor a, at::Tensor b) {
   PyObject *x = THPVariable_Wrap(std::move(a)), *y = x ? THPVariable_Wrap(std::move(b)) : nullptr;
   if (!y) {
@@ -215,7 +221,7 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const bool full = p_in.dim() == 2 && p_in.size(0) == B && p_in.size(1) == S;
     const at::Tensor pos = full ? p_in : p_in.expand({B, S});
     const at::Tensor qkv = qkv_in.stride(2) == 1 ? qkv_in : qkv_in.contiguous(), f = f_in.contiguous();
-    at::Tensor q = at::empty({B, Hq, S, D}, qkv.options()), k = at::empty({B, Hkv, S, D}, qkv.options());
+    at::Tensor q = empty({B, Hq, S, D}, st, dev), k = empty({B, Hkv, S, D}, st, dev);
     const Launch at_(qkv);
     check(L.rope(qkv.const_data_ptr(), qkv.stride(0), qkv.stride(1), (int32_t)B, (int32_t)S, Hq, Hkv, (int32_t)D,
                  (int32_t)(2 * half), PyObject_IsTrue(a[8]) ? 1 : 0, w[0].defined() ? w[0].const_data_ptr() : nullptr,
@@ -261,7 +267,7 @@ PyObject *block_bounds_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 4, [](PyObject *const *a) {
     const Index ix(a[0], a[1]);
     const int64_t first = integer(a[2]), m = integer(a[3]);
-    at::Tensor out = at::empty({ix.B, ix.H, m, 2, ix.D}, ix.scales.options());
+    at::Tensor out = empty({ix.B, ix.H, m, 2, ix.D}, at::kFloat, ix.codes.device());
     const Launch at_(ix.codes);
     check(L.bounds_read((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.B * ix.H,
                         ix.cap, first, m, (int32_t)ix.D, out.mutable_data_ptr<float>(), at_.stream),
@@ -288,9 +294,9 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Launch at_(ix.codes);
     size_t need = 0;
     check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, q.S, T, bt, &need), "select");
-    at::Tensor blocks = at::empty({ix.B, ix.H, q.S, top}, ix.codes.options().dtype(at::kInt)), scores, ws;
-    if (want) scores = at::empty({ix.B, ix.H, q.S, top}, ix.scales.options());
-    if (need) ws = at::empty({(int64_t)need}, ix.codes.options());
+    at::Tensor blocks = empty({ix.B, ix.H, q.S, top}, at::kInt, dev), scores, ws;
+    if (want) scores = empty({ix.B, ix.H, q.S, top}, at::kFloat, dev);
+    if (need) ws = empty({(int64_t)need}, at::kByte, dev);
     check(L.select((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.cap, bt,
                    (int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S,
                    q.sb, q.sh, q.sq, starts_ptr(starts), first, recent, top, blocks.mutable_data_ptr<int32_t>(),
@@ -326,12 +332,12 @@ PyObject *sparse_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::Tensor starts = starts_of(a[7], B, dev, what), blocks = b_in.contiguous();
     const bool want = PyObject_IsTrue(a[8]) == 1;
     at::Tensor out, lse, ws;
-    out = at::empty({B, q.Hq, q.S, D}, want ? q.t.options().dtype(at::kFloat) : q.t.options());
-    if (want) lse = at::empty({B, q.Hq, q.S}, out.options());
+    out = empty({B, q.Hq, q.S, D}, want ? at::kFloat : q.t.scalar_type(), dev);
+    if (want) lse = empty({B, q.Hq, q.S}, at::kFloat, dev);
     const Launch at_(pool);
     size_t need = 0;
     check(L.sparse_ws(d, T, q.Hq, q.S, (int32_t)top, (int32_t)bt, &need), what);
-    if (need) ws = at::empty({(int64_t)need}, pool.options());
+    if (need) ws = empty({(int64_t)need}, at::kByte, dev);
     check(L.sparse(d, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S, q.sb, q.sh, q.sq, (float)real(a[4]),
                    starts_ptr(starts), blocks.const_data_ptr<int32_t>(), (int32_t)top, (int32_t)bt,
                    out.mutable_data_ptr(), want ? CQ_F32 : q.dtype, want ? lse.mutable_data_ptr<float>() : nullptr,

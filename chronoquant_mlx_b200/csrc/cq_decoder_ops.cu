@@ -16,6 +16,8 @@
 // torch op.  Only the order of the fp32 sum of squares differs from torch's
 // reduction, so a value can land one dtype ulp away.
 #include "cq_common.cuh"
+#include "cq_launch.cuh"
+#include "cq_ptx.cuh"
 
 namespace cq {
 namespace dec {
@@ -195,6 +197,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, DT == CQ_F32 ? 3 : 4) qk_norm
   constexpr int LPH = D / 8, groups = kRopeWarps * 32 / LPH, DH = groups / TILE, UN = 4;
   using Raw = typename Quad<DT>::Raw;
   constexpr int ES = sizeof(Raw) / 4, ISTEP = DH * D * ES;  // bytes between two of a group's heads in a row
+  ptx::grid_dependency_wait();
   const unsigned tok0 = blockIdx.x * TILE, n_tok = (unsigned)A.B * (unsigned)A.S;  // below 2^31
   const int half = A.rot / 2;
   const int l = threadIdx.x & (LPH - 1), group = threadIdx.x / LPH;
@@ -312,6 +315,7 @@ template <int DT>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_rows_kernel(RopeArgs A) {
   __shared__ float2 s_cs[128];              // (cos, sin) of each pair
   __shared__ float s_x[kRopeWarps][256];    // a head's normalised channels
+  ptx::grid_dependency_wait();
   const int64_t tok = blockIdx.x;
   const int b = (int)(tok / A.S), s = (int)(tok - (int64_t)b * A.S);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -451,12 +455,10 @@ extern "C" int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t
                      : (tiled ? dec::qk_norm_rope_quads_kernel<DT, 256, 8> : dec::qk_norm_rope_quads_kernel<DT, 256, 1>))
     auto *fn = dtype == CQ_F16 ? CQ_ROPE(CQ_F16) : dtype == CQ_BF16 ? CQ_ROPE(CQ_BF16) : CQ_ROPE(CQ_F32);
 #undef CQ_ROPE
-    fn<<<grid, dec::kRopeWarps * 32, 0, st>>>(A);
-    return check_launch("cq_qk_norm_rope_rows");
+    return launch_after(fn, grid, dec::kRopeWarps * 32, 0, st, "cq_qk_norm_rope_rows", A);
   }
   auto *fn = dtype == CQ_F16    ? dec::qk_norm_rope_rows_kernel<CQ_F16>
              : dtype == CQ_BF16 ? dec::qk_norm_rope_rows_kernel<CQ_BF16>
                                 : dec::qk_norm_rope_rows_kernel<CQ_F32>;
-  fn<<<(unsigned)n, dec::kRopeWarps * 32, 0, st>>>(A);
-  return check_launch("cq_qk_norm_rope_rows");
+  return launch_after(fn, dim3((unsigned)n), dec::kRopeWarps * 32, 0, st, "cq_qk_norm_rope_rows", A);
 }

@@ -19,6 +19,7 @@
 #include <string>
 #include <type_traits>
 
+#include "cq_launch.cuh"
 #include "cq_prefill.cuh"
 #include "cq_ptx.cuh"
 #include "cq_sparse.cuh"
@@ -72,6 +73,7 @@ __device__ __forceinline__ void store_codes(int8_t *codes, int d, int D, float l
 
 __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
   __shared__ float s_red[8];
+  ptx::grid_dependency_wait();
   const CacheView &cv = A.cv;
   int64_t T = A.T, t0 = A.t0;
   if (A.len_dev) {
@@ -147,6 +149,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
   constexpr int W = D / 8, RPI = 32 / W;  // words (lanes) per row, rows at once
   constexpr int UN = 8;                   // steps whose loads are in flight
   const int lane = threadIdx.x & 31;
+  ptx::grid_dependency_wait();
   const CacheView &cv = A.cv;
   const CompView &c = cv.c[0];
   int64_t T = A.T, t0 = A.t0;
@@ -267,6 +270,7 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
 __global__ void __launch_bounds__(256) bounds_read_kernel(const int8_t *codes, const float *scales, int64_t units,
                                                           int64_t max_blocks, int64_t first, int64_t n, int D,
                                                           float *out) {
+  ptx::grid_dependency_wait();
   const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   if (row >= units * n) return;
   const int64_t u = row / n, j = first + (row - u * n);
@@ -1098,12 +1102,10 @@ static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const cha
     auto *fn = D == 64    ? sparse::block_bounds_rows_kernel<64>
                : D == 128 ? sparse::block_bounds_rows_kernel<128>
                           : sparse::block_bounds_rows_kernel<256>;
-    fn<<<(unsigned)((grid + 3) / 4), 128, 0, st>>>(A, (unsigned)grid);
-    return check_launch(what);
+    return launch_after(fn, dim3((unsigned)((grid + 3) / 4)), 128, 0, st, what, A, (unsigned)grid);
   }
   const int threads = (A.cv.D + 31) & ~31;
-  sparse::block_bounds_kernel<<<(unsigned)grid, threads, 0, st>>>(A);
-  return check_launch(what);
+  return launch_after(sparse::block_bounds_kernel, dim3((unsigned)grid), threads, 0, st, what, A);
 }
 
 extern "C" int cq_block_bounds(const cq_paged_cache *cache, int64_t t0, int64_t T, int32_t block_tokens, int8_t *codes,
@@ -1136,9 +1138,8 @@ extern "C" int cq_block_bounds_read(const int8_t *codes, const float *scales, in
   if (n == 0) return CQ_OK;
   CQ_REQUIRE(n <= (1LL << 33) / units, CQ_ERR_INVALID, "cq_block_bounds_read: grid too large");
   const int64_t grid = (units * n + 7) / 8;  // a warp per block
-  sparse::bounds_read_kernel<<<(unsigned)grid, 256, 0, (cudaStream_t)stream>>>(codes, scales, units, max_blocks, first,
-                                                                              n, head_dim, out);
-  return check_launch("cq_block_bounds_read");
+  return launch_after(sparse::bounds_read_kernel, dim3((unsigned)grid), 256, 0, (cudaStream_t)stream,
+                      "cq_block_bounds_read", codes, scales, units, max_blocks, first, n, head_dim, out);
 }
 
 // The form of a selection: the head groups' power of two (its log), whether the tensor-core kernels take it, whether
@@ -1183,29 +1184,6 @@ extern "C" int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_
   if (r) return r;
   *bytes = f.bytes;
   return CQ_OK;
-}
-
-// A launch that may start while the kernel before it in the stream drains (it
-// waits for that kernel's results itself).
-template <class... P, class... X>
-static int launch_after(void (*fn)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, const char *what,
-                        X... args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
-  if (e != cudaSuccess) {
-    cudaGetLastError();  // reported here, not by the next call
-    return set_error(CQ_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-  }
-  return check_launch(what);
 }
 
 // One entry per head size (64, 96, 128, 256) and power of two of the group.
