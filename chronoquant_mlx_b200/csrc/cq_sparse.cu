@@ -551,107 +551,140 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 }
 
 // The `top` best visible blocks of a (unit, query token) row with every key in a
-// register: W warps hold KPT keys a thread.  The threshold key is found from the
-// highest bit on which the row's keys differ: with up to four warps bit by bit
-// (count the keys that reach a candidate), with more of them, whose meetings
-// cost more, eight bits at a time by a histogram of the keys still in question.
-// As soon as no more than kShort keys reach the threshold so far, those are
-// gathered in index order in shared memory, and one warp goes on with them
-// alone, bit by bit (ranking them against each other instead took 3 us more).
-// Where that never happens (long lists, many equal keys) the search runs to the
-// last bit.  The list is written in index order, of equal keys the lowest
-// indexes.
+// register: W warps, each thread with the keys of KPT blocks next to each other.
+// First a threshold is guessed that some more than `top` keys reach, from the
+// scores' mean and deviation: one count settles it for scores that look normal,
+// where a search bit by bit takes a dozen (512 queries x 1024 blocks x 8 units, 32
+// of each: 26 us without, 21 us with it).  If four guesses miss, the threshold key
+// is found from the highest bit on which the row's keys differ: with up to four
+// warps bit by bit (count the keys that reach a candidate), with more of them,
+// whose meetings cost more, eight bits at a time by a histogram of the keys still
+// in question.  As soon as no more than kShort keys reach the threshold so far,
+// those are gathered in index order in shared memory, and one warp goes on with
+// them alone, two bits at a time (ranking them against each other instead took 3
+// us more).  Where that never happens (long lists, many equal keys) the search
+// runs to the last bit.  The list is written in index order, of equal keys the
+// lowest indexes.  Keys of neighbouring blocks in a thread make the positions a sum
+// over threads (keys dealt out in turn, with a count per warp and turn: 21 us,
+// this: 15 us).
 constexpr int kShort = 128;
 
-// Exclusive prefix of `n` (at most 32 * PER) packed counts in shared memory, in
-// place, by one warp; returns the sum.
-template <int PER>
-__device__ __forceinline__ int warp_prefix(int *v, int n, int lane) {
-  int sum = 0;
-#pragma unroll
-  for (int e = 0; e < PER; ++e)
-    if (lane * PER + e < n) sum += v[lane * PER + e];
-  int before = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
-  }
-  const int all = __shfl_sync(0xffffffffu, before, 31);
-  before -= sum;
-#pragma unroll
-  for (int e = 0; e < PER; ++e)
-    if (lane * PER + e < n) {
-      const int x = v[lane * PER + e];
-      v[lane * PER + e] = before;
-      before += x;
-    }
-  return all;
-}
-
-template <int KPT, bool HIST>
+template <bool HIST>
 struct TopkShared {
   uint32_t key[kShort];
   int idx[kShort];
   int hist[HIST ? 256 : 1];
   int cnt[4];
-  int pre[KPT * 32 < 64 ? 64 : KPT * 32];
+  __align__(16) int pre[128];  // four a warp
 };
 
-// Row `row` (unit * q_len + query token) with its scores at `score`, by the CTA's
-// first W warps (named barrier 1); HIST: W may exceed four.
+// Query token i of a unit with its scores at `score` (16-byte aligned), by the
+// CTA's first W warps (named barrier 1); HIST: W may exceed four.
 template <int KPT, bool HIST>
-__device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigned row, const float *score, int W,
-                                         TopkShared<KPT, HIST> &sh) {
+__device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigned unit, int i, const float *score, int W,
+                                         TopkShared<HIST> &sh) {
   uint32_t *s_key = sh.key;
   int *s_idx = sh.idx, *s_hist = sh.hist, *s_cnt = sh.cnt, *s_pre = sh.pre;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto meet = [&]() { ptx::named_barrier_sync(1, W * 32); };
   // 32-bit positions (the launch keeps T there): a 64-bit division takes a hundred instructions
-  const unsigned unit = row / (unsigned)A.q_len, bt = (unsigned)A.bt;
-  const int b = (int)(unit / (unsigned)A.H);
-  const unsigned p = (unsigned)(T - A.q_len) + (row - unit * (unsigned)A.q_len);
-  const unsigned st = (unsigned)min(first_token(A.starts, b), (int64_t)INT32_MAX);
-  const int fb = (int)(st / bt), lb = (int)(p / bt);
-  const int nv = st > p ? 0 : lb - fb + 1;
-  int32_t *out = A.blocks + (int64_t)row * A.top;
-  float *out_s = A.block_scores ? A.block_scores + (int64_t)row * A.top : nullptr;
+  const unsigned bt = (unsigned)A.bt, p = (unsigned)(T - A.q_len) + (unsigned)i;
+  int fb = 0, lb = (int)(p / bt);  // the blocks this token may see
+  if (A.starts) {
+    const int b = (int)(unit / (unsigned)A.H);
+    const unsigned st = (unsigned)min(first_token(A.starts, b), (int64_t)INT32_MAX);
+    fb = (int)(st / bt);
+    if (st > p) lb = fb - 1;
+  }
+  const int nv = lb - fb + 1;
+  const int64_t row = (int64_t)unit * A.q_len + i;
+  int32_t *out = A.blocks + row * A.top;
+  float *out_s = A.block_scores ? A.block_scores + row * A.top : nullptr;
   const int tid = warp * 32 + lane, step = W * 32;
   for (int k = min(nv, A.top) + tid; k < A.top; k += step) {
     out[k] = -1;
     if (out_s) out_s[k] = -INFINITY;
   }
-  uint32_t key[KPT];  // 0: no block (visible ones are above it)
+  uint32_t key[KPT];  // of blocks j0 .. j0 + KPT - 1; 0: no block (visible ones are above it)
   uint32_t all_or = 0, all_and = 0xffffffffu;
+  float s1 = 0.f, s2 = 0.f;  // sums of the scores that compete and of their squares
+  const int j0 = tid * KPT;
+  {
+    float4 v[KPT / 4];
 #pragma unroll
-  for (int k = 0; k < KPT; ++k) {
-    const int x = k * step + tid;
-    key[k] = x >= nv ? 0u : (x < A.first || x >= nv - A.recent) ? 0xffffffffu : order_key(score[fb + x]);
-    if (key[k] != 0u && key[k] != 0xffffffffu) {
-      all_or |= key[k];
-      all_and &= key[k];
+    for (int k = 0; k < KPT / 4; ++k)
+      v[k] = j0 + 4 * k < (int)A.ns ? ((const float4 *)score)[(j0 >> 2) + k] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const unsigned rivals = (unsigned)max(nv - A.first - A.recent, 0);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+      const float x = (&v[k / 4].x)[k % 4];
+      const int at = j0 + k - fb;
+      key[k] = (unsigned)at < (unsigned)nv ? 0xffffffffu : 0u;
+      if ((unsigned)(at - A.first) < rivals) {
+        key[k] = order_key(x);
+        all_or |= key[k];
+        all_and &= key[k];
+        s1 += x;
+        s2 = fmaf(x, x, s2);
+      }
     }
   }
-  uint32_t thr = 1;  // keys at or above it are taken, those equal to it from the lowest index on
-  int reach = nv;    // keys that reach it
+  uint32_t thr = 1;   // keys at or above it are taken, those equal to it from the lowest index on
+  uint32_t from = 1;  // a bound below it, at which the gathered keys begin
+  int reach = nv;     // keys that reach thr, or from
   int bit = -1;
   if (nv > A.top) {
     // the bits above the highest differing one are those of every key that is not forced
     all_or = __reduce_or_sync(0xffffffffu, all_or);
     all_and = __reduce_and_sync(0xffffffffu, all_and);
+    int above = A.first + A.recent;  // keys above those in question (all of them visible: nv > top)
+    // the rank at which a guessed threshold aims: behind the last one taken, within what can be gathered
+    const float rank = 1.25f * (float)(A.top - above) + 8.f, rivals = (float)(nv - above);
+    const bool guess = nv > kShort && rank + (float)above <= 0.9f * kShort && rivals >= 2.f * rank;
+    if (guess) s1 = warp_sum(s1), s2 = warp_sum(s2);
     if (W > 1) {
-      if (lane == 0) s_pre[2 * warp] = (int)all_or, s_pre[2 * warp + 1] = (int)all_and;
+      if (lane == 0) {
+        s_pre[4 * warp] = (int)all_or, s_pre[4 * warp + 1] = (int)all_and;
+        s_pre[4 * warp + 2] = __float_as_int(s1), s_pre[4 * warp + 3] = __float_as_int(s2);
+      }
       meet();
-      all_or = __reduce_or_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane] : 0u);
-      all_and = __reduce_and_sync(0xffffffffu, lane < W ? (uint32_t)s_pre[2 * lane + 1] : 0xffffffffu);
+      const int4 of = lane < W ? ((const int4 *)s_pre)[lane] : make_int4(0, -1, 0, 0);
+      all_or = __reduce_or_sync(0xffffffffu, (uint32_t)of.x);
+      all_and = __reduce_and_sync(0xffffffffu, (uint32_t)of.y);
+      if (guess) s1 = warp_sum(__int_as_float(of.z)), s2 = warp_sum(__int_as_float(of.w));
       meet();  // s_pre is written again below
     }
     const uint32_t differ = all_or & ~all_and;  // first + recent <= top < nv: some key is not forced
     bit = differ ? 31 - __clz(differ) : -1;
     thr = bit < 0 ? all_and : all_and & ~((2u << bit) - 1u);
     const bool shorten = A.top <= kShort;
-    int above = A.first + A.recent;  // keys above those in question (all of them visible: nv > top)
     if (above == A.top) thr = 0xffffffffu, reach = A.top, bit = -1;  // the forced blocks fill the list
+    // The threshold guessed: where a normal distribution of these scores' mean and deviation has `rank` of them
+    // (quantile by Abramowitz and Stegun 26.2.22), moved by half a deviation while too few or too many reach it.
+    if (guess && bit >= 0) {
+      const float per = __fdividef(1.f, rivals), mean = s1 * per, var = fmaxf(s2 * per - mean * mean, 1e-30f);
+      const float sd = var * rsqrtf(var), w = 2.f * __logf(rivals * __fdividef(1.f, rank)), u = w * rsqrtf(w);
+      float z = u - __fdividef(2.30753f + 0.27061f * u, 1.f + u * (0.99229f + 0.04481f * u));
+      for (int tries = 0; tries < 4; ++tries) {
+        const uint32_t cand = max(order_key(fmaf(z, sd, mean)), 1u);
+        int c = 0;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) c += key[k] >= cand;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (W > 1) {
+          if (lane == 0) s_pre[(tries & 1) * 32 + warp] = c;
+          meet();
+          c = __reduce_add_sync(0xffffffffu, lane < W ? s_pre[(tries & 1) * 32 + lane] : 0);
+        }
+        if (c >= A.top && c <= kShort) {
+          from = cand;
+          reach = c;
+          break;
+        }
+        z += c < A.top ? -0.5f : 0.5f;
+      }
+      if (W > 1) meet();  // s_pre is written again below
+    }
     if (!HIST || W <= 4) {
       int par = 0;
       for (; bit >= 0 && reach != A.top && !(shorten && reach <= kShort); --bit) {
@@ -706,42 +739,66 @@ __device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigne
       bit = shift - 1;
     }
   }
-  if (reach <= kShort && reach > 0) {  // gather the keys that reach the threshold, in index order
-    int running = 0;
+  int all = 0;
+  auto before = [&](int mine) {  // sum of the threads' `mine` before this one; `all`: of all of them
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    all = __shfl_sync(0xffffffffu, upto, 31);
+    int base = 0;
     if (W > 1) {
-#pragma unroll
-      for (int k = 0; k < KPT; ++k) {
-        const unsigned in = __ballot_sync(0xffffffffu, key[k] >= max(thr, 1u));
-        if (lane == 0) s_pre[k * W + warp] = __popc(in);
-      }
+      if (lane == 0) s_pre[warp] = all;
       meet();
-      if (warp == 0) warp_prefix<KPT>(s_pre, KPT * W, lane);
-      meet();
+      const int x = lane < W ? s_pre[lane] : 0;
+      base = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+      all = __reduce_add_sync(0xffffffffu, x);
     }
+    return base + upto - mine;
+  };
+  if (reach <= kShort && reach > 0) {  // gather the keys that reach the threshold, in index order
+    from = max(from, thr);
+    int mine = 0;
 #pragma unroll
-    for (int k = 0; k < KPT; ++k) {
-      const bool in = key[k] >= max(thr, 1u);
-      const unsigned m = __ballot_sync(0xffffffffu, in);
-      const int at = (W > 1 ? s_pre[k * W + warp] : running) + __popc(m & ((1u << lane) - 1u));
-      running += __popc(m);
-      if (in) {
+    for (int k = 0; k < KPT; ++k) mine += key[k] >= from;
+    int at = before(mine);
+#pragma unroll
+    for (int k = 0; k < KPT; ++k)
+      if (key[k] >= from) {
         s_key[at] = key[k];
-        s_idx[at] = fb + k * step + tid;
+        s_idx[at++] = j0 + k;
       }
-    }
     meet();
     if (warp != 0) return;
     constexpr int N = kShort / 32;
     uint32_t kk[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) kk[k] = k * 32 + lane < reach ? s_key[k * 32 + lane] : 0u;
-    for (; bit >= 0 && reach > A.top; --bit) {
-      const uint32_t cand = thr | (1u << bit);
-      int c = 0;
+    if (reach > A.top) {  // from the highest bit on which these differ, two bits at a time: three counts in one sum
+      uint32_t o = 0, n = 0xffffffffu;
 #pragma unroll
-      for (int k = 0; k < N; ++k) c += kk[k] >= cand;
-      c = __reduce_add_sync(0xffffffffu, c);
-      if (c >= A.top) thr = cand, reach = c;
+      for (int k = 0; k < N; ++k)
+        if (kk[k] != 0u && kk[k] != 0xffffffffu) o |= kk[k], n &= kk[k];
+      o = __reduce_or_sync(0xffffffffu, o);
+      n = __reduce_and_sync(0xffffffffu, n);
+      bit = (o & ~n) ? 31 - __clz(o & ~n) : -1;
+      thr = bit < 0 ? n : n & ~((2u << bit) - 1u);
+      while (bit >= 0 && reach > A.top) {
+        const int sh = max(bit - 1, 0);
+        const uint32_t c1 = thr | (1u << sh), c2 = bit ? thr | (2u << sh) : c1, c3 = bit ? thr | (3u << sh) : c1;
+        unsigned c = 0;  // at most kShort each: a byte holds it
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          c += (kk[k] >= c1 ? 1u : 0u) + (kk[k] >= c2 ? 0x100u : 0u) + (kk[k] >= c3 ? 0x10000u : 0u);
+        c = __reduce_add_sync(0xffffffffu, c);
+        const int n1 = c & 255, n2 = (c >> 8) & 255, n3 = c >> 16;
+        if (n3 >= A.top) thr = c3, reach = n3;
+        else if (n2 >= A.top) thr = c2, reach = n2;
+        else if (n1 >= A.top) thr = c1, reach = n1;
+        bit = sh - 1;
+      }
     }
     // reach > top now means equal keys at the threshold: the lowest indexes of them
     int gt_all = 0;
@@ -765,56 +822,37 @@ __device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigne
     }
     return;
   }
-  // the rest from the registers: per key slot k and warp, keys above the threshold (low half) and equal to it (high)
-  int mine = 0, all_gt = 0;
+  // the rest from the registers: keys above the threshold (low half) and equal to it (high)
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < KPT; ++k) mine += key[k] > thr ? 1 : key[k] == thr ? 1 << 16 : 0;
+  const int first = before(mine);
+  const int need = A.top - (all & 0xffff);  // equal keys to take
+  int gt = first & 0xffff, eq = first >> 16;
 #pragma unroll
   for (int k = 0; k < KPT; ++k) {
-    const unsigned gt = __ballot_sync(0xffffffffu, key[k] > thr), eq = __ballot_sync(0xffffffffu, key[k] == thr);
-    const int packed = __popc(gt) | (__popc(eq) << 16);
-    if (W > 1) {
-      if (lane == 0) s_pre[k * W + warp] = packed;
-    } else if (lane == k) {
-      mine = packed;
-    }
-    all_gt += __popc(gt);
-  }
-  if (W > 1) {
-    meet();
-    if (warp == 0) {
-      const int all = warp_prefix<KPT>(s_pre, KPT * W, lane);
-      if (lane == 0) s_cnt[0] = all;
-    }
-    meet();
-    all_gt = s_cnt[0] & 0xffff;
-  }
-  const int need = A.top - all_gt;  // equal keys to take
-  int running = 0;
-#pragma unroll
-  for (int k = 0; k < KPT; ++k) {
-    const bool gt = key[k] > thr, eq = key[k] == thr;
-    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    const int base = W > 1 ? s_pre[k * W + warp] : running;
-    const unsigned below = (1u << lane) - 1u;
-    const int g0 = (base & 0xffff) + __popc(bg & below), e0 = (base >> 16) + __popc(be & below);
-    if (gt || (eq && e0 < need)) {
-      const int at = g0 + min(e0, need), j = fb + k * step + tid;
+    const bool above = key[k] > thr, tie = key[k] == thr;
+    if (above || (tie && eq < need)) {
+      const int at = gt + min(eq, need), j = j0 + k;
       out[at] = j;
       if (out_s) out_s[at] = score[j];
     }
-    if (W == 1) running += __shfl_sync(0xffffffffu, mine, k);
+    gt += above;
+    eq += tie;
   }
 }
 
 template <int KPT, int THREADS>
 __global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
-  __shared__ TopkShared<KPT, (THREADS > 128)> sh;
+  __shared__ TopkShared<(THREADS > 128)> sh;
   ptx::grid_dependency_wait();
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
   if (T == 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) set_length_error();
     return;
   }
-  topk_row<KPT, (THREADS > 128)>(A, T, blockIdx.x, A.score + (int64_t)blockIdx.x * A.ns, W, sh);
+  topk_row<KPT, (THREADS > 128)>(A, T, blockIdx.y, (int)blockIdx.x,
+                                 A.score + ((int64_t)blockIdx.y * A.q_len + blockIdx.x) * A.ns, W, sh);
 }
 
 // Scores and lists of one unit by one CTA, for a decode step's few query tokens
@@ -828,7 +866,7 @@ template <int KS, int GP>
 __global__ void __launch_bounds__(kOneWarps * 32) block_select_one_kernel(SelectArgs A) {
   constexpr int STR = 2 * KS * 32 + 64;
   extern __shared__ __align__(16) unsigned char s_a[];  // int8 [16][STR], fp32 [16], fp32 scores [q_len][ns]
-  __shared__ TopkShared<4, true> sh;
+  __shared__ TopkShared<true> sh;
   float *s_sg = (float *)(s_a + 16 * STR), *s_score = s_sg + 16;
   const unsigned unit = blockIdx.x;
   ptx::grid_dependency_wait();
@@ -849,7 +887,7 @@ __global__ void __launch_bounds__(kOneWarps * 32) block_select_one_kernel(Select
   if (warp >= W) return;
   for (int i = 0; i < A.q_len; ++i) {
     if (i) ptx::named_barrier_sync(1, W * 32);
-    topk_row<4, true>(A, T, unit * (unsigned)A.q_len + i, s_score + i * A.ns, W, sh);
+    topk_row<4, true>(A, T, unit, i, s_score + i * A.ns, W, sh);
   }
 }
 
@@ -1232,7 +1270,8 @@ static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t s
   int kpt = rows >= 4 * sm_count() && A.n > 128 ? 8 : 4;
   while (kpt < 16 && A.n > (int64_t)kpt * 32 * 32) kpt *= 2;
   const int64_t W = (A.n + kpt * 32 - 1) / (kpt * 32);
-  if (W > 32 || A.T >= (1LL << 31)) {
+  const int64_t units = (int64_t)A.B * A.H;
+  if (W > 32 || A.T >= (1LL << 31) || units > 65535) {
     block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
     return check_launch("cq_block_select");
   }
@@ -1240,7 +1279,7 @@ static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t s
                                 : kpt == 4 ? block_topk_regs_kernel<4, 1024>
                                 : kpt == 8 ? block_topk_regs_kernel<8, 1024>
                                            : block_topk_regs_kernel<16, 1024>;
-  return launch_after(fn, dim3((unsigned)rows), (int)W * 32, 0, st, "cq_block_select", A, (int)W);
+  return launch_after(fn, dim3((unsigned)A.q_len, (unsigned)units), (int)W * 32, 0, st, "cq_block_select", A, (int)W);
 }
 
 extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens,
