@@ -552,6 +552,11 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 
 // The `top` best visible blocks of a (unit, query token) row with every key in a
 // register: W warps, each thread with the keys of KPT blocks next to each other.
+// W is a trade of one row's time against the number of rows at once: of 4096 rows
+// of 512, 1024, 2048 and 4096 blocks, one warp a row takes 7.8 and 11.7 us (from
+// 2049 on keys leave the registers), up to four 11.5, 14.5, 19.4 and 31.7, up to
+// 32 with four or eight keys a thread 24 and 44 us for the last two; of 128 rows
+// of 1024 one warp a row takes 5.6, eight of four keys a thread 4.2 us.
 // First a threshold is guessed that some more than `top` keys reach, from the
 // scores' mean and deviation: one count settles it for scores that look normal,
 // where a search bit by bit takes a dozen (512 queries x 1024 blocks x 8 units, 32
@@ -569,24 +574,31 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 // this: 15 us).
 constexpr int kShort = 128;
 
-template <bool HIST>
+enum class Warps { ONE, FEW, MANY };  // a row's warps: one, up to four, up to 32
+
+template <Warps N>
 struct TopkShared {
   uint32_t key[kShort];
   int idx[kShort];
-  int hist[HIST ? 256 : 1];
+  int hist[N == Warps::MANY ? 256 : 1];
   int cnt[4];
-  __align__(16) int pre[128];  // four a warp
+  __align__(16) int pre[N == Warps::ONE ? 4 : 128];  // four a warp
 };
 
-// Query token i of a unit with its scores at `score` (16-byte aligned), by the
-// CTA's first W warps (named barrier 1); HIST: W may exceed four.
-template <int KPT, bool HIST>
-__device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigned unit, int i, const float *score, int W,
-                                         TopkShared<HIST> &sh) {
+// Query token i of a unit with its scores at `score` (16-byte aligned), by W
+// warps (named barrier 1), of which this is number `warp`.
+template <int KPT, Warps NW>
+__device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigned unit, int i, const float *score,
+                                         int n_warps, int warp, TopkShared<NW> &sh) {
+  constexpr bool HIST = NW == Warps::MANY;
+  const int W = NW == Warps::ONE ? 1 : n_warps;
   uint32_t *s_key = sh.key;
   int *s_idx = sh.idx, *s_hist = sh.hist, *s_cnt = sh.cnt, *s_pre = sh.pre;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto meet = [&]() { ptx::named_barrier_sync(1, W * 32); };
+  const int lane = threadIdx.x & 31;
+  auto meet = [&]() {
+    if (NW == Warps::ONE) __syncwarp();
+    else ptx::named_barrier_sync(1, W * 32);
+  };
   // 32-bit positions (the launch keeps T there): a 64-bit division takes a hundred instructions
   const unsigned bt = (unsigned)A.bt, p = (unsigned)(T - A.q_len) + (unsigned)i;
   int fb = 0, lb = (int)(p / bt);  // the blocks this token may see
@@ -799,6 +811,8 @@ __device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigne
         else if (n1 >= A.top) thr = c1, reach = n1;
         bit = sh - 1;
       }
+    } else {
+      thr = 1;  // all of them, and nothing of the lanes without a key (0)
     }
     // reach > top now means equal keys at the threshold: the lowest indexes of them
     int gt_all = 0;
@@ -842,17 +856,20 @@ __device__ __forceinline__ void topk_row(const SelectArgs &A, int64_t T, unsigne
   }
 }
 
-template <int KPT, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_topk_regs_kernel(SelectArgs A, int W) {
-  __shared__ TopkShared<(THREADS > 128)> sh;
+template <int KPT, Warps NW>
+__global__ void __launch_bounds__(NW == Warps::MANY ? 1024 : 128) block_topk_regs_kernel(SelectArgs A, int W) {
+  constexpr int ROWS = NW == Warps::ONE ? 4 : 1;  // rows per CTA
+  __shared__ TopkShared<NW> sh[ROWS];
   ptx::grid_dependency_wait();
   const int64_t T = launch_length(A.T, A.len_dev, A.q_len);
   if (T == 0) {
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) set_length_error();
     return;
   }
-  topk_row<KPT, (THREADS > 128)>(A, T, blockIdx.y, (int)blockIdx.x,
-                                 A.score + ((int64_t)blockIdx.y * A.q_len + blockIdx.x) * A.ns, W, sh);
+  const int warp = threadIdx.x >> 5, r = NW == Warps::ONE ? warp : 0, i = (int)blockIdx.x * ROWS + r;
+  if (i >= A.q_len) return;
+  topk_row<KPT, NW>(A, T, blockIdx.y, i, A.score + ((int64_t)blockIdx.y * A.q_len + i) * A.ns, W,
+                    NW == Warps::ONE ? 0 : warp, sh[r]);
 }
 
 // Scores and lists of one unit by one CTA, for a decode step's few query tokens
@@ -866,7 +883,7 @@ template <int KS, int GP>
 __global__ void __launch_bounds__(kOneWarps * 32) block_select_one_kernel(SelectArgs A) {
   constexpr int STR = 2 * KS * 32 + 64;
   extern __shared__ __align__(16) unsigned char s_a[];  // int8 [16][STR], fp32 [16], fp32 scores [q_len][ns]
-  __shared__ TopkShared<true> sh;
+  __shared__ TopkShared<Warps::MANY> sh;
   float *s_sg = (float *)(s_a + 16 * STR), *s_score = s_sg + 16;
   const unsigned unit = blockIdx.x;
   ptx::grid_dependency_wait();
@@ -887,7 +904,7 @@ __global__ void __launch_bounds__(kOneWarps * 32) block_select_one_kernel(Select
   if (warp >= W) return;
   for (int i = 0; i < A.q_len; ++i) {
     if (i) ptx::named_barrier_sync(1, W * 32);
-    topk_row<4, true>(A, T, unit, i, s_score + i * A.ns, W, sh);
+    topk_row<4, Warps::MANY>(A, T, unit, i, s_score + i * A.ns, W, warp, sh);
   }
 }
 
@@ -1266,20 +1283,31 @@ static int launch_scores(const sparse::SelectArgs &A, const SelectForm &f, cudaS
 
 static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t st) {
   using namespace sparse;
-  // A CTA per row, four keys a thread; where rows abound eight (up to four warps), whose rounds cost fewer meetings
-  int kpt = rows >= 4 * sm_count() && A.n > 128 ? 8 : 4;
-  while (kpt < 16 && A.n > (int64_t)kpt * 32 * 32) kpt *= 2;
-  const int64_t W = (A.n + kpt * 32 - 1) / (kpt * 32);
   const int64_t units = (int64_t)A.B * A.H;
-  if (W > 32 || A.T >= (1LL << 31) || units > 65535) {
+  if (A.n > 16 * 1024 || A.T >= (1LL << 31) || units > 65535) {
     block_topk_kernel<<<(unsigned)rows, 256, 0, st>>>(A);
     return check_launch("cq_block_select");
   }
-  void (*fn)(SelectArgs, int) = W <= 4 ? (kpt == 4 ? block_topk_regs_kernel<4, 128> : block_topk_regs_kernel<8, 128>)
-                                : kpt == 4 ? block_topk_regs_kernel<4, 1024>
-                                : kpt == 8 ? block_topk_regs_kernel<8, 1024>
-                                           : block_topk_regs_kernel<16, 1024>;
-  return launch_after(fn, dim3((unsigned)A.q_len, (unsigned)units), (int)W * 32, 0, st, "cq_block_select", A, (int)W);
+  // a warp a row from 12 rows per SM on (1024 blocks: 1184 rows 6.7 us against 6.2 with four warps, 2400 rows 9.3
+  // against 10.0; up to 256 blocks the same either way)
+  if (A.n > 256 && A.n <= 1024 && rows >= 12 * sm_count()) {
+    auto *fn = A.n <= 512 ? block_topk_regs_kernel<16, Warps::ONE> : block_topk_regs_kernel<32, Warps::ONE>;
+    return launch_after(fn, dim3((unsigned)(A.q_len + 3) / 4, (unsigned)units), 128, 0, st, "cq_block_select", A, 1);
+  }
+  // keys a thread: four, or where rows abound so many that up to four warps hold a row (320 rows of 2048 blocks 5.2
+  // us against 6.2, 4096 rows 19.4 against 24)
+  int kpt = 4;
+  if (A.n > 128 && A.n <= 4096 && rows >= 2 * sm_count()) kpt = A.n <= 1024 ? 8 : A.n <= 2048 ? 16 : 32;
+  while (A.n > (int64_t)kpt * 32 * 32) kpt *= 2;  // up to 16
+  const int W = (int)((A.n + kpt * 32 - 1) / (kpt * 32));
+  using Fn = void (*)(SelectArgs, int);
+  static const Fn few[4] = {block_topk_regs_kernel<4, Warps::FEW>, block_topk_regs_kernel<8, Warps::FEW>,
+                            block_topk_regs_kernel<16, Warps::FEW>, block_topk_regs_kernel<32, Warps::FEW>};
+  static const Fn many[3] = {block_topk_regs_kernel<4, Warps::MANY>, block_topk_regs_kernel<8, Warps::MANY>,
+                             block_topk_regs_kernel<16, Warps::MANY>};
+  const int size = kpt == 4 ? 0 : kpt == 8 ? 1 : kpt == 16 ? 2 : 3;
+  return launch_after(W <= 4 ? few[size] : many[size], dim3((unsigned)A.q_len, (unsigned)units), W * 32, 0, st,
+                      "cq_block_select", A, W);
 }
 
 extern "C" int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens,

@@ -300,6 +300,56 @@ def test_select_many_equal_scores(blocks):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["normal", "skewed", "two values", "outliers"])
+@pytest.mark.parametrize("S,blocks", [(450, 200), (450, 300), (450, 1000), (100, 1000), (75, 1500), (75, 4000),
+                                      (9, 4000), (1, 700)])
+def test_select_of_many_rows(S, blocks, kind):
+    """Every form of the search (a warp, up to four or more warps a row) on
+    scores that do and do not look normal, padded and not, for short, middle and
+    long lists.  The reference sorts the whole row, equal scores by index."""
+    B, H, G, D, bt, first, recent = 2, 4, 2, 64, 16, 1, 2
+    T = blocks * bt - 5
+    g = torch.Generator(device="cuda").manual_seed(S * blocks)
+    k = torch.randn((B, H, blocks, 1, D), generator=g, device="cuda").expand(-1, -1, -1, bt, -1).clone()
+    u = torch.rand((B, H, blocks, 1, 1), generator=g, device="cuda")
+    if kind == "skewed":
+        k *= torch.exp2(-12 * u ** 0.25)
+    elif kind == "two values":
+        k = torch.ones_like(k) * (1 + (u > 0.6))
+    elif kind == "outliers":
+        k = torch.where(u > 0.99, 300 * k, k)
+    k = k.reshape(B, H, blocks * bt, D)[:, :, :T].half()
+    cache = ChronoQuantCache()
+    cache.update_and_fetch(k, k)
+    index = BlockIndex(cache, bt).update()
+    q = queries(B, H * G, S, D, torch.bfloat16, seed=blocks)
+    codes, scales = index.codes[:, :, :blocks].double(), index.scales[:, :, :blocks]
+    x = q.float()
+    amax = x.abs().amax(-1, keepdim=True)
+    q8 = torch.round(x * (torch.full_like(amax, 127.0) / amax)).double().view(B, H, G, S, D)
+    sg = (amax / torch.full_like(amax, 127.0)).view(B, H, G, S, 1)
+    dot = (torch.einsum("bhgsd,bhnd->bhgsn", q8.clamp(min=0), codes[:, :, :, 1])
+           + torch.einsum("bhgsd,bhnd->bhgsn", q8.clamp(max=0), codes[:, :, :, 0])).float()
+    score = ((sg * scales[:, :, None, None]) * dot).amax(2)  # [B, H, S, n]
+    j = torch.arange(blocks, device="cuda")
+    p = (T - S + torch.arange(S, device="cuda")).view(1, 1, S, 1)
+    for starts in (None, torch.tensor([37, T // 3], device="cuda")):
+        st = torch.zeros((B, 1, 1, 1), dtype=torch.int64, device="cuda") if starts is None else starts.view(B, 1, 1, 1)
+        fb, lb = st // bt, p // bt
+        seen = (j >= fb) & (j <= lb)
+        forced = seen & ((j < fb + first) | (j > lb - recent))
+        rank = torch.where(forced, math.inf, torch.where(seen, score, -math.inf))
+        order = torch.sort(rank, dim=-1, descending=True, stable=True).indices
+        for top in (4, 40, 100, min(blocks, 900)):
+            want = torch.where(seen.expand_as(rank).gather(-1, order[..., :top]), order[..., :top], blocks)
+            want = want.sort(-1).values
+            want_s = torch.where(want < blocks, score.gather(-1, want.clamp(max=blocks - 1)), -math.inf)
+            got, s = index.select(q, top, first=first, recent=recent, starts=starts, return_scores=True)
+            assert torch.equal(got, torch.where(want < blocks, want, -1).int()), top
+            assert torch.equal(s, want_s), top
+
+
+@gpu
 @pytest.mark.parametrize("D", [8, 32, 64, 72, 96, 256])
 def test_select_head_dims(D):
     cache = make_cache(2, 2, 600, D, seed=D)
