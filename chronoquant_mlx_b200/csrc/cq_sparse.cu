@@ -336,29 +336,47 @@ __device__ __forceinline__ void mma_s8_16832(int (&c)[4], uint32_t a0, uint32_t 
 // maximum over a group's heads goes by halves: each exchange also halves the
 // values a lane holds, so every lane ends with its own ones to store.  Bound by
 // latency and issue, not by the tensor pipe: a row tile against 16 blocks is
-// about 220 instructions, 16 of them products, and 14 warps an SM issue in 46 %
-// of the slots.  2048 rows x 1024 blocks x 256 codes x 8 units take 30 us; with
-// the codes as fp16, whose fragments cost conversions, 47 us.  One launch that
-// also lists, with the scores in shared memory, takes 64 us there against 54 us
-// for this kernel and the next: too few warps fit beside the scores.
+// about 200 instructions, 16 of them products, and 14 warps an SM issue in less
+// than half of the slots.  2048 rows x 1024 blocks x 256 codes x 8 units take 27
+// us (7.5 us of products); two row tiles at once 29, half the row tiles a CTA 34,
+// and with the codes as fp16, whose fragments cost conversions, 47 us.  One launch
+// that also lists, with the scores in shared memory, took 10 us more there than
+// this kernel and the next: too few warps fit beside the scores.
 constexpr int kScoreWarps = 8, kScoreCols = 16;  // blocks per warp and pass
 
-// Query rows [0, rows) of a unit from token i0 on into shared memory, by WARPS warps.
+// Query rows [0, rows) of a unit from token i0 on into shared memory, by WARPS
+// warps.  A lane holds KS channels next to each other: one load where the rows are
+// aligned for it, one store each for the two halves of a code row.  The rows
+// behind the group's heads get the scale NaN.
 template <int KS, int GP, int WARPS>
 __device__ __forceinline__ void quantise_rows(const SelectArgs &A, unsigned unit, int i0, int rows, unsigned char *s_a,
                                               float *s_sg) {
   constexpr int D = KS * 32, STR = 2 * D + 64, UN = WARPS > 8 ? 1 : 4;  // rows whose loads are in flight
+  constexpr bool VEC = KS != 3;
+  using Raw = typename std::conditional<KS == 8, uint4, typename std::conditional<KS == 4, uint2, uint32_t>::type>::type;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = (int)(unit / (unsigned)A.H), h = (int)(unit - (unsigned)b * (unsigned)A.H);
+  const bool wide = VEC && ((((uintptr_t)A.q) & (2 * KS - 1)) | ((uint64_t)(A.q_sb | A.q_sh | A.q_sq) & (KS - 1))) == 0;
   for (int r0 = warp; r0 < rows; r0 += UN * WARPS) {
     float x[UN][KS];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int r = r0 + u * WARPS, i = i0 + r / GP, hd = r & (GP - 1);
       const bool real = r < rows && i < A.q_len && hd < A.G;
-      const int64_t qb = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq;
+      const int64_t at = b * A.q_sb + (int64_t)(h * A.G + hd) * A.q_sh + (int64_t)i * A.q_sq + lane * KS;
+      if (VEC && wide) {
+        Raw w = {};
+        if (real) w = *(const Raw *)((const uint16_t *)A.q + at);
+        const uint32_t *p = (const uint32_t *)&w;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) x[u][k] = real ? load_as_float(A.q, qb + lane * KS + k, A.q_dtype) : 0.f;
+        for (int k = 0; k < KS; ++k) {
+          const uint16_t e = (uint16_t)(p[k / 2] >> (k & 1 ? 16 : 0));
+          x[u][k] = A.q_dtype == CQ_BF16 ? __uint_as_float((uint32_t)e << 16) : __half2float(__ushort_as_half(e));
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) x[u][k] = real ? load_as_float(A.q, at + k, A.q_dtype) : 0.f;
+      }
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
@@ -372,13 +390,24 @@ __device__ __forceinline__ void quantise_rows(const SelectArgs &A, unsigned unit
       }
       const QueryScale qs(warp_max(amax));
       int8_t *row = (int8_t *)s_a + r * STR + lane * KS;
+      uint32_t lo[(KS + 3) / 4] = {}, hi[(KS + 3) / 4] = {};
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int c = qs.code(x[u][k]);
-        row[k] = (int8_t)min(c, 0);
-        row[D + k] = (int8_t)max(c, 0);
+        lo[k / 4] |= ((uint32_t)min(c, 0) & 255u) << (8 * (k & 3));
+        hi[k / 4] |= (uint32_t)max(c, 0) << (8 * (k & 3));
       }
-      if (lane == 0) s_sg[r] = qs.s;
+      if constexpr (KS == 2) {
+        *(uint16_t *)row = (uint16_t)lo[0];
+        *(uint16_t *)(row + D) = (uint16_t)hi[0];
+      } else if constexpr (KS == 3) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) row[k] = (int8_t)(lo[0] >> (8 * k)), row[D + k] = (int8_t)(hi[0] >> (8 * k));
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS / 4; ++k) ((uint32_t *)row)[k] = lo[k], ((uint32_t *)(row + D))[k] = hi[k];
+      }
+      if (lane == 0) s_sg[r] = (r & (GP - 1)) < A.G ? qs.s : __int_as_float(0x7fffffff);
     }
   }
 }
@@ -410,7 +439,6 @@ __device__ __forceinline__ void score_tile(const SelectArgs &A, const BlockCodes
                                            const float *sg_tile, int i, int j0, float *dst) {
   constexpr int STR = 2 * KS * 32 + 64;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const bool pad0 = (g & (GP - 1)) >= A.G, pad1 = ((g + 8) & (GP - 1)) >= A.G;
   int acc[2][4] = {};
   const unsigned char *a = a_tile + g * STR + 16 * t;
 #pragma unroll
@@ -431,8 +459,8 @@ __device__ __forceinline__ void score_tile(const SelectArgs &A, const BlockCodes
     for (int e = 0; e < 2; ++e) {
       const float x = __fmul_rn(__fmul_rn(sg0, f.sj[nb][e]), (float)acc[nb][e]);
       const float y = __fmul_rn(__fmul_rn(sg1, f.sj[nb][e]), (float)acc[nb][2 + e]);
-      v[nb][0][e] = pad0 ? -INFINITY : __fadd_rn(x, 0.f);  // -0 becomes +0: equal scores have equal keys
-      v[nb][1][e] = pad1 ? -INFINITY : __fadd_rn(y, 0.f);
+      v[nb][0][e] = x;  // NaN in the rows behind the group, which the maximum leaves out
+      v[nb][1][e] = y;
     }
   auto swap_max = [&](float &keep, float give, int o) { keep = fmaxf(keep, __shfl_xor_sync(0xffffffffu, give, o)); };
   int nb0 = 0, hf0 = 0;  // which of the values this lane holds
@@ -479,7 +507,8 @@ __device__ __forceinline__ void score_tile(const SelectArgs &A, const BlockCodes
       bool mine = i + tok < A.q_len && j0 + col < (int)A.ns;
       if (GP >= 8) mine = mine && !(g & 4);
       if (GP == 16) mine = mine && !(g & 2);
-      if (mine) *(float2 *)(dst + tok * A.ns + col) = make_float2(v[nb][hf][0], v[nb][hf][1]);
+      if (mine)  // -0 becomes +0: equal scores have equal keys
+        *(float2 *)(dst + tok * A.ns + col) = make_float2(__fadd_rn(v[nb][hf][0], 0.f), __fadd_rn(v[nb][hf][1], 0.f));
     }
 }
 
@@ -553,9 +582,9 @@ __global__ void __launch_bounds__(256) block_score_kernel(SelectArgs A) {
 // The `top` best visible blocks of a (unit, query token) row with every key in a
 // register: W warps, each thread with the keys of KPT blocks next to each other.
 // W is a trade of one row's time against the number of rows at once: of 4096 rows
-// of 512, 1024, 2048 and 4096 blocks, one warp a row takes 7.8 and 11.7 us (from
-// 2049 on keys leave the registers), up to four 11.5, 14.5, 19.4 and 31.7, up to
-// 32 with four or eight keys a thread 24 and 44 us for the last two; of 128 rows
+// of 512, 1024, 2048 and 4096 blocks, one warp a row takes 7.8, 11.7 and 19.4 us,
+// up to four 11.5, 14.5, 19.4 and 31.7, up to 32 with eight keys a thread 24 and
+// 44 us for the last two; of 128 rows
 // of 1024 one warp a row takes 5.6, eight of four keys a thread 4.2 us.
 // First a threshold is guessed that some more than `top` keys reach, from the
 // scores' mean and deviation: one count settles it for scores that look normal,
@@ -875,8 +904,8 @@ __global__ void __launch_bounds__(NW == Warps::MANY ? 1024 : 128) block_topk_reg
 // Scores and lists of one unit by one CTA, for a decode step's few query tokens
 // (one row tile) and up to kOneBlocks blocks: the scores stay in shared memory,
 // one launch and no workspace.  Bound by latency (a launch, the codes' loads, the
-// search's meetings): one sequence of 8192 tokens 5.9 us, 8.5 us as two kernels;
-// 16 of 32768 tokens 7.7 us, 10.4 us as two kernels.
+// search's meetings): one sequence of 8192 tokens 4.8 us, 16 of 32768 tokens 7.4
+// us; as two kernels 2.6 us more each.
 constexpr int kOneWarps = 16, kOneBlocks = 2048;
 
 template <int KS, int GP>
