@@ -191,8 +191,9 @@ __device__ __forceinline__ void load_q_tile(const QuerySrc &p, int lane, QFrag &
     f.qb[J][1] = __byte_perm(w.x, w.z, 0x7632u);
     f.qb[J][2] = __byte_perm(w.y, w.w, 0x5410u);
     f.qb[J][3] = __byte_perm(w.y, w.w, 0x7632u);
-    ptx::mma_f16_16816(cc, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, f.qb[J][0], f.qb[J][1]);
-    ptx::mma_f16_16816(cc, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, f.qb[J][2], f.qb[J][3]);
+    constexpr uint32_t EIGHT = 0x00080008u;  // 8 * 2^-24, as the codes come
+    ptx::mma_f16_16816(cc, EIGHT, EIGHT, EIGHT, EIGHT, f.qb[J][0], f.qb[J][1]);
+    ptx::mma_f16_16816(cc, EIGHT, EIGHT, EIGHT, EIGHT, f.qb[J][2], f.qb[J][3]);
   }
   f.qc = make_float2(cc[0], cc[1]);
 }
@@ -278,9 +279,12 @@ __device__ __forceinline__ float lds_half_as_float(uint32_t a) {
 // MASK: 0 every token of the chunk counts, 1 tokens below nvalid, 2 tokens
 // from vlo on and below nvalid (one of this group's at least).
 // RAW: K codes enter the score MMAs as 1024 + n and 1024 + 16n (load_q's
-// fragments: fewest operations; the sums reach 1032 sum|q|, whose fp32 rounding
-// shows in the scores); otherwise as 64 + n = code + 72 (load_q_tile's: two
-// shifts more per word, sums of at most 79 sum|q|, a 13 times smaller error).
+// fragments; the sums reach 1032 sum|q|, whose fp32 rounding shows in the scores);
+// otherwise as the nibbles alone (load_q_tile's fragments): the bits of n and 16n
+// in a half are the subnormal numbers n * 2^-24 and 16n * 2^-24, exact operands
+// without an offset, summed apart and weighted by 2^24 and 2^20 with the scale
+// (sums of at most 15 sum|q|; as 64 + n, with sums of 79 sum|q|, 4096 units of 32
+// chunks took 221 us, so 217).
 template <class G, int MASK, bool RAW = true>
 __device__ __forceinline__ bool k_group(WarpState &st, const KAddr &A, const QFrag &f, int t0, int nvalid, int lane,
                                         uint2 (&bp)[2], __half2 &fh, int vlo = 0) {
@@ -295,8 +299,9 @@ __device__ __forceinline__ bool k_group(WarpState &st, const KAddr &A, const QFr
     const uint32_t rk = (uint32_t)((tb - (tb >> lsk)) * 64);  // K rows before the tile
     const uint4 wk0 = ptx::lds_u128(A.cdK + rk);
     const uint4 wk1 = ptx::lds_u128(A.cdK + rk + 8 * 64);
-    const float sk0 = lds_half_as_float(A.scK + tb * 2) * LOG2E;
-    const float sk1 = lds_half_as_float(A.scK + (tb + 8) * 2) * LOG2E;
+    constexpr float UNIT = RAW ? LOG2E : LOG2E * 16777216.f;
+    const float sk0 = lds_half_as_float(A.scK + tb * 2) * UNIT;
+    const float sk1 = lds_half_as_float(A.scK + (tb + 8) * 2) * UNIT;
     const float2 qa = ptx::lds_f2(A.qa + (uint32_t)((tb >> lsk) * 32));  // one K anchor per tile (stride >= 16)
     // raw nibbles (1024+n, 1024+16n) against q (q/16 on the 16n lanes); the
     // accumulator starts at -q.(all-8 word), which removes the raw offset
@@ -305,21 +310,24 @@ __device__ __forceinline__ bool k_group(WarpState &st, const KAddr &A, const QFr
     const uint32_t w1[4] = {wk1.x, wk1.y, wk1.z, wk1.w};
 #pragma unroll
     for (int J = 0; J < 4; ++J) {
-      uint32_t h0[4], h1[4];
       if constexpr (RAW) {
+        uint32_t h0[4], h1[4];
         ptx::nibbles_to_half2_raw(w0[J], h0);  // (d0,d4) (d1,d5) (d2,d6) (d3,d7)
         ptx::nibbles_to_half2_raw(w1[J], h1);
+        ptx::mma_f16_16816(ca, h0[0], h1[0], h0[1], h1[1], f.qb[J][0], f.qb[J][1]);
+        ptx::mma_f16_16816(cb, h0[2], h1[2], h0[3], h1[3], f.qb[J][2], f.qb[J][3]);
       } else {
-        ptx::nibbles_to_half2_64(w0[J], h0);
-        ptx::nibbles_to_half2_64(w1[J], h1);
+        constexpr uint32_t EVEN = 0x000f000fu, ODD = 0x00f000f0u;
+        const uint32_t v0 = w0[J] >> 8, v1 = w1[J] >> 8;
+        ptx::mma_f16_16816(ca, w0[J] & EVEN, w1[J] & EVEN, v0 & EVEN, v1 & EVEN, f.qb[J][0], f.qb[J][2]);
+        ptx::mma_f16_16816(cb, w0[J] & ODD, w1[J] & ODD, v0 & ODD, v1 & ODD, f.qb[J][1], f.qb[J][3]);
       }
-      ptx::mma_f16_16816(ca, h0[0], h1[0], h0[1], h1[1], f.qb[J][0], f.qb[J][1]);
-      ptx::mma_f16_16816(cb, h0[2], h1[2], h0[3], h1[3], f.qb[J][2], f.qb[J][3]);
     }
-    s[tile][0] = fmaf(sk0, ca[0] + cb[0], qa.x);
-    s[tile][1] = fmaf(sk0, ca[1] + cb[1], qa.y);
-    s[tile][2] = fmaf(sk1, ca[2] + cb[2], qa.x);
-    s[tile][3] = fmaf(sk1, ca[3] + cb[3], qa.y);
+    constexpr float W = RAW ? 1.f : 0.0625f;  // of cb
+    s[tile][0] = fmaf(sk0, fmaf(cb[0], W, ca[0]), qa.x);
+    s[tile][1] = fmaf(sk0, fmaf(cb[1], W, ca[1]), qa.y);
+    s[tile][2] = fmaf(sk1, fmaf(cb[2], W, ca[2]), qa.x);
+    s[tile][3] = fmaf(sk1, fmaf(cb[3], W, ca[3]), qa.y);
     if (MASK) {
       // tokens past the end: score -inf (their buffer bytes are stale)
       if (tb + g >= nvalid) s[tile][0] = s[tile][1] = -INFINITY;

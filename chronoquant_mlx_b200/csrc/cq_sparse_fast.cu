@@ -12,10 +12,10 @@
 // cluster through distributed shared memory: one launch, no workspace, and the
 // order of every sum is fixed.
 //
-// Bound by latency where units are few (one query over 32 blocks of 64: 7.9 us)
-// and by instructions where they are many: 4096 units of 32 chunks take 221 us,
-// 1016 instructions a chunk of which half run on the half-rate integer pipe, at
-// 57 % issue with the 16 warps an SM that registers and buffers leave room for.
+// Bound by latency where units are few (one query over 32 blocks of 64: 7.8 us)
+// and by instructions where they are many: 4096 units of 32 chunks take 217 us,
+// 1025 instructions a chunk of which half run on the half-rate integer pipe, at
+// 58 % issue with the 16 warps an SM that registers and buffers leave room for.
 // Several query tokens per unit, sharing the chunks that more than one of them
 // lists, took 255 to 301 us (neighbouring lists overlap by a third).
 //
