@@ -35,4 +35,3 @@ def stream_ptr(device: torch.device | None = None) -> int:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
-

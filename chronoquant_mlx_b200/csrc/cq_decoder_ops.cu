@@ -186,7 +186,7 @@ __device__ __forceinline__ void store_quad(void *p, int64_t i, const float4 v) {
 // products of norm weight and sine or cosine in registers: a pair (x, y) of a
 // head with root r becomes r (x wc - y ws'), r (y wc' + x ws).  Neighbouring
 // groups hold neighbouring tokens, whose output rows are contiguous.  Bound by
-// HBM: 2 x 8191 tokens of 32 + 8 + 8 bf16 heads of 128 (336 MB) take 61.5 us, 84 %
+// HBM: 2 x 8191 tokens of 32 + 8 + 8 bf16 heads of 128 (336 MB) take 60.9 us, 85 %
 // of the measured copy rate; with two or eight heads in flight 66 and 67 us.
 struct PairTurn {  // coefficients of one pair: out0 = x * xc - y * ys, out1 = y * yc + x * xs
   float xc, ys, yc, xs;

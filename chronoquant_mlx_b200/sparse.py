@@ -15,10 +15,13 @@ addition around the same cache.  Three steps, each on the caller's stream::
 channels in 8 bits (2 * head_dim + 4 bytes a block); ``select`` scores every
 block by the largest q.k its ranges allow and lists the best ones per query
 token; the attention kernel reads the listed blocks of the paged cache
-directly.  Lists hold at most 4096 blocks.  Queries are the newest tokens of the cache: query i of q_len sits at
-position offset - q_len + i and sees nothing behind it.  ``starts`` gives the
-first real token of each sequence of a left-padded batch; a row that sees no
-token gets zeros.
+directly.  Lists hold at most 4096 blocks.  Queries are the newest tokens of the
+cache: query i of q_len sits at position offset - q_len + i and sees nothing
+behind it.  ``starts`` gives the first real token of each sequence of a
+left-padded batch; a row that sees no token gets zeros.  The lengths are the
+host's: a call captured into a CUDA graph replays at the length it was captured
+at (``decoder.Qwen3StyleDecoder(sparse=...)`` captures steps that read the length
+from device memory).
 """
 
 from __future__ import annotations
@@ -102,6 +105,8 @@ class BlockIndex:
         n = self.n_blocks - int(first)
         if first < 0 or n < 0 or self.codes is None:
             raise ValueError(f"BlockIndex: first block {first} outside [0, {self.n_blocks}] (or nothing summarised)")
+        if self._store is not self.cache.store:
+            raise ValueError("BlockIndex: the cache's state was replaced since the last update()")
         return _lib.calls().block_bounds_read(self.codes, self.scales, int(first), n)
 
     @traced("cq.block_select")

@@ -216,6 +216,21 @@ def test_bounds_follow_the_cache():
 
 
 @gpu
+def test_index_of_a_replaced_state():
+    """A cache restored to another state of the same length: ranges of the old
+    one are not handed out, and a selection summarises anew."""
+    a, b = make_cache(1, 2, 300, 128, seed=1), make_cache(1, 2, 300, 128, seed=2)
+    index, q = BlockIndex(a, 32).update(), queries(1, 4, 1, 128, torch.float16)
+    index.bounds()
+    a.state = b.state
+    with pytest.raises(ValueError, match="replaced"):
+        index.bounds()
+    other = BlockIndex(b, 32)
+    assert torch.equal(index.select(q, 5), other.select(q, 5))
+    assert torch.equal(index.bounds(), other.bounds())
+
+
+@gpu
 def test_bounds_with_infinite_and_nan_keys():
     """A block with an infinite or NaN anchor keeps finite ranges; the others are untouched."""
     clean, dirty = make_cache(1, 1, 256, 128, seed=4, stride_k=16), make_cache(1, 1, 256, 128, seed=4, stride_k=16)
@@ -557,23 +572,48 @@ def test_infinite_values_stay_with_the_queries_that_see_them(kw, G):
         assert torch.isfinite(out[:, :, :2]).all() and not torch.isfinite(out[0, :, 2, 3]).any()
 
 
+def score_slack(cache, q, scale):
+    """How far scores may be off, beside the roundings that check_attention
+    counts.  q.code is accumulated over nibbles n <= 15 from -8 sum q on, so
+    partial sums stay below 24 * sum|q|; each of at most 16 accumulation steps
+    errs by 2^-23 of them, and the token's scale multiplies the result.  The
+    anchor's product errs by 16 * 2^-23 * sum|q| * max|anchor|."""
+    st = cache.state
+    qsum = (q * torch.tensor(scale, dtype=q.dtype, device="cuda")).double().abs().sum(-1).max()
+    return 16 * 2.0 ** -23 * qsum * (24 * st[3].double().max() + st[0].double().abs().max())
+
+
 @gpu
 def test_sparse_attention_extreme_scores():
-    """Scores of some thousands: no overflow, and few keys decide.
-
-    The scores' error grows with the query: q.code is accumulated with the codes
-    as 64 + n <= 79, so partial sums stay below 79 * sum|q|, each of at most 16
-    accumulation steps errs by 2^-23 of them, and the token's scale multiplies
-    the result; the anchor's product errs by 16 * 2^-23 * sum|q| * max|anchor|."""
+    """Scores of some thousands: no overflow, and few keys decide."""
     cache = make_cache(1, 1, 400, 128, seed=2)
     q = queries(1, 4, 1, 128, torch.float16, amp=300.0)
     blocks = torch.tensor([0, 2, 4, 6], dtype=torch.int32, device="cuda").view(1, 1, 1, 4)
     K, V = decoded(cache)
     ref, rlse, vmax = ref_sparse(K, V, q, 0.25, blocks, 64)
     out, lse = chronoquant_sparse_sdpa(q, cache, 0.25, blocks, 64, return_lse=True)
-    st = cache.state
-    qsum = (q * torch.tensor(0.25, dtype=q.dtype, device="cuda")).double().abs().sum(-1).max()
-    slack = 16 * 2.0 ** -23 * qsum * (79 * st[3].double().max() + st[0].double().abs().max())
+    slack = score_slack(cache, q, 0.25)
+    assert (lse.double() - rlse).abs().max() <= 2.0 ** -10 + slack
+    assert ((out.double() - ref).abs() <= (5 * 2.0 ** -11 + 2 * slack) * vmax).all()
+
+
+@gpu
+@pytest.mark.parametrize("kw", [LAYOUTS[0], LAYOUTS[1]])
+def test_sparse_attention_tiny_queries_of_large_keys(kw):
+    """Query values that are subnormal in fp16 against keys of thousands: the
+    scores are sums of products of subnormal numbers."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    k = (3000 * torch.randn((1, 1, 400, 128), generator=g, device="cuda")).half()
+    v = torch.randn((1, 1, 400, 128), generator=g, device="cuda").half()
+    cache = ChronoQuantCache(**kw)
+    cache.update_and_fetch(k, v)
+    q = queries(1, 4, 2, 128, torch.float16, amp=2.0 ** -13)
+    blocks = torch.tensor([0, 1, 4, 6], dtype=torch.int32, device="cuda").expand(1, 1, 2, 4)
+    K, V = decoded(cache)
+    ref, rlse, vmax = ref_sparse(K, V, q, 0.25, blocks, 64)
+    assert rlse.max() > math.log(3 * 64 + 16) + 0.2  # 208 tokens, and their scores count
+    out, lse = chronoquant_sparse_sdpa(q, cache, 0.25, blocks, 64, return_lse=True)
+    slack = score_slack(cache, q, 0.25)
     assert (lse.double() - rlse).abs().max() <= 2.0 ** -10 + slack
     assert ((out.double() - ref).abs() <= (5 * 2.0 ** -11 + 2 * slack) * vmax).all()
 
