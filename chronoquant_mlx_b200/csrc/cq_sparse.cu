@@ -1290,11 +1290,11 @@ static int launch_scores(const sparse::SelectArgs &A, const SelectForm &f, cudaS
   if (f.mma) {
     using Fn = void (*)(SelectArgs, int, int);
     static const Fn table[4][5] = CQ_BY_SIZE(block_score_mma_kernel);
-    const int tpt = 16 >> f.lg, row_tiles = (A.q_len + tpt - 1) / tpt;
+    const int tpt = 16 >> f.lg, row_tiles = (A.q_len - 1) / tpt + 1;
     // A CTA's rows are quantised once for all its columns, so it takes many columns as soon as there are two
     // CTAs per SM without splitting them; few row tiles, so that this happens early
     const int tiles = std::min(row_tiles, 4);
-    const int64_t groups = (row_tiles + tiles - 1) / tiles;
+    const int64_t groups = ((int64_t)row_tiles + tiles - 1) / tiles;
     CQ_REQUIRE(groups < 65536, CQ_ERR_UNSUPPORTED, "cq_block_select: too many query tokens");
     const int per = kScoreWarps * kScoreCols;
     const int64_t cols = (A.n + per - 1) / per;
@@ -1321,7 +1321,7 @@ static int launch_topk(const sparse::SelectArgs &A, int64_t rows, cudaStream_t s
   // against 10.0; up to 256 blocks the same either way)
   if (A.n > 256 && A.n <= 1024 && rows >= 12 * sm_count()) {
     auto *fn = A.n <= 512 ? block_topk_regs_kernel<16, Warps::ONE> : block_topk_regs_kernel<32, Warps::ONE>;
-    return launch_after(fn, dim3((unsigned)(A.q_len + 3) / 4, (unsigned)units), 128, 0, st, "cq_block_select", A, 1);
+    return launch_after(fn, dim3(((unsigned)A.q_len + 3) / 4, (unsigned)units), 128, 0, st, "cq_block_select", A, 1);
   }
   // keys a thread: four, or where rows abound so many that up to four warps hold a row (320 rows of 2048 blocks 5.2
   // us against 6.2, 4096 rows 19.4 against 24)
