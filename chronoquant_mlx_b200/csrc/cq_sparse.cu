@@ -38,6 +38,7 @@ struct BoundsArgs {
   int64_t t0, T;            // blocks of tokens t0 .. T-1
   const int64_t *len_dev;   // else: of the last S tokens of *len_dev
   int S, bt, nb;            // nb: blocks per unit in the grid
+  int64_t j0;               // the first of them, without len_dev
   int8_t *codes;
   float *scales;
   int64_t max_blocks;
@@ -59,16 +60,11 @@ __device__ __forceinline__ float ceil_code(float x, float s, float r) {
   return fmaf(-c, s, x) > 0.f ? c + 1.f : c;
 }
 
-// One channel's codes from its range; s: the block's scale (max|x| / 126).
-__device__ __forceinline__ void store_codes(int8_t *codes, int d, int D, float lo, float hi, float s) {
-  float l = 0.f, h = 0.f;
-  if (s > 0.f) {
-    const float r = 1.f / s;
-    h = ceil_code(hi, s, r);
-    l = -ceil_code(-lo, s, r);
-  }
-  codes[d] = (int8_t)fminf(fmaxf(l, -127.f), 127.f);
-  codes[D + d] = (int8_t)fminf(fmaxf(h, -127.f), 127.f);
+// One channel's codes from its range, in the low bytes (lower, upper); s: the
+// block's scale (max|x| / 126), r about 1 / s, both 0 where every key is 0.
+__device__ __forceinline__ int2 range_codes(float lo, float hi, float s, float r) {
+  const float h = ceil_code(hi, s, r), l = -ceil_code(-lo, s, r);
+  return make_int2((int)fminf(fmaxf(l, -127.f), 127.f), (int)fminf(fmaxf(h, -127.f), 127.f));
 }
 
 __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
@@ -110,7 +106,12 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
   for (int w = 0; w < (int)(blockDim.x >> 5); ++w) amax = fmaxf(amax, s_red[w]);
   const float s = __fdiv_rn(amax, 126.f);
   const int64_t row = unit * A.max_blocks + j;
-  if (d < cv.D) store_codes(A.codes + row * 2 * cv.D, d, cv.D, lo, hi, s);
+  if (d < cv.D) {
+    const int2 c = range_codes(lo, hi, s, s > 0.f ? 1.f / s : 0.f);
+    int8_t *codes = A.codes + row * 2 * cv.D + d;
+    codes[0] = (int8_t)c.x;
+    codes[cv.D] = (int8_t)c.y;
+  }
   if (threadIdx.x == 0) A.scales[row] = s;
 }
 
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(256) block_bounds_kernel(BoundsArgs A) {
 // maximum of a code pair): with one word a lane the lanes' meeting at the end,
 // the anchors and the addresses cost a third of what they cost with four (2012
 // instructions per 64 tokens of two anchors then).  8 x 16384 tokens of 8 heads
-// of 128 (78 MB) take 34 us, 73 % issue.  An I-frame's scale slot is
+// of 128 (78 MB) take 33 us with their ranges read back.  An I-frame's scale slot is
 // 0, so whatever its row reads (the row before it, inside the chunk block; the
 // chunk's first token reads row 0) gives p = 0, the anchor itself.
 
@@ -144,31 +145,32 @@ __device__ __forceinline__ void range_of_word(uint32_t word, __half2 scale, __ha
   }
 }
 
+// Positions are stepped from anchor to anchor (divisions for each: 36 us); with
+// nine or ten CTAs an SM, or half the loads in flight: 34, 37 and 39 us.
 template <int D>
-__global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, unsigned n_warps) {
+__global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A) {
   constexpr int W = D / 8, RPI = 32 / W;  // words (lanes) per row, rows at once
   constexpr int UN = 8;                   // steps whose loads are in flight
   const int lane = threadIdx.x & 31;
   ptx::grid_dependency_wait();
   const CacheView &cv = A.cv;
   const CompView &c = cv.c[0];
-  int64_t T = A.T, t0 = A.t0;
+  // positions in 32 bits (the launch keeps them there)
+  unsigned T = (unsigned)A.T, j = (unsigned)A.j0;
   if (A.len_dev) {
-    T = launch_length(A.T, A.len_dev, A.S);
+    T = (unsigned)launch_length(A.T, A.len_dev, A.S);
     if (T == 0) {
-      if (blockIdx.x == 0 && threadIdx.x == 0) set_length_error();
+      if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) set_length_error();
       return;
     }
-    t0 = T - A.S;
+    j = (T - (unsigned)A.S) / (unsigned)A.bt;
   }
-  // positions in 32 bits (the launch keeps them there)
-  const unsigned wi = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (wi >= n_warps) return;
-  const unsigned unit = wi / (unsigned)A.nb;
-  const int j = (int)((unsigned)t0 / (unsigned)A.bt + (wi - unit * (unsigned)A.nb));
-  const int ta = j * A.bt, tb = (int)min((unsigned)T, (unsigned)ta + (unsigned)A.bt);
-  if (ta >= (int)T) return;
-  const int b = (int)(unit / (unsigned)cv.H), h = (int)(unit - (unsigned)b * cv.H);
+  const unsigned wi = blockIdx.x * 4 + (threadIdx.x >> 5), unit = blockIdx.y;
+  if (wi >= (unsigned)A.nb) return;
+  j += wi;
+  if (j * (unsigned)A.bt >= T) return;
+  const int ta = (int)(j * (unsigned)A.bt), tb = (int)min(T, (unsigned)(ta + A.bt));
+  const int b = (int)(unit / (unsigned)cv.H), h = (int)(unit - (unsigned)b * (unsigned)cv.H);
   const int row = lane / W, word = lane % W;  // which of the rows at once, which 8 channels
   const __half2 inf = __float2half2_rn(INFINITY), ninf = __float2half2_rn(-INFINITY);
   __half2 lo[4], hi[4];
@@ -176,14 +178,13 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
   for (int k = 0; k < 4; ++k) lo[k] = inf, hi[k] = ninf;
 
   const int ct = c.pc + c.ac;  // tokens per chunk
-  int t = ta;
-  while (t < tb) {  // one anchor's tokens at a time: they lie in one chunk of one page
-    const int lp = (int)((unsigned)t / (unsigned)cv.P);
-    const int tl = t - lp * cv.P;
-    const int jc = (int)((unsigned)tl / (unsigned)ct), x0 = tl - jc * ct;  // chunk, position in it
-    const int xa = (int)((unsigned)x0 / (unsigned)c.stride);               // its anchor in the chunk
+  // one anchor's tokens at a time: they lie in one chunk of one page
+  int lp = (int)((unsigned)ta / (unsigned)cv.P), tl = ta - lp * cv.P;          // page, position in it
+  int jc = (int)((unsigned)tl / (unsigned)ct), x0 = tl - jc * ct;              // chunk, position in it
+  int xa = (int)((unsigned)x0 / (unsigned)c.stride);                           // its anchor in the chunk
+  for (int t = ta;;) {
     const int n = min(tb - t, (xa + 1) * c.stride - x0);
-    const int64_t ph = page_of(cv, b, lp) * cv.H + h;
+    const int64_t ph = page_of(cv, b, lp) * cv.H + h;  // looked up again rather than held: registers are short
     const uint4 an = *(const uint4 *)(c.kf + ph * c.kf_hs + jc * c.kf_cs + xa * D + word * 8);
     const int i0 = x0 - xa - 1 + row;  // this lane's first code row
     const uint32_t *crow = c.codes + ph * c.cd_hs + jc * c.cd_cs + i0 * W + word;
@@ -219,6 +220,12 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
       hi[k] = __hmax2(hi[k], __hadd2_rn(ptx::u2h2(pr), phi[k]));
     }
     t += n;
+    if (t >= tb) break;
+    ++xa;  // an anchor's last token was passed: the next anchor, chunk or page
+    x0 += n;
+    tl += n;
+    if (x0 == ct) x0 = xa = 0, ++jc;
+    if (tl == cv.P) tl = jc = 0, ++lp;
   }
   // lanes of the same channels: rows meet by halves, each keeping half of its pairs, until a lane holds 4 / RPI pairs
   int k0 = 0;  // first pair this lane still holds
@@ -254,13 +261,21 @@ __global__ void __launch_bounds__(128) block_bounds_rows_kernel(BoundsArgs A, un
   }
   amax = warp_max(amax);
   const float s = __fdiv_rn(amax, 126.f);
+  const float r = s > 0.f ? 1.f / s : 0.f;
   const int64_t at = (int64_t)unit * A.max_blocks + j;
-  int8_t *codes = A.codes + at * 2 * D;
+  int8_t *codes = A.codes + at * 2 * D + word * 8 + k0;
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int d = word * 8 + k0 + k;
-    store_codes(codes, d, D, l[2 * k], u[2 * k], s);
-    store_codes(codes, d + 4, D, l[2 * k + 1], u[2 * k + 1], s);
+  for (int e = 0; e < 2; ++e) {  // NP neighbouring channels from k0 on, and from k0 + 4 on
+    uint32_t lw = 0, uw = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int2 q = range_codes(l[2 * k + e], u[2 * k + e], s, r);
+      lw |= ((uint32_t)q.x & 255u) << (8 * k);
+      uw |= ((uint32_t)q.y & 255u) << (8 * k);
+    }
+    using Store = typename std::conditional<NP == 4, uint32_t, typename std::conditional<NP == 2, uint16_t, uint8_t>::type>::type;
+    *(Store *)(codes + 4 * e) = (Store)lw;
+    *(Store *)(codes + D + 4 * e) = (Store)uw;
   }
   if (lane == 0) A.scales[at] = s;
 }
@@ -1177,16 +1192,19 @@ static int bounds_checks(const cq_paged_cache *cache, int64_t T, int32_t bt, con
 static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const char *what) {
-  const int64_t grid = (int64_t)A.cv.B * A.cv.H * A.nb;
+  const int64_t units = (int64_t)A.cv.B * A.cv.H;
+  CQ_REQUIRE(units < (1LL << 31), CQ_ERR_INVALID, std::string(what) + ": grid too large");
+  const int64_t grid = units * A.nb;
   CQ_REQUIRE(grid < (1LL << 31), CQ_ERR_INVALID, std::string(what) + ": grid too large");
   const CompView &c = A.cv.c[0];
   const int D = A.cv.D, rows = D == 64 ? 4 : D == 128 ? 2 : 1;  // code rows a warp takes at once
   if ((D == 64 || D == 128 || D == 256) && c.order == CQ_ORDER_NATURAL && c.stok && c.stride % rows == 0 &&
-      c.stride > 1 && A.bt % rows == 0 && aligned16(c.kf) && (c.kf_hs | c.kf_cs) % 8 == 0 && A.T + A.bt < (1LL << 31)) {
+      c.stride > 1 && A.bt % rows == 0 && aligned16(c.kf) && (c.kf_hs | c.kf_cs) % 8 == 0 &&
+      A.T + A.bt < (1LL << 31) && units <= 65535) {
     auto *fn = D == 64    ? sparse::block_bounds_rows_kernel<64>
                : D == 128 ? sparse::block_bounds_rows_kernel<128>
                           : sparse::block_bounds_rows_kernel<256>;
-    return launch_after(fn, dim3((unsigned)((grid + 3) / 4)), 128, 0, st, what, A, (unsigned)grid);
+    return launch_after(fn, dim3((unsigned)((A.nb - 1) / 4 + 1), (unsigned)units), 128, 0, st, what, A);
   }
   const int threads = (A.cv.D + 31) & ~31;
   return launch_after(sparse::block_bounds_kernel, dim3((unsigned)grid), threads, 0, st, what, A);
@@ -1198,7 +1216,8 @@ extern "C" int cq_block_bounds(const cq_paged_cache *cache, int64_t t0, int64_t 
   if (r) return r;
   CQ_REQUIRE(t0 >= 0 && t0 <= T, CQ_ERR_INVALID, "cq_block_bounds: t0 must lie in [0, T]");
   if (t0 == T) return CQ_OK;
-  sparse::BoundsArgs A{make_view(*cache), t0, T, nullptr, 0, block_tokens, 0, codes, scales, max_blocks};
+  sparse::BoundsArgs A{make_view(*cache), t0,   T,     nullptr, 0, block_tokens, 0, t0 / block_tokens,
+                       codes,             scales, max_blocks};
   A.nb = (int)((T - 1) / block_tokens - t0 / block_tokens + 1);
   return launch_bounds(A, (cudaStream_t)stream, "cq_block_bounds");
 }
@@ -1209,8 +1228,9 @@ extern "C" int cq_block_bounds_at(const cq_paged_cache *cache, const int64_t *le
   int r = bounds_checks(cache, max_len, block_tokens, codes, scales, max_blocks, "cq_block_bounds_at");
   if (r) return r;
   CQ_REQUIRE(len_dev && S >= 1 && S <= max_len, CQ_ERR_INVALID, "cq_block_bounds_at: bad length arguments");
-  sparse::BoundsArgs A{make_view(*cache), 0, max_len, len_dev, S, block_tokens, 0, codes, scales, max_blocks};
-  A.nb = (S + block_tokens - 2) / block_tokens + 1;  // the most blocks S tokens can touch
+  sparse::BoundsArgs A{make_view(*cache), 0,    max_len, len_dev, S, block_tokens, 0, 0,
+                       codes,             scales, max_blocks};
+  A.nb = (int)(((int64_t)S + block_tokens - 2) / block_tokens + 1);  // the most blocks S tokens can touch
   return launch_bounds(A, (cudaStream_t)stream, "cq_block_bounds_at");
 }
 
