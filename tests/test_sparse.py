@@ -317,7 +317,7 @@ def test_select_many_equal_scores(blocks):
 @gpu
 @pytest.mark.parametrize("kind", ["normal", "skewed", "two values", "outliers"])
 @pytest.mark.parametrize("S,blocks", [(450, 200), (450, 300), (450, 1000), (100, 1000), (75, 1500), (75, 4000),
-                                      (9, 4000), (1, 700)])
+                                      (9, 4000), (3, 6000), (40, 9000), (1, 700)])
 def test_select_of_many_rows(S, blocks, kind):
     """Every form of the search (a warp, up to four or more warps a row) on
     scores that do and do not look normal, padded and not, for short, middle and
