@@ -215,7 +215,8 @@ class Qwen3StyleDecoder:
     # -- context ---------------------------------------------------------------
     def fill_context(self, T0: int, chunk: int = 4096, seed: int = 1) -> None:
         """Encode a synthetic T0-token context into every layer's cache (under
-        a sequence split, this rank's token range of it)."""
+        a sequence split, this rank's token range of it).  A step captured
+        before is dropped: capture again."""
         c = self.cfg
         g = torch.Generator(device=self.device).manual_seed(seed)
         h0, h1 = self.rank * self.kv_heads, (self.rank + 1) * self.kv_heads  # this rank's kv-heads
@@ -299,7 +300,9 @@ class Qwen3StyleDecoder:
 
     def _prepare_attention(self) -> None:
         """Per-layer descriptors, device-resident lengths and one shared
-        workspace (layers run in order on one stream)."""
+        workspace (layers run in order on one stream).  A step captured before
+        holds the addresses of the old ones: it is dropped."""
+        self.graph = None
         lib = _lib.lib()
         need_max = 0
         if self.sparse is not None:

@@ -155,3 +155,19 @@ def test_prefill_refusals():
     m.seq_group = object()
     with pytest.raises(NotImplementedError):
         m.prefill(prompt(2, 4))
+
+
+@gpu
+def test_a_new_context_drops_the_captured_step():
+    """A captured step holds the lengths and buffers of the context it was
+    captured over: a context filled in afterwards needs another capture."""
+    for sparse in (None, dict(top=4)):
+        m = Qwen3StyleDecoder(CFG, 2, 200, FT, seed=3, sparse=sparse)
+        m.fill_context(100)
+        m.capture()
+        m.fill_context(20)
+        with pytest.raises(RuntimeError, match="capture"):
+            m.decode(1)
+        m.capture()
+        assert torch.isfinite(m.decode(2)).all()
+        assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == 122
