@@ -227,6 +227,7 @@ class Qwen3StyleDecoder:
             t_lo, t_hi = shard_bounds(T0, self.seq_world, c0.stride_k, c0.stride_v)[self.seq_rank]
             if t_hi <= t_lo:
                 raise ValueError("sequence split: every rank needs a non-empty token range")
+        self._follow_steps()
         for L in self.layers:
             for t in range(0, T0, chunk):
                 n = min(chunk, T0 - t)
@@ -241,13 +242,14 @@ class Qwen3StyleDecoder:
     # -- prompts -----------------------------------------------------------------
     def prefill(self, ids: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         """Run the prompt ``ids`` [B, S] through the model after whatever the
-        caches hold, ``chunk`` tokens at a time, and encode its K/V.  Returns the
-        last token's logits [B, vocab]; the next step starts from their argmax.
-        A step captured before is dropped (it holds the old lengths): capture again."""
+        caches hold (tokens of eager steps among it), ``chunk`` tokens at a time,
+        and encode its K/V.  Returns the last token's logits [B, vocab]; the next
+        step starts from their argmax.  A step captured before is dropped (it holds the old lengths): capture again."""
         if self.seq_group is not None:
             raise NotImplementedError("prefill under a sequence split is not supported")
         if ids.dim() != 2 or ids.shape[0] != self.B or ids.shape[1] < 1 or chunk < 1:
             raise ValueError(f"prefill: ids must be [{self.B}, S] with S >= 1, got {tuple(ids.shape)}")
+        self._follow_steps()
         t0 = self.layers[0]["cache"].offset
         if t0 + ids.shape[1] > self.max_len:
             raise ValueError(f"prefill past max_len {self.max_len}")
@@ -298,6 +300,18 @@ class Qwen3StyleDecoder:
             L["index"] = BlockIndex(L["cache"], self.sparse["block_tokens"])
         return L["index"]
 
+    def _follow_steps(self) -> None:
+        """Bring the caches' host-side offsets up to what eager steps encoded:
+        those advance the lengths on the device alone.  (A caller's own attention
+        appends through the cache, whose offset is ahead then; a restored cache has
+        another store, which no step has written.)"""
+        if not self.tail:  # a sequence split's other ranks hold a fixed range
+            return
+        known = [L for L in self.layers if L.get("store") is not None and L["store"] is L["cache"].store]
+        if known:
+            for L, n in zip(known, torch.stack([L["len"][0] for L in known]).tolist()):
+                L["cache"].offset = max(L["cache"].offset, n)
+
     def _prepare_attention(self) -> None:
         """Per-layer descriptors, device-resident lengths and one shared
         workspace (layers run in order on one stream).  A step captured before
@@ -311,6 +325,7 @@ class Qwen3StyleDecoder:
             st = L["cache"].store
             st.ensure(self.max_len, self.max_len)
             L["desc"] = st.descriptor()
+            L["store"] = st
             L["len"] = torch.tensor([L["cache"].offset, 0], dtype=torch.int64, device=self.device)
             need = ctypes.c_size_t(0)
             _lib.check(lib.cq_attention_workspace(ctypes.byref(L["desc"]), self.max_len, self.heads, 1, 0,
@@ -467,7 +482,9 @@ class Qwen3StyleDecoder:
 
     def step_eager(self, attention=None) -> torch.Tensor:
         """One decode step without a graph (``attention(L, q, k, v)`` may
-        replace the kernel, e.g. by a reference).  Returns logits [B, vocab]."""
+        replace the kernel, e.g. by a reference).  Returns logits [B, vocab].
+        No host sync: the length on the device advances, and the caches' host-side
+        offsets follow at the next ``prefill`` or ``fill_context``."""
         return self._step_body(attention)
 
     def capture(self) -> None:

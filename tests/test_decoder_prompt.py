@@ -171,3 +171,43 @@ def test_a_new_context_drops_the_captured_step():
         m.capture()
         assert torch.isfinite(m.decode(2)).all()
         assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == 122
+
+
+@gpu
+@pytest.mark.parametrize("sparse", [None, dict(top=6)])
+def test_prompts_and_eager_steps_in_turn(sparse):
+    """Eager steps advance the length on the device alone; a prompt behind them
+    goes on from there, and so does a filled-in context."""
+    ids = prompt(2, 75)
+    whole = Qwen3StyleDecoder(CFG, 2, 120, FT, seed=3).prefill(ids)
+    m = Qwen3StyleDecoder(CFG, 2, 120, FT, seed=3, sparse=sparse)
+    m.prefill(ids[:, :60])
+    for t in range(60, 63):
+        m.ids.copy_(ids[:, t])
+        m.step_eager()
+    m.prefill(ids[:, 63:70])
+    assert m.layers[0]["cache"].offset == m.layers[1]["cache"].offset == int(m.pos) == 70
+    m.ids.copy_(ids[:, 70])
+    m.step_eager()
+    got = m.prefill(ids[:, 71:])
+    assert rel(got, whole) < 2e-2
+    for L in m.layers:
+        assert L["cache"].offset == int(L["len"][0]) == 75
+        assert sparse is None or L["index"].covered == 75
+    # a caller's own attention appends through the cache: its offset is the length then
+    def attend(L, q, k, v):
+        L["cache"].update_and_fetch(k.unsqueeze(2), v.unsqueeze(2))
+        return q
+    m.step_eager(attend)
+    m.prefill(ids[:, :2])
+    assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == int(m.pos) == 78
+    # another state restored into the caches is what the next prompt follows, however short
+    for L in m.layers:
+        c = type(L["cache"])(**FT)
+        c.update_and_fetch(*(torch.randn((2, 2, 40, 128), device="cuda").bfloat16() for _ in range(2)))
+        L["cache"].state = c.state
+    m.prefill(ids[:, :2])
+    assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == int(m.pos) == 42
+    m.step_eager()
+    m.fill_context(5)
+    assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == 48
