@@ -244,7 +244,9 @@ class Qwen3StyleDecoder:
         """Run the prompt ``ids`` [B, S] through the model after whatever the
         caches hold (tokens of eager steps among it), ``chunk`` tokens at a time,
         and encode its K/V.  Returns the last token's logits [B, vocab]; the next
-        step starts from their argmax.  A step captured before is dropped (it holds the old lengths): capture again."""
+        step starts from their argmax.  A step captured before is dropped (it
+        holds the old lengths): capture again.  After an error the caches hold what
+        they held before the call."""
         if self.seq_group is not None:
             raise NotImplementedError("prefill under a sequence split is not supported")
         if ids.dim() != 2 or ids.shape[0] != self.B or ids.shape[1] < 1 or chunk < 1:
@@ -255,12 +257,23 @@ class Qwen3StyleDecoder:
             raise ValueError(f"prefill past max_len {self.max_len}")
         ids = ids.to(self.device)
         self.graph = None
-        for a in range(0, ids.shape[1], chunk):
-            xn = self._chunk_body(ids[:, a:a + chunk], t0 + a)
-        logits = xn.view(self.B, -1, self.cfg.hidden)[:, -1] @ self.lm_head.t()
+        before = [(L, dict(L), L["cache"].offset) for L in self.layers]
+        try:
+            for a in range(0, ids.shape[1], chunk):
+                xn = self._chunk_body(ids[:, a:a + chunk], t0 + a)
+            logits = xn.view(self.B, -1, self.cfg.hidden)[:, -1] @ self.lm_head.t()
+            self._prepare_attention()
+        except BaseException:  # what layers encoded so far is behind their offsets again, and written over next time
+            for L, held, offset in before:
+                L.clear()
+                L.update(held)
+                L["cache"].offset = offset
+                if "index" in L:  # its last block's ranges may hold more than the tokens before: summarised anew
+                    bt = self.sparse["block_tokens"]
+                    L["index"].covered = min(L["index"].covered, offset // bt * bt)
+            raise
         self.ids.copy_(logits.argmax(-1))
         self.pos.fill_(t0 + ids.shape[1])
-        self._prepare_attention()
         return logits
 
     def _chunk_body(self, ids: torch.Tensor, t0: int) -> torch.Tensor:

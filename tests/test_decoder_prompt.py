@@ -211,3 +211,37 @@ def test_prompts_and_eager_steps_in_turn(sparse):
     m.step_eager()
     m.fill_context(5)
     assert m.layers[1]["cache"].offset == int(m.layers[1]["len"][0]) == 48
+
+
+@gpu
+@pytest.mark.parametrize("sparse", [None, dict(top=4, block_tokens=32)])
+def test_a_prompt_that_failed_can_be_run_again(sparse, monkeypatch):
+    """An error inside a chunk (no memory, say) leaves every layer's cache and
+    index at the length before the prompt."""
+    ids = prompt(2, 90)
+    a, b = (Qwen3StyleDecoder(CFG, 2, 200, FT, seed=3, sparse=sparse) for _ in range(2))
+    for m in (a, b):
+        m.fill_context(150 - 40)
+    attend, seen = b._chunk_attention, []
+
+    def fail(L, q):
+        seen.append(q.shape[2])
+        out = attend(L, q)
+        if len(seen) == 4:  # the second layer of the second chunk
+            raise torch.cuda.OutOfMemoryError("no memory")
+        return out
+
+    monkeypatch.setattr(b, "_chunk_attention", fail)
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        b.prefill(ids, chunk=40)
+    for L in b.layers:
+        assert L["cache"].offset == 110
+        if sparse:
+            fresh = BlockIndex(L["cache"], 32).update()
+            assert torch.equal(L["index"].update().bounds(), fresh.bounds()) and L["index"].covered == 110
+    assert torch.equal(b.prefill(ids, chunk=30), a.prefill(ids, chunk=30))
+    for x, y in zip(a.layers, b.layers):
+        assert x["cache"].offset == y["cache"].offset == 200
+        for s, t in zip(x["cache"].state, y["cache"].state):
+            assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
+        assert sparse is None or torch.equal(x["index"].bounds(), y["index"].bounds())
