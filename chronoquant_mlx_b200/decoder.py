@@ -340,10 +340,11 @@ class Qwen3StyleDecoder:
             L["desc"] = st.descriptor()
             L["store"] = st
             L["len"] = torch.tensor([L["cache"].offset, 0], dtype=torch.int64, device=self.device)
-            need = ctypes.c_size_t(0)
-            _lib.check(lib.cq_attention_workspace(ctypes.byref(L["desc"]), self.max_len, self.heads, 1, 0,
-                                                  ctypes.byref(need)), "decoder")
-            need_max = max(need_max, need.value)
+            if self.sparse is None:  # a sparse step has a workspace of its own
+                need = ctypes.c_size_t(0)
+                _lib.check(lib.cq_attention_workspace(ctypes.byref(L["desc"]), self.max_len, self.heads, 1, 0,
+                                                      ctypes.byref(need)), "decoder")
+                need_max = max(need_max, need.value)
         self.workspace = torch.zeros(max(1, (need_max + 3) // 4), dtype=torch.float32, device=self.device)
         self.attn_out = torch.empty((self.B, self.heads, self.cfg.head_dim), dtype=self.dtype, device=self.device)
         if self.seq_group is not None:
@@ -379,13 +380,20 @@ class Qwen3StyleDecoder:
         """Encode this step's k/v, refresh the newest block's key ranges, list
         the blocks each kv-head's queries attend to and attend over them."""
         lib, sp, st, index = _lib.lib(), self.sparse, stream_ptr(self.device), L["index"]
-        ks, vs, qs, bt = k.stride(), v.stride(), q.stride(), sp["block_tokens"]
+        ks, vs = k.stride(), v.stride()
         d, n = ctypes.byref(L["desc"]), L["len"].data_ptr()
-        codes, scales, cap = index.codes.data_ptr(), index.scales.data_ptr(), index.codes.shape[2]
-        ws, wsb = self.sparse_ws.data_ptr(), self.sparse_ws.numel()
         _lib.check(lib.cq_append_at(d, k.data_ptr(), ks[0], ks[1], 0, v.data_ptr(), vs[0], vs[1], 0, cq_dtype(k), n, 1,
                                     st), "decoder")
-        _lib.check(lib.cq_block_bounds_at(d, n, self.max_len, 1, bt, codes, scales, cap, st), "decoder")
+        _lib.check(lib.cq_block_bounds_at(d, n, self.max_len, 1, sp["block_tokens"], index.codes.data_ptr(),
+                                          index.scales.data_ptr(), index.codes.shape[2], st), "decoder")
+        return self._sparse_attend(L, q)
+
+    def _sparse_attend(self, L: dict, q: torch.Tensor) -> torch.Tensor:
+        """The part of a sparse step that reads the cache only: list, attend."""
+        lib, sp, st, index = _lib.lib(), self.sparse, stream_ptr(self.device), L["index"]
+        qs, bt, d, n = q.stride(), sp["block_tokens"], ctypes.byref(L["desc"]), L["len"].data_ptr()
+        codes, scales, cap = index.codes.data_ptr(), index.scales.data_ptr(), index.codes.shape[2]
+        ws, wsb = self.sparse_ws.data_ptr(), self.sparse_ws.numel()
         _lib.check(lib.cq_block_select(codes, scales, cap, bt, self.B, self.kv_heads, self.cfg.head_dim, self.max_len, n,
                                        q.data_ptr(), cq_dtype(q), self.heads, 1, qs[0], qs[1], 0, None, sp["first"],
                                        sp["recent"], sp["top"], self.blocks.data_ptr(), None, ws, wsb, st), "decoder")
@@ -501,11 +509,13 @@ class Qwen3StyleDecoder:
         return self._step_body(attention)
 
     def capture(self) -> None:
-        """Capture one decode step as a CUDA graph (after ``fill_context``)."""
+        """Capture one decode step as a CUDA graph (after ``fill_context`` or
+        ``prefill``).  The dense step runs in the decode kernel and takes its
+        layouts; a sparse one takes every layout and group of the cache."""
         lib = _lib.lib()
         c = self.cfg
         # one-time set-up outside the capture: cuBLAS handles (one matmul of each
-        # shape) and the attention kernel's attributes (a read-only attention call)
+        # shape) and the attention kernels' attributes (a read-only attention call)
         x = torch.zeros((self.B, c.hidden), device=self.device, dtype=self.dtype)
         L0 = self.layers[0]
         for wt in (L0["wqkv"], L0["wgu"], self.lm_head):
@@ -519,10 +529,13 @@ class Qwen3StyleDecoder:
             self._merge_partials()
         q = torch.zeros((self.B, self.heads, c.head_dim), device=self.device, dtype=self.dtype)
         qs = q.stride()
-        _lib.check(lib.cq_attention_at(ctypes.byref(L0["desc"]), L0["len"].data_ptr(), self.max_len, q.data_ptr(),
-                                       cq_dtype(q), self.heads, qs[0], qs[1], 1.0, self.attn_out.data_ptr(),
-                                       cq_dtype(self.attn_out), None, self.workspace.data_ptr(),
-                                       self.workspace.numel() * 4, stream_ptr(self.device)), "decoder")
+        if self.sparse is not None:
+            self._sparse_attend(L0, q)
+        else:
+            _lib.check(lib.cq_attention_at(ctypes.byref(L0["desc"]), L0["len"].data_ptr(), self.max_len, q.data_ptr(),
+                                           cq_dtype(q), self.heads, qs[0], qs[1], 1.0, self.attn_out.data_ptr(),
+                                           cq_dtype(self.attn_out), None, self.workspace.data_ptr(),
+                                           self.workspace.numel() * 4, stream_ptr(self.device)), "decoder")
         torch.cuda.synchronize(self.device)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):

@@ -245,3 +245,25 @@ def test_a_prompt_that_failed_can_be_run_again(sparse, monkeypatch):
         for s, t in zip(x["cache"].state, y["cache"].state):
             assert torch.equal(s.view(torch.uint8), t.view(torch.uint8))
         assert sparse is None or torch.equal(x["index"].bounds(), y["index"].bounds())
+
+
+@gpu
+@pytest.mark.parametrize("cfg,kw", [(CFG, dict(stride_k=12, stride_v=4)),
+                                    (DecoderConfig(layers=2, hidden=512, heads=32, kv_heads=2, head_dim=128, ffn=1024,
+                                                   vocab=1000), FT)])
+def test_sparse_steps_of_other_layouts_are_captured(cfg, kw):
+    """Layouts and groups (of 16 heads) that the dense decode kernel does not
+    take: a sparse step needs none of it, captured steps are the eager ones."""
+    T0, sp = 300, dict(top=4, block_tokens=32)
+    g, e = (Qwen3StyleDecoder(cfg, 2, T0 + 40, kw, seed=3, sparse=sp) for _ in range(2))
+    for m in (g, e):
+        m.fill_context(T0)
+    g.capture()
+    for i in range(30):  # past a block's end
+        ids = torch.tensor([5 + i, 77 - i], device="cuda")
+        g.ids.copy_(ids)
+        e.ids.copy_(ids)
+        lg, le = g.decode(1).float().clone(), e.step_eager().float()
+        assert rel(lg, le) <= 1e-3, i
+        assert torch.equal(g.blocks, e.blocks), i
+    assert g.layers[1]["cache"].offset == int(g.layers[1]["len"][0]) == T0 + 30
