@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <dlfcn.h>
@@ -87,6 +88,14 @@ struct Launch {
     stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   }
 };
+
+// The id of the capture that records the stream, 0 where it runs.
+unsigned long long capture_id(void *stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id));
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
 
 // Queries [B, Hq, Tq, D] of a cache of H kv-heads on `device`, holding T tokens.
 struct Queries {
@@ -250,7 +259,7 @@ struct Index {
   }
 };
 
-// block_bounds(descriptor, t0, T, block_tokens, codes, scales)
+// block_bounds(descriptor, t0, T, block_tokens, codes, scales) -> the id of the capture that recorded it, 0: it runs
 PyObject *block_bounds(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 6, [](PyObject *const *a) {
     const Index ix(a[4], a[5]);
@@ -258,7 +267,15 @@ PyObject *block_bounds(PyObject *, PyObject *const *args, Py_ssize_t n) {
     check(L.bounds((const cq_paged_cache *)integer(a[0]), integer(a[1]), integer(a[2]), int32(a[3], "block_tokens"),
                    (int8_t *)ix.codes.mutable_data_ptr(), ix.scales.mutable_data_ptr<float>(), ix.cap, at_.stream),
           "BlockIndex.update");
-    Py_RETURN_NONE;
+    return PyLong_FromUnsignedLongLong(capture_id(at_.stream));
+  });
+}
+
+// capture_of(codes) -> the id of the capture that records the stream of the index's device, 0 where it runs
+PyObject *capture_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  return guarded(args, n, 1, [](PyObject *const *a) {
+    const Launch at_(tensor(a[0], "codes"));
+    return PyLong_FromUnsignedLongLong(capture_id(at_.stream));
   });
 }
 
@@ -384,7 +401,7 @@ PyObject *load(PyObject *, PyObject *args) {
 
 #define FAST(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(qk_norm_rope), FAST(block_bounds),     FAST(block_bounds_read),
-                         FAST(block_select), FAST(sparse_attention), {"load", load, METH_VARARGS, nullptr},
+                         FAST(capture_of),   FAST(block_select),     FAST(sparse_attention), {"load", load, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

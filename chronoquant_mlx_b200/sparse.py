@@ -41,7 +41,14 @@ class BlockIndex:
     ``block_tokens``: tokens per block, a multiple of 16 (64 suits the cache's
     chunk sizes).  ``codes`` int8 [B, Hkv, capacity, 2, D] and ``scales`` fp32
     [B, Hkv, capacity] follow the cache's page pool; ``covered`` is the number
-    of tokens summarised."""
+    of tokens summarised.
+
+    An update recorded into a CUDA graph counts for the calls of that capture;
+    ``covered`` stays what it was, and what comes later summarises those tokens
+    for itself.  A replay summarises the tokens of its capture: after the cache
+    has grown it leaves the last of their blocks short, until ``update(start)``
+    from that length.  ``reserve`` room before a capture: growing moves the
+    tensors, which a graph's replays would not follow."""
 
     def __init__(self, cache, block_tokens: int = 64):
         if int(block_tokens) < 16 or int(block_tokens) % 16:
@@ -51,12 +58,19 @@ class BlockIndex:
         self.codes = None
         self.scales = None
         self.covered = 0
+        self._recorded = None  # (capture, tokens) of the last update that a capture recorded
         self._store = None
+
+    def _tokens(self) -> int:
+        """Tokens summarised for the next call: ``covered``, or what the capture it is recorded by recorded before."""
+        if self._recorded is not None and self._recorded[0] == _lib.calls().capture_of(self.codes):
+            return self._recorded[1]
+        return self.covered
 
     @property
     def n_blocks(self) -> int:
         """Blocks summarised so far (the last one may be partial)."""
-        return -(-self.covered // self.block_tokens)
+        return -(-self._tokens() // self.block_tokens)
 
     @property
     def nbytes(self) -> int:
@@ -68,13 +82,19 @@ class BlockIndex:
         if st is None:
             raise ValueError("BlockIndex: the cache is empty")
         if st is not self._store:  # another store (a restored state): nothing of the old ranges holds
-            self._store, self.codes, self.scales, self.covered = st, None, None, 0
+            self._store, self.codes, self.scales, self.covered, self._recorded = st, None, None, 0, None
         need = -(-max(int(tokens), st.capacity_tokens()) // self.block_tokens)
         have = 0 if self.codes is None else self.codes.shape[2]
         if need <= have:
             return
-        codes = torch.zeros((st.B, st.H, need, 2, st.D), dtype=torch.int8, device=st.device)
-        scales = torch.zeros((st.B, st.H, need), dtype=torch.float32, device=st.device)
+        with torch.cuda.device(st.device):
+            recorded = torch.cuda.is_current_stream_capturing()
+        if have and recorded:
+            raise RuntimeError("BlockIndex: the index has to grow, which a capture cannot record; reserve() before it")
+        # in a capture no zeros either: a replay would write them over ranges summarised since
+        new = torch.empty if recorded else torch.zeros
+        codes = new((st.B, st.H, need, 2, st.D), dtype=torch.int8, device=st.device)
+        scales = new((st.B, st.H, need), dtype=torch.float32, device=st.device)
         if have:
             codes[:, :, :have].copy_(self.codes)
             scales[:, :, :have].copy_(self.scales)
@@ -95,8 +115,12 @@ class BlockIndex:
         if not 0 <= t0 <= T:
             raise ValueError(f"BlockIndex: start {t0} outside [0, {T}]")
         t0 = min(t0, self.covered)
-        _lib.calls().block_bounds(ctypes.addressof(st.descriptor()), t0, T, self.block_tokens, self.codes, self.scales)
-        self.covered = T
+        capture = _lib.calls().block_bounds(ctypes.addressof(st.descriptor()), t0, T, self.block_tokens, self.codes,
+                                            self.scales)
+        if capture:
+            self._recorded = (capture, T)
+        else:
+            self.covered, self._recorded = T, None
         return self
 
     def bounds(self, first: int = 0) -> torch.Tensor:
@@ -119,10 +143,11 @@ class BlockIndex:
         the lower index).  ``starts``: int64 [B], first real token of each
         sequence.  ``return_scores``: also the listed blocks' scores (fp32, -inf
         behind), by which lists of ranks that share a sequence can be merged."""
-        if self.covered != self.cache.offset or self.cache.store is not self._store or self.covered == 0:
+        T = self.cache.offset
+        if T == 0 or self.cache.store is not self._store or self.covered != T and self._tokens() != T:
             self.update()
-        return _lib.calls().block_select(self.codes, self.scales, self.block_tokens, self.covered, queries, top, first,
-                                         recent, starts, return_scores)
+        return _lib.calls().block_select(self.codes, self.scales, self.block_tokens, T, queries, top, first, recent,
+                                         starts, return_scores)
 
 
 @traced("cq.sparse_sdpa")

@@ -812,3 +812,72 @@ def test_c_sizes_past_32_bits_are_refused():
     for over in (dict(Hq=2 ** 30), dict(S=2 ** 28, T=2 ** 29)):
         assert L.cq_sparse_attention(far, *{**SPARSE_ARGS, **over}.values(), None) == -2
     assert L.cq_block_bounds_read(P, P, 2 ** 40, 2 ** 40, 0, 2 ** 40, 128, P, None) == -1
+
+
+@gpu
+def test_a_captured_update_counts_once_it_has_run():
+    """update() in a capture summarises nothing until the graph is replayed:
+    what runs meanwhile does not take the ranges for granted."""
+    cache = make_cache(2, 2, 150, 128, seed=3)
+    index = BlockIndex(cache, 32)
+    index.reserve(400)
+    index.update()
+    more = make_cache(2, 2, 100, 128, seed=4).reconstruct_history()
+    cache.update_and_fetch(*more)
+    q = queries(2, 8, 1, 128, torch.float16)
+    fresh = BlockIndex(cache, 32).update()
+    want, bounds = fresh.select(q, 4, return_scores=True), fresh.bounds()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        ranges = index.update().bounds()  # 250 tokens here, recorded
+        lists = index.select(q, 4)
+        assert index.n_blocks == 8
+    assert index.covered == 150 and index.n_blocks == 5 and index.bounds().shape[2] == 5
+    with torch.cuda.graph(second):
+        others = index.select(q, 4, return_scores=True)  # its own update, not the other graph's
+    second.replay()
+    assert torch.equal(others[0], want[0]) and torch.equal(others[1], want[1])
+    index.codes[:, :, 4:].zero_()  # as before the replay
+    got = index.select(q, 4, return_scores=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert index.covered == 250 and torch.equal(index.bounds(), bounds)
+    index.codes[:, :, 4:].zero_()
+    first.replay()
+    assert torch.equal(ranges, bounds) and torch.equal(lists, want[0])
+    assert torch.equal(index.bounds(), bounds)
+
+
+@gpu
+def test_an_index_allocated_in_a_capture():
+    """An index made inside a capture computes everything when replayed.  A
+    replay summarises the tokens of the capture, so of what other calls computed
+    meanwhile its last block alone is lost, which an update from there brings back."""
+    cache = make_cache(1, 2, 200, 128, seed=3)
+    q = queries(1, 8, 1, 128, torch.float16)
+    want = BlockIndex(cache, 32).select(q, 3)
+    index, graph = BlockIndex(cache, 32), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = index.update().select(q, 3)
+    graph.replay()
+    assert torch.equal(got, want)
+    cache.update_and_fetch(*(x[:, :, :30] for x in make_cache(1, 2, 100, 128, seed=4).reconstruct_history()))
+    index.update()
+    graph.replay()
+    now = BlockIndex(cache, 32).update().bounds()
+    assert torch.equal(index.bounds()[:, :, :6], now[:, :, :6]) and torch.equal(index.bounds(7), now[:, :, 7:])
+    assert torch.equal(index.update(200).bounds(), now)
+
+
+@gpu
+def test_an_index_does_not_grow_in_a_capture():
+    """Growing moves the ranges; a replay would copy them from memory given
+    back since.  Refused, and the index still works."""
+    cache = make_cache(1, 1, 250, 128, seed=3)
+    index = BlockIndex(cache, 32).update()
+    cache.update_and_fetch(*make_cache(1, 1, 600, 128, seed=4).reconstruct_history())  # the pool grows
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="reserve"):
+        with torch.cuda.graph(graph):
+            index.update()
+    assert index.covered == 250
+    assert torch.equal(index.update().bounds(), BlockIndex(cache, 32).update().bounds())
