@@ -81,10 +81,9 @@ class BlockIndex:
         st = self.cache.store
         if st is None:
             raise ValueError("BlockIndex: the cache is empty")
-        if st is not self._store:  # another store (a restored state): nothing of the old ranges holds
-            self._store, self.codes, self.scales, self.covered, self._recorded = st, None, None, 0, None
+        other = st is not self._store  # a restored state: nothing of the old ranges holds
         need = -(-max(int(tokens), st.capacity_tokens()) // self.block_tokens)
-        have = 0 if self.codes is None else self.codes.shape[2]
+        have = 0 if other or self.codes is None else self.codes.shape[2]
         if need <= have:
             return
         with torch.cuda.device(st.device):
@@ -98,7 +97,9 @@ class BlockIndex:
         if have:
             codes[:, :, :have].copy_(self.codes)
             scales[:, :, :have].copy_(self.scales)
-        self.codes, self.scales = codes, scales
+        self.codes, self.scales = codes, scales  # from here on nothing fails
+        if other:
+            self._store, self.covered, self._recorded = st, 0, None
 
     @traced("cq.block_bounds")
     def update(self, start: int | None = None) -> "BlockIndex":

@@ -881,3 +881,30 @@ def test_an_index_does_not_grow_in_a_capture():
             index.update()
     assert index.covered == 250
     assert torch.equal(index.update().bounds(), BlockIndex(cache, 32).update().bounds())
+
+
+@gpu
+def test_an_index_without_memory_to_grow_is_left_as_it_was(monkeypatch):
+    """No memory for the ranges of a restored or longer cache: the call fails,
+    and the next one starts over."""
+    cache = make_cache(1, 1, 100, 128, seed=3)
+    index = BlockIndex(cache, 32).update()
+    q = queries(1, 4, 1, 128, torch.float16)
+    zeros = torch.zeros
+
+    def refuse(size, **kw):
+        if kw.get("dtype") is torch.float32:  # the second of the index's two tensors
+            raise torch.cuda.OutOfMemoryError("no memory")
+        return zeros(size, **kw)
+
+    for other in (make_cache(1, 1, 700, 128, seed=5), make_cache(1, 1, 90, 128, seed=6)):
+        cache.state = other.state
+        with monkeypatch.context() as m:
+            m.setattr(torch, "zeros", refuse)
+            for call in (index.update, lambda: index.select(q, 3), index.update):
+                with pytest.raises(torch.cuda.OutOfMemoryError):
+                    call()
+            with pytest.raises(ValueError, match="replaced"):
+                index.bounds()
+        assert torch.equal(index.select(q, 3), BlockIndex(other, 32).select(q, 3))
+        assert torch.equal(index.bounds(), BlockIndex(other, 32).update().bounds())
