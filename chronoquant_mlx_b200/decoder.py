@@ -251,6 +251,11 @@ class Qwen3StyleDecoder:
             raise NotImplementedError("prefill under a sequence split is not supported")
         if ids.dim() != 2 or ids.shape[0] != self.B or ids.shape[1] < 1 or chunk < 1:
             raise ValueError(f"prefill: ids must be [{self.B}, S] with S >= 1, got {tuple(ids.shape)}")
+        if ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"prefill: ids must be int32 or int64, got {ids.dtype}")
+        lo, hi = (int(x) for x in ids.aminmax())  # an embedding row that is not there would end the GPU context
+        if lo < 0 or hi >= self.cfg.vocab:
+            raise ValueError(f"prefill: ids {lo} to {hi} outside [0, {self.cfg.vocab})")
         self._follow_steps()
         t0 = self.layers[0]["cache"].offset
         if t0 + ids.shape[1] > self.max_len:

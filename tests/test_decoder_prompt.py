@@ -267,3 +267,18 @@ def test_sparse_steps_of_other_layouts_are_captured(cfg, kw):
         assert rel(lg, le) <= 1e-3, i
         assert torch.equal(g.blocks, e.blocks), i
     assert g.layers[1]["cache"].offset == int(g.layers[1]["len"][0]) == T0 + 30
+
+
+def test_prefill_refuses_ids_outside_the_vocabulary():
+    """An embedding row that is not there would end the process's GPU context: refused on the host."""
+    m = Qwen3StyleDecoder(CFG, 2, 64, device="cpu")
+    good = prompt(2, 4)
+    for bad in (-1, -CFG.vocab, CFG.vocab, 2 ** 40):
+        ids = good.clone()
+        ids[1, 2] = bad
+        with pytest.raises(ValueError, match="outside"):
+            m.prefill(ids)
+    for dtype in (torch.float32, torch.bool, torch.uint8):  # masks, to an indexing
+        with pytest.raises(TypeError, match="int32 or int64"):
+            m.prefill((good > 0).to(dtype))
+    assert m.layers[0]["cache"].offset == 0
