@@ -103,8 +103,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const void *qkv, int6
 }
 
 // Head norm and rotation of many tokens.  The angle of a channel pair is pos *
-// inv_freq in fp64 (a product of two fp32 numbers is off by radians at far
-// positions), reduced to [-pi, pi] there; its sine and cosine are shared by the
+// inv_freq in fp64 as a product and what its rounding left off (a product of two
+// fp32 numbers is off by radians at far positions, one rounded to fp64 by 6e-5 at
+// 2^40), reduced to [-pi, pi] there; its sine and cosine are shared by the
 // token's heads.  All arithmetic is fp32 with one rounding to the tensor type at
 // the end.
 struct RopeArgs {
@@ -121,13 +122,15 @@ struct RopeArgs {
 
 constexpr int kRopeWarps = 8;
 
-// (cos, sin) of pair i at position p.
+// (cos, sin) of pair i at position p, exact to fp32 for |p| <= 2^53 (larger ones round to a double themselves) and
+// |inv_freq| <= 1.
 __device__ __forceinline__ float2 rope_angle(int64_t p, float inv_freq) {
-  const double ang = (double)p * (double)inv_freq;
-  // 2 pi as the sum of two doubles (Cody and Waite's reduction): the remainder keeps its digits for any angle below 2^53 turns
+  const double pd = (double)p, f = (double)inv_freq, ang = pd * f, rest = fma(pd, f, -ang);
+  // 2 pi as the sum of two doubles (Cody and Waite's reduction): ang - n hi is a double's few last bits for the n
+  // next to ang / hi, n lo is below 0.4, and what lo leaves off of 2 pi (below 2^-106) times n stays below 2^-54
   const double hi = 6.283185307179586, lo = 2.4492935982947064e-16;
   const double n = rint(ang * (1.0 / hi));
-  const double r = fma(-n, lo, fma(-n, hi, ang));
+  const double r = fma(-n, lo, fma(-n, hi, ang)) + rest;
   float sn, cs;
   sincospif((float)(r * (2.0 / hi)), &sn, &cs);  // of r = pi x: no reduction left to do
   return make_float2(cs, sn);

@@ -363,8 +363,8 @@ int cq_silu_mul(const void *gu, void *y, int64_t rows, int32_t ffn, int dtype, v
  * 8, <= 256).  Per q and k head x: x * rsqrt(mean(x^2) + eps) * w (q_norm_w /
  * k_norm_w [head_dim]; both NULL: no norm), then the first rot_dim channels
  * are rotated by the angles pos[b*pos_sb + s*pos_ss] * inv_freq[i], i <
- * rot_dim/2 (fp64 product; inv_freq fp32, pos int64): pairs (i, i +
- * rot_dim/2), or (2i, 2i + 1) with adjacent != 0.  fp32 arithmetic, one
+ * rot_dim/2 (inv_freq fp32, pos int64; the angle exact to fp32 for |pos| <=
+ * 2^53 and |inv_freq| <= 1): pairs (i, i + rot_dim/2), or (2i, 2i + 1) with adjacent != 0.  fp32 arithmetic, one
  * rounding at the end.  q_out [batch][n_q_heads][tokens][head_dim], k_out
  * [batch][n_kv_heads][tokens][head_dim], contiguous.  dtype CQ_F16, CQ_BF16 or
  * CQ_F32 for qkv, weights and outputs. */

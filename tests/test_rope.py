@@ -6,6 +6,7 @@ two products, the angle's reduction (pi * 2^-24), sine and cosine (2 steps) and
 the rotation, in all at most (D/2 + 20) * 2^-24 of |a| + |b| of the pair."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -172,3 +173,32 @@ def test_c_nothing_to_do():
 def test_c_too_many_heads():
     for over in (dict(Hq=2 ** 31 - 1), dict(Hkv=2 ** 30)):
         assert _lib.lib().cq_qk_norm_rope_rows(*{**ARGS, **over}.values(), None) == -2
+
+
+PI = Fraction(314159265358979323846264338327950288419716939937510582097494459230781640628620899, 10 ** 80)
+
+
+@gpu
+@pytest.mark.parametrize("pairs", ["halves", "adjacent"])
+@pytest.mark.parametrize("D", [128, 72])
+def test_angles_of_positions_up_to_2_to_53(pairs, D):
+    """Positions whose product with a frequency has more bits than a double:
+    the angles are exact fractions here, reduced by 80 digits of pi."""
+    pos = [2 ** 30 + 7, 2 ** 40 + 12345, -(2 ** 45) - 3, 2 ** 50 - 77, 2 ** 53 - 1, -(2 ** 53)]
+    qkv = inputs(1, len(pos), 4, 2, D, torch.float32)[0]
+    f = freqs(D)
+    turns = [[Fraction(p) * Fraction(x) / (2 * PI) for x in f.tolist()] for p in pos]
+    ang = torch.tensor([[float((t - round(t)) * 2 * PI) for t in row] for row in turns], device="cuda",
+                       dtype=torch.float64)
+    cos, sin = ang.cos()[None, :, None], ang.sin()[None, :, None]
+    ref, mag = [], []
+    for a, b in ((0, 4), (4, 6)):
+        x = qkv.double()[..., a * D:b * D].reshape(1, len(pos), b - a, D)
+        lo, hi = ((slice(0, D // 2), slice(D // 2, D)) if pairs == "halves" else (slice(0, D, 2), slice(1, D, 2)))
+        y, m = torch.empty_like(x), torch.empty_like(x)
+        y[..., lo] = x[..., lo] * cos - x[..., hi] * sin
+        y[..., hi] = x[..., hi] * cos + x[..., lo] * sin
+        m[..., lo] = m[..., hi] = x[..., lo].abs() + x[..., hi].abs()
+        ref.append(y.transpose(1, 2))
+        mag.append(m.transpose(1, 2))
+    check(qk_norm_rope(qkv, 4, 2, f, torch.tensor(pos, device="cuda"), pairs=pairs), ref, mag, D)
