@@ -2,8 +2,9 @@
 // operators in C++: argument checks, output allocation, stream lookup and the
 // call of the C library in one step.  A decode step's kernels run for 3 to 10 us;
 // checked in Python and called through ctypes such a call took 11 to 18 us of
-// host time, from here 5.  The module holds no kernels and keeps nothing
-// between calls; the C functions come from the library that load() is given.
+// host time, from here 5.  Python's lock is given up once the arguments are read
+// (allocations and launches may wait).  The module holds no kernels and keeps
+// nothing between calls; the C functions come from the library that load() is given.
 #include <Python.h>
 
 #include <ATen/ATen.h>
@@ -67,11 +68,28 @@ int32_t int32(PyObject *o, const char *what) {
   if (v < INT32_MIN || v > INT32_MAX) refuse(PyExc_ValueError, std::string(what) + " is out of range");
   return (int32_t)v;
 }
+bool truth(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Refused{nullptr, ""};
+  return v != 0;
+}
 double real(PyObject *o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Refused{nullptr, ""};
   return v;
 }
+// Python's lock given up from here to lock() or the scope's end: no call of Python's API meanwhile.
+struct Unlocked {
+  PyThreadState *state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked &) = delete;
+  ~Unlocked() { lock(); }
+  void lock() {
+    if (state) PyEval_RestoreThread(state);
+    state = nullptr;
+  }
+};
+
 std::string shape_of(const at::Tensor &t) {
   std::string s = "[";
   for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
@@ -134,9 +152,11 @@ Queries queries(const at::Tensor &q, int64_t B, int64_t H, int64_t D, int64_t T,
   return r;
 }
 
-at::Tensor starts_of(PyObject *o, int64_t B, c10::Device device, const char *what) {
-  if (o == Py_None) return {};
-  const at::Tensor &s = tensor(o, "starts");
+const at::Tensor *tensor_or_none(PyObject *o, const char *what) { return o == Py_None ? nullptr : &tensor(o, what); }
+
+at::Tensor starts_of(const at::Tensor *given, int64_t B, c10::Device device, const char *what) {
+  if (!given) return {};
+  const at::Tensor &s = *given;
   if (s.scalar_type() != at::kLong || s.dim() != 1 || s.size(0) != B || s.device() != device)
     refuse(PyExc_ValueError, std::string(what) + ": starts must be int64 [" + std::to_string(B) + "] on " +
                                  device.str() + ", got " + shape_of(s) + " on " + s.device().str());
@@ -190,6 +210,11 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 9, [](PyObject *const *a) {
     const at::Tensor &qkv_in = tensor(a[0], "qkv");
     const int32_t Hq = int32(a[1], "n_q_heads"), Hkv = int32(a[2], "n_kv_heads");
+    const at::Tensor &f_in = tensor(a[3], "inv_freq"), &p_in = tensor(a[4], "positions");
+    const at::Tensor *w_in[2] = {tensor_or_none(a[5], "a norm weight"), tensor_or_none(a[6], "a norm weight")};
+    const float eps = (float)real(a[7]);
+    const int32_t adjacent = truth(a[8]);
+    Unlocked unlocked;
     if (qkv_in.dim() != 3)
       refuse(PyExc_ValueError, "qk_norm_rope: qkv must be [B, S, (Hq + 2 Hkv) * D], got " + shape_of(qkv_in));
     const int64_t B = qkv_in.size(0), S = qkv_in.size(1), width = qkv_in.size(2);
@@ -206,22 +231,20 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (st != at::kHalf && st != at::kBFloat16 && st != at::kFloat)
       refuse(PyExc_TypeError, "qk_norm_rope: expected float16, bfloat16 or float32");
     const int dt = st == at::kHalf ? CQ_F16 : st == at::kBFloat16 ? CQ_BF16 : CQ_F32;
-    const at::Tensor &f_in = tensor(a[3], "inv_freq");
     if (f_in.scalar_type() != at::kFloat || f_in.dim() != 1 || f_in.device() != dev)
       refuse(PyExc_ValueError, "qk_norm_rope: inv_freq must be fp32 [rot / 2] on " + dev.str());
     const int64_t half = f_in.size(0);
     if (2 * half > D)
       refuse(PyExc_ValueError, "qk_norm_rope: " + std::to_string(half) + " frequencies rotate more than " +
                                    std::to_string(D) + " channels");
-    const at::Tensor &p_in = tensor(a[4], "positions");
     if (p_in.scalar_type() != at::kLong || p_in.device() != dev)
       refuse(PyExc_ValueError, "qk_norm_rope: positions must be int64 on " + dev.str());
-    if ((a[5] == Py_None) != (a[6] == Py_None))
+    if (!w_in[0] != !w_in[1])
       refuse(PyExc_ValueError, "qk_norm_rope: give both norm weights or neither");
     at::Tensor w[2];
-    if (a[5] != Py_None)
+    if (w_in[0])
       for (int i = 0; i < 2; ++i) {
-        const at::Tensor &x = tensor(a[5 + i], "a norm weight");
+        const at::Tensor &x = *w_in[i];
         if (x.dim() != 1 || x.size(0) != D || x.scalar_type() != st || x.device() != dev)
           refuse(PyExc_ValueError, "qk_norm_rope: norm weights must be of qkv's type, [" + std::to_string(D) + "], on " +
                                        dev.str());
@@ -233,11 +256,12 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
     at::Tensor q = empty({B, Hq, S, D}, st, dev), k = empty({B, Hkv, S, D}, st, dev);
     const Launch at_(qkv);
     check(L.rope(qkv.const_data_ptr(), qkv.stride(0), qkv.stride(1), (int32_t)B, (int32_t)S, Hq, Hkv, (int32_t)D,
-                 (int32_t)(2 * half), PyObject_IsTrue(a[8]) ? 1 : 0, w[0].defined() ? w[0].const_data_ptr() : nullptr,
+                 (int32_t)(2 * half), adjacent, w[0].defined() ? w[0].const_data_ptr() : nullptr,
                  w[1].defined() ? w[1].const_data_ptr() : nullptr, f.const_data_ptr<float>(),
-                 pos.const_data_ptr<int64_t>(), pos.stride(0), pos.stride(1), (float)real(a[7]), q.mutable_data_ptr(),
+                 pos.const_data_ptr<int64_t>(), pos.stride(0), pos.stride(1), eps, q.mutable_data_ptr(),
                  k.mutable_data_ptr(), dt, at_.stream),
           "qk_norm_rope");
+    unlocked.lock();
     return pair(std::move(q), std::move(k));
   });
 }
@@ -263,18 +287,24 @@ struct Index {
 PyObject *block_bounds(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 6, [](PyObject *const *a) {
     const Index ix(a[4], a[5]);
+    const cq_paged_cache cache = *(const cq_paged_cache *)integer(a[0]);
+    const int64_t t0 = integer(a[1]), T = integer(a[2]);
+    const int32_t bt = int32(a[3], "block_tokens");
+    Unlocked unlocked;
     const Launch at_(ix.codes);
-    check(L.bounds((const cq_paged_cache *)integer(a[0]), integer(a[1]), integer(a[2]), int32(a[3], "block_tokens"),
-                   (int8_t *)ix.codes.mutable_data_ptr(), ix.scales.mutable_data_ptr<float>(), ix.cap, at_.stream),
+    check(L.bounds(&cache, t0, T, bt, (int8_t *)ix.codes.mutable_data_ptr(), ix.scales.mutable_data_ptr<float>(),
+                   ix.cap, at_.stream),
           "BlockIndex.update");
-    return PyLong_FromUnsignedLongLong(capture_id(at_.stream));
+    const unsigned long long id = capture_id(at_.stream);
+    unlocked.lock();
+    return PyLong_FromUnsignedLongLong(id);
   });
 }
 
 // capture_of(codes) -> the id of the capture that records the stream of the index's device, 0 where it runs
 PyObject *capture_of(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 1, [](PyObject *const *a) {
-    const Launch at_(tensor(a[0], "codes"));
+    const Launch at_(tensor(a[0], "codes"));  // nothing here waits
     return PyLong_FromUnsignedLongLong(capture_id(at_.stream));
   });
 }
@@ -284,11 +314,13 @@ PyObject *block_bounds_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 4, [](PyObject *const *a) {
     const Index ix(a[0], a[1]);
     const int64_t first = integer(a[2]), m = integer(a[3]);
+    Unlocked unlocked;
     at::Tensor out = empty({ix.B, ix.H, m, 2, ix.D}, at::kFloat, ix.codes.device());
     const Launch at_(ix.codes);
     check(L.bounds_read((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.B * ix.H,
                         ix.cap, first, m, (int32_t)ix.D, out.mutable_data_ptr<float>(), at_.stream),
           "BlockIndex.bounds");
+    unlocked.lock();
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -300,14 +332,16 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const int32_t bt = int32(a[2], "block_tokens"), top = int32(a[5], "top"), first = int32(a[6], "first"),
                   recent = int32(a[7], "recent");
     const int64_t T = integer(a[3]);
+    const at::Tensor &q_in = tensor(a[4], "queries"), *starts_in = tensor_or_none(a[8], "starts");
+    const bool want = truth(a[9]);
+    Unlocked unlocked;
     if (top < 1 || top > 4096 || first < 0 || recent < 0 || (int64_t)first + recent > top)
       refuse(PyExc_ValueError, "select: need 1 <= top <= 4096 and first + recent <= top, got top=" +
                                    std::to_string(top) + ", first=" + std::to_string(first) +
                                    ", recent=" + std::to_string(recent));
     const auto dev = ix.codes.device();
-    const Queries q = queries(tensor(a[4], "queries"), ix.B, ix.H, ix.D, T, dev, "select");
-    const at::Tensor starts = starts_of(a[8], ix.B, dev, "select");
-    const bool want = PyObject_IsTrue(a[9]) == 1;
+    const Queries q = queries(q_in, ix.B, ix.H, ix.D, T, dev, "select");
+    const at::Tensor starts = starts_of(starts_in, ix.B, dev, "select");
     const Launch at_(ix.codes);
     size_t need = 0;
     check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, q.S, T, bt, &need), "select");
@@ -320,6 +354,7 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
                    want ? scores.mutable_data_ptr<float>() : nullptr, need ? ws.mutable_data_ptr() : nullptr, need,
                    at_.stream),
           "select");
+    unlocked.lock();
     return want ? pair(std::move(blocks), std::move(scores)) : THPVariable_Wrap(std::move(blocks));
   });
 }
@@ -329,37 +364,40 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *sparse_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 9, [](PyObject *const *a) {
     const char *what = "chronoquant_sparse_sdpa";
-    const auto *d = (const cq_paged_cache *)integer(a[0]);
-    const at::Tensor &pool = tensor(a[1], "the page pool");
+    const cq_paged_cache cache = *(const cq_paged_cache *)integer(a[0]);
+    const at::Tensor &pool = tensor(a[1], "the page pool"), &q_in = tensor(a[3], "queries"),
+                     &b_in = tensor(a[5], "blocks"), *starts_in = tensor_or_none(a[7], "starts");
+    const int64_t T = integer(a[2]), bt = integer(a[6]), B = cache.batch, H = cache.kv_heads, D = cache.head_dim;
+    const float scale = (float)real(a[4]);
+    const bool want = truth(a[8]);
+    Unlocked unlocked;
     const auto dev = pool.device();
-    const int64_t T = integer(a[2]), B = d->batch, H = d->kv_heads, D = d->head_dim;
-    const Queries q = queries(tensor(a[3], "queries"), B, H, D, T, dev, what);
-    const at::Tensor &b_in = tensor(a[5], "blocks");
+    const Queries q = queries(q_in, B, H, D, T, dev, what);
     if (b_in.dim() != 4 || b_in.size(0) != B || b_in.size(1) != H || b_in.size(2) != q.S ||
         b_in.scalar_type() != at::kInt)
       refuse(PyExc_ValueError, std::string(what) + ": blocks must be int32 [" + std::to_string(B) + ", " +
                                    std::to_string(H) + ", " + std::to_string(q.S) + ", n], got " + shape_of(b_in));
     if (b_in.device() != dev)
       refuse(PyExc_ValueError, std::string(what) + ": blocks on " + b_in.device().str() + ", the cache on " + dev.str());
-    const int64_t top = b_in.size(3), bt = integer(a[6]);
+    const int64_t top = b_in.size(3);
     if (top < 1 || top > 4096)
       refuse(PyExc_ValueError, std::string(what) + ": lists of 1 to 4096 blocks, got " + std::to_string(top));
     if (bt < 16 || bt % 16 || bt > (1 << 30))
       refuse(PyExc_ValueError, "block_tokens must be a positive multiple of 16, got " + std::to_string(bt));
-    const at::Tensor starts = starts_of(a[7], B, dev, what), blocks = b_in.contiguous();
-    const bool want = PyObject_IsTrue(a[8]) == 1;
+    const at::Tensor starts = starts_of(starts_in, B, dev, what), blocks = b_in.contiguous();
     at::Tensor out, lse, ws;
     out = empty({B, q.Hq, q.S, D}, want ? at::kFloat : q.t.scalar_type(), dev);
     if (want) lse = empty({B, q.Hq, q.S}, at::kFloat, dev);
     const Launch at_(pool);
     size_t need = 0;
-    check(L.sparse_ws(d, T, q.Hq, q.S, (int32_t)top, (int32_t)bt, &need), what);
+    check(L.sparse_ws(&cache, T, q.Hq, q.S, (int32_t)top, (int32_t)bt, &need), what);
     if (need) ws = empty({(int64_t)need}, at::kByte, dev);
-    check(L.sparse(d, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S, q.sb, q.sh, q.sq, (float)real(a[4]),
+    check(L.sparse(&cache, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S, q.sb, q.sh, q.sq, scale,
                    starts_ptr(starts), blocks.const_data_ptr<int32_t>(), (int32_t)top, (int32_t)bt,
                    out.mutable_data_ptr(), want ? CQ_F32 : q.dtype, want ? lse.mutable_data_ptr<float>() : nullptr,
                    need ? ws.mutable_data_ptr() : nullptr, need, at_.stream),
           what);
+    unlocked.lock();
     return want ? pair(std::move(out), std::move(lse)) : THPVariable_Wrap(std::move(out));
   });
 }

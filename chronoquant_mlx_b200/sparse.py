@@ -116,8 +116,8 @@ class BlockIndex:
         if not 0 <= t0 <= T:
             raise ValueError(f"BlockIndex: start {t0} outside [0, {T}]")
         t0 = min(t0, self.covered)
-        capture = _lib.calls().block_bounds(ctypes.addressof(st.descriptor()), t0, T, self.block_tokens, self.codes,
-                                            self.scales)
+        d = st.descriptor()  # held here while its address is in use
+        capture = _lib.calls().block_bounds(ctypes.addressof(d), t0, T, self.block_tokens, self.codes, self.scales)
         if capture:
             self._recorded = (capture, T)
         else:
@@ -163,5 +163,6 @@ def chronoquant_sparse_sdpa(queries: torch.Tensor, cache, scale: float, blocks: 
     st, T = cache.store, cache.offset
     if st is None or T == 0:
         raise ValueError("chronoquant_sparse_sdpa: the cache is empty")
-    return _lib.calls().sparse_attention(ctypes.addressof(st.descriptor()), st.buf, T, queries, scale, blocks,
-                                         block_tokens, starts, return_lse)
+    d = st.descriptor()  # held here while its address is in use
+    return _lib.calls().sparse_attention(ctypes.addressof(d), st.buf, T, queries, scale, blocks, block_tokens, starts,
+                                         return_lse)

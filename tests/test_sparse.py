@@ -12,11 +12,14 @@ of the output type; the log-sum-exp within 2^-10."""
 
 import ctypes
 import math
+import threading
+import time
 
 import pytest
 import torch
 
-from chronoquant_mlx_b200 import BlockIndex, ChronoQuantCache, _lib, chronoquant_sdpa, chronoquant_sparse_sdpa
+from chronoquant_mlx_b200 import (BlockIndex, ChronoQuantCache, _lib, chronoquant_sdpa, chronoquant_sparse_sdpa,
+                                  qk_norm_rope)
 
 gpu = pytest.mark.gpu
 
@@ -908,3 +911,39 @@ def test_an_index_without_memory_to_grow_is_left_as_it_was(monkeypatch):
                 index.bounds()
         assert torch.equal(index.select(q, 3), BlockIndex(other, 32).select(q, 3))
         assert torch.equal(index.bounds(), BlockIndex(other, 32).update().bounds())
+
+
+@gpu
+def test_other_threads_run_while_a_call_waits():
+    """A call that waits for room in the launch queue holds no other Python
+    thread up: this one keeps waking every millisecond or so meanwhile."""
+    cache = make_cache(1, 1, 500, 128)
+    index = BlockIndex(cache, 32).update()
+    q = queries(1, 4, 1, 128, torch.float16)
+    qkv, f = torch.zeros((1, 1, 384), device="cuda"), torch.ones(64, device="cuda")
+    pos = torch.zeros(1, dtype=torch.int64, device="cuda")
+    blocks = index.select(q, 3)
+    calls = {"update": lambda: index.update(499), "bounds": index.bounds, "select": lambda: index.select(q, 3),
+             "attention": lambda: chronoquant_sparse_sdpa(q, cache, 0.1, blocks, 32),
+             "rotation": lambda: qk_norm_rope(qkv, 1, 1, f, pos)}
+    for name, call in calls.items():
+        call()
+        torch.cuda.synchronize()
+        done = threading.Event()
+
+        def work():
+            for _ in range(3000):  # the queue holds about a thousand launches
+                call()
+            done.set()
+
+        torch.cuda._sleep(800_000_000)  # cycles: 0.4 s
+        thread = threading.Thread(target=work)
+        worst, last = 0.0, time.perf_counter()
+        thread.start()
+        while not done.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            worst, last = max(worst, now - last), now
+        thread.join()
+        torch.cuda.synchronize()
+        assert worst < 0.15, (name, worst)
