@@ -107,7 +107,6 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False, checks: boo
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         calls = ex.submit(build_calls, force)
         objs = list(ex.map(compile_one, srcs))
-    calls.result()
     newest_obj = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(out) or os.path.getmtime(out) < newest_obj:
         tmp = out + ".tmp"
@@ -116,6 +115,7 @@ def build(force: bool = False, jobs: int = 8, verbose: bool = False, checks: boo
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
         os.replace(tmp, out)
+    calls.result()  # reported once the library stands: a binding of the C ABI needs no extension
     return out
 
 
