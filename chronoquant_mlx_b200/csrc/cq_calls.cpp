@@ -15,6 +15,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <exception>
 #include <stdexcept>
 #include <string>
@@ -325,6 +326,11 @@ PyObject *block_bounds_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
   });
 }
 
+// Scores of a selection held at once.  A chunk of queries with more of them (4 bytes a query token, kv-head and
+// block: 8192 queries over a million tokens would ask for 4.3 GB) is listed by parts.  1 GB, because parts cost a
+// little: 2048 queries x 16384 blocks x 8 units take 1914 us at once, 2205 us in four parts of 256 MB.
+constexpr size_t kScoreBytes = (size_t)1 << 30;
+
 // block_select(codes, scales, block_tokens, T, queries, top, first, recent, starts, want_scores)
 PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
   return guarded(args, n, 10, [](PyObject *const *a) {
@@ -343,17 +349,38 @@ PyObject *block_select(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const Queries q = queries(q_in, ix.B, ix.H, ix.D, T, dev, "select");
     const at::Tensor starts = starts_of(starts_in, ix.B, dev, "select");
     const Launch at_(ix.codes);
-    size_t need = 0;
-    check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, q.S, T, bt, &need), "select");
     at::Tensor blocks = empty({ix.B, ix.H, q.S, top}, at::kInt, dev), scores, ws;
     if (want) scores = empty({ix.B, ix.H, q.S, top}, at::kFloat, dev);
-    if (need) ws = empty({(int64_t)need}, at::kByte, dev);
-    check(L.select((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.cap, bt,
-                   (int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, T, nullptr, q.t.const_data_ptr(), q.dtype, q.Hq, q.S,
-                   q.sb, q.sh, q.sq, starts_ptr(starts), first, recent, top, blocks.mutable_data_ptr<int32_t>(),
-                   want ? scores.mutable_data_ptr<float>() : nullptr, need ? ws.mutable_data_ptr() : nullptr, need,
-                   at_.stream),
-          "select");
+    // n query tokens from token i on, of a sequence that ends with the last of them
+    const auto list = [&](int32_t i, int32_t n, at::Tensor &to, at::Tensor &to_scores) {
+      const int64_t T_n = T - (q.S - i - n);
+      size_t need = 0;
+      check(L.select_ws((int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, q.Hq, n, T_n, bt, &need), "select");
+      if (need > kScoreBytes && n > 1) return need;
+      if (need && (!ws.defined() || (size_t)ws.numel() < need)) ws = empty({(int64_t)need}, at::kByte, dev);
+      check(L.select((const int8_t *)ix.codes.const_data_ptr(), ix.scales.const_data_ptr<float>(), ix.cap, bt,
+                     (int32_t)ix.B, (int32_t)ix.H, (int32_t)ix.D, T_n, nullptr,
+                     (const char *)q.t.const_data_ptr() + 2 * (int64_t)i * q.sq, q.dtype, q.Hq, n, q.sb, q.sh, q.sq,
+                     starts_ptr(starts), first, recent, top, to.mutable_data_ptr<int32_t>(),
+                     want ? to_scores.mutable_data_ptr<float>() : nullptr, need ? ws.mutable_data_ptr() : nullptr, need,
+                     at_.stream),
+            "select");
+      return (size_t)0;
+    };
+    if (const size_t need = list(0, q.S, blocks, scores)) {
+      const size_t token = need / q.S;  // bytes of a query token's scores
+      const int32_t fit = (int32_t)std::max<size_t>(1, kScoreBytes / token), parts = (q.S - 1) / fit + 1;
+      const int32_t most = (q.S - 1) / parts + 1;  // even parts: at most `fit` tokens
+      ws = empty({(int64_t)(token * most)}, at::kByte, dev);
+      for (int32_t i = 0, n; i < q.S; i += n) {
+        n = std::min(most, q.S - i);
+        at::Tensor part = empty({ix.B, ix.H, n, top}, at::kInt, dev), part_scores;
+        if (want) part_scores = empty({ix.B, ix.H, n, top}, at::kFloat, dev);
+        list(i, n, part, part_scores);
+        blocks.narrow(2, i, n).copy_(part);
+        if (want) scores.narrow(2, i, n).copy_(part_scores);
+      }
+    }
     unlocked.lock();
     return want ? pair(std::move(blocks), std::move(scores)) : THPVariable_Wrap(std::move(blocks));
   });

@@ -143,7 +143,8 @@ class BlockIndex:
         blocks a token may see are always listed, the others by score (ties to
         the lower index).  ``starts``: int64 [B], first real token of each
         sequence.  ``return_scores``: also the listed blocks' scores (fp32, -inf
-        behind), by which lists of ranks that share a sequence can be merged."""
+        behind), by which lists of ranks that share a sequence can be merged.
+        Scratch: up to 1 GB of scores at a time, longer chunks go by parts."""
         T = self.cache.offset
         if T == 0 or self.cache.store is not self._store or self.covered != T and self._tokens() != T:
             self.update()

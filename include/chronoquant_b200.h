@@ -411,7 +411,9 @@ int cq_block_bounds_read(const int8_t *codes, const float *scales, int64_t units
  * in cq_attention.  T: tokens summarised; with len_dev (may be NULL) the
  * length is read from device memory and T is the largest it may be.
  * workspace: cq_block_select_workspace bytes (0 for a decode step's few rows,
- * else 4 per query token, kv-head and block), 16-byte aligned, contents ignored. */
+ * else 4 per query token, kv-head and block), 16-byte aligned, contents ignored.
+ * With less memory a chunk is listed by parts: query tokens i .. i + n - 1 alone
+ * as n queries of T - (q_len - i - n) tokens get the same lists. */
 int cq_block_select_workspace(int32_t batch, int32_t kv_heads, int32_t head_dim, int32_t n_q_heads, int32_t q_len,
                               int64_t T, int32_t block_tokens, size_t *bytes);
 int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks, int32_t block_tokens, int32_t batch,

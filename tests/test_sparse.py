@@ -947,3 +947,61 @@ def test_other_threads_run_while_a_call_waits():
         thread.join()
         torch.cuda.synchronize()
         assert worst < 0.15, (name, worst)
+
+
+@gpu
+@pytest.mark.parametrize("padded", [False, True])
+def test_select_of_very_many_scores_bounds_its_memory(padded):
+    """A chunk of queries over many blocks (a third more scores than 1 GB
+    holds): listed by parts of the chunk, as one call lists them."""
+    B, H, G, S, D, bt, top, first, recent = 2, 4, 2, 3000, 64, 16, 12, 1, 2
+    T = 240000 - 3
+    n = -(-T // bt)
+    cache = make_cache(B, H, T, D, seed=9)
+    index = BlockIndex(cache, bt).update()
+    q = queries(B, H * G, S, D, torch.bfloat16)
+    starts = torch.tensor([3, T - S + 700], device="cuda") if padded else None
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got, s = index.select(q, top, first=first, recent=recent, starts=starts, return_scores=True)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < 1100 << 20
+    codes, scales = index.codes[:, :, :n].double(), index.scales[:, :, :n]
+    j = torch.arange(n, device="cuda")
+    lb = (T - S + torch.arange(S, device="cuda"))[:, None] // bt
+    for b in range(B):
+        st = 0 if starts is None else int(starts[b])
+        fb = st // bt
+        x = q[b].float().view(H, G, S, D)
+        amax = x.abs().amax(-1, keepdim=True)
+        q8 = torch.round(x * (torch.full_like(amax, 127.0) / amax)).double()
+        sg = amax / torch.full_like(amax, 127.0)
+        for h in range(H):
+            dot = (q8[h].clamp(min=0) @ codes[b, h, :, 1].T + q8[h].clamp(max=0) @ codes[b, h, :, 0].T).float()
+            score = ((sg[h] * scales[b, h]) * dot).amax(0)
+            seen = (j >= fb) & (j <= lb) & (torch.arange(S, device="cuda")[:, None] + T - S >= st)
+            rank = torch.where((j < fb + first) | (j > lb - recent), math.inf, score)
+            rank = torch.where(seen, rank, -math.inf)
+            order = torch.sort(rank, dim=-1, descending=True, stable=True).indices[:, :top]
+            want = torch.where(seen.gather(-1, order), order, n).sort(-1).values
+            want_s = torch.where(want < n, score.gather(-1, want.clamp(max=n - 1)), -math.inf)
+            assert torch.equal(got[b, h], torch.where(want < n, want, -1).int())
+            assert torch.equal(s[b, h], want_s)
+
+
+@gpu
+def test_select_by_parts_lists_what_each_token_alone_does():
+    """Four parts of a chunk against calls of one query token each, whose
+    scores do not depend on the split."""
+    B, H, D, bt, top = 4, 8, 8, 16, 20
+    T = 600_000  # 37500 blocks: 4.8 MB of scores a query token
+    codes = torch.randint(-127, 128, (B, H, T // bt, 2, D), dtype=torch.int8, device="cuda",
+                          generator=torch.Generator(device="cuda").manual_seed(4))
+    scales = torch.rand((B, H, T // bt), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    q = queries(B, H, 700, D, torch.float16)  # 3.4 GB in one piece
+    got, s = _lib.calls().block_select(codes, scales, bt, T, q, top, 1, 2, None, True)
+    for i in (0, 1, 174, 175, 176, 349, 350, 524, 525, 699):  # the parts' ends, each token alone
+        t = T - 700 + i + 1
+        one, one_s = _lib.calls().block_select(codes, scales, bt, t, q[:, :, i:i + 1], top, 1, 2, None, True)
+        assert torch.equal(got[:, :, i], one[:, :, 0]) and torch.equal(s[:, :, i], one_s[:, :, 0])
