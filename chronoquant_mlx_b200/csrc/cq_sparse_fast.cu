@@ -12,6 +12,15 @@
 // cluster through distributed shared memory: one launch, no workspace, and the
 // order of every sum is fixed.
 //
+// Scores, maxima, sums and outputs are held in fp32.  Fewer bits where the tensor
+// cores take fp16 operands, as in the decode kernel: q * scale (exact for queries
+// of either type within fp16's normal range); P, up to 2^8 while the maximum lags
+// (2^-11 relative); P times the token's V scale (2^-11 more, finite for scales
+// below 256); P summed per V anchor in fp32 and rounded as the operand that weights
+// the anchors; earlier P of a chunk times the correction when the maximum moves.
+// With sum p = 1 an output stays within 5 * 2^-11 max|v| of the exact one; fp32
+// operands (tf32 products) would halve the products' rate and double the buffers.
+//
 // Bound by latency where units are few (one query over 32 blocks of 64: 7.8 us)
 // and by instructions where they are many: 4096 units of 32 chunks take 217 us,
 // 1025 instructions a chunk of which half run on the half-rate integer pipe, at

@@ -28,7 +28,8 @@ def qk_norm_rope(qkv: torch.Tensor, n_q_heads: int, n_kv_heads: int, inv_freq: t
     int64, broadcastable to [B, S]; inv_freq fp32 -- as pairs (i, i + half)
     (``pairs="halves"``) or (2i, 2i + 1) (``"adjacent"``).  fp32 arithmetic,
     one rounding to qkv's dtype (float16, bfloat16 or float32); angles keep
-    their phase for positions up to 2^53."""
+    their phase for positions up to 2^53.  No gradients, as everywhere in this
+    package: the results are detached whatever qkv and the weights require."""
     if pairs not in ("halves", "adjacent"):
         raise ValueError(f"qk_norm_rope: pairs must be 'halves' or 'adjacent', got {pairs!r}")
     return _lib.calls().qk_norm_rope(qkv, n_q_heads, n_kv_heads, inv_freq, positions, q_weight, k_weight, eps,

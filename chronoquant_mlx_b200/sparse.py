@@ -160,7 +160,14 @@ def chronoquant_sparse_sdpa(queries: torch.Tensor, cache, scale: float, blocks: 
     n], ascending as ``BlockIndex.select`` lists them (an entry that is negative
     or not above its predecessor is left out).  Returns [B, Hq, Tq, D] in the
     query dtype; with ``return_lse`` an fp32 output and the fp32 log-sum-exp [B,
-    Hq, Tq] (-inf for a row that sees no token), for merging."""
+    Hq, Tq] (-inf for a row that sees no token), for merging.
+
+    The layouts of the decode kernel hold queries * scale and the weights times a
+    token's value scale in fp16, as it does: ``|queries * scale|`` has to stay
+    below 65520 and keeps fp16's digits below 2^-14, and value scales have to stay
+    below 256 (residuals of 1792 in 4-bit codes), or a head comes out infinite or
+    NaN.  Other layouts keep the query dtype's range.  No gradients: the cache is a store of encoded tokens, and
+    the result is detached whatever the queries require."""
     st, T = cache.store, cache.offset
     if st is None or T == 0:
         raise ValueError("chronoquant_sparse_sdpa: the cache is empty")

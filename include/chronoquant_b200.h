@@ -434,7 +434,8 @@ int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks
  * for the layouts that the sm_100a kernel takes: those of the decode kernel,
  * block_tokens a multiple of cq_decode_chunk_tokens, a GQA group <= 8).  For
  * those layouts q * scale is held in fp16 as in the decode kernel, so it has to
- * stay in fp16's range.  Both workspace functions answer for the current device. */
+ * stay in fp16's range, and so is a weight (up to 2^8) times its token's V scale,
+ * which has to stay below 256.  Both workspace functions answer for the current device. */
 int cq_sparse_attention_workspace(const cq_paged_cache *cache, int64_t T, int32_t n_q_heads, int32_t q_len,
                                   int32_t top, int32_t block_tokens, size_t *bytes);
 int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,
