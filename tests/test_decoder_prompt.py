@@ -10,8 +10,9 @@ import math
 import pytest
 import torch
 
-from chronoquant_mlx_b200 import BlockIndex, chronoquant_sparse_sdpa
+from chronoquant_mlx_b200 import BlockIndex, chronoquant_sparse_sdpa, decoder
 from chronoquant_mlx_b200.decoder import DecoderConfig, Qwen3StyleDecoder
+from test_sparse import check_attention, decoded, ref_bounds, ref_select, ref_sparse
 
 gpu = pytest.mark.gpu
 
@@ -282,3 +283,82 @@ def test_prefill_refuses_ids_outside_the_vocabulary():
         with pytest.raises(TypeError, match="int32 or int64"):
             m.prefill((good > 0).to(dtype))
     assert m.layers[0]["cache"].offset == 0
+
+
+@gpu
+@pytest.mark.parametrize("kw,cfg", [(FT, CFG), (dict(), CFG), (dict(stride_k=12, stride_v=4), CFG),
+                                    (FT, DecoderConfig(layers=2, hidden=512, heads=18, kv_heads=2, head_dim=128,
+                                                       ffn=1024, vocab=1000))])
+def test_sparse_prompt_chunks_against_64_bits(kw, cfg, monkeypatch):
+    """Every chunk of a prompt, layer by layer: dense attention while the lists
+    hold every block, then the lists of the definition over the layer's own cache
+    and 64-bit attention over them, each row's own block among them."""
+    sp = dict(top=5, block_tokens=64, first=1, recent=2)
+    m = Qwen3StyleDecoder(cfg, 2, 700, kw, seed=3, sparse=sp)
+    attend, select_blocks, seen = m._chunk_attention, [], []
+    sparse_sdpa = decoder.chronoquant_sparse_sdpa
+
+    def listed(q, cache, scale, blocks, bt, **rest):
+        select_blocks.append(blocks)
+        return sparse_sdpa(q, cache, scale, blocks, bt, **rest)
+
+    def checked(L, q):
+        before = len(select_blocks)
+        out = attend(L, q)
+        cache = L["cache"]
+        T, S = cache.offset, q.shape[2]
+        if T <= 5 * 64:
+            assert len(select_blocks) == before
+        else:
+            assert len(select_blocks) == before + 1
+            blocks = select_blocks[-1]
+            codes, scales = ref_bounds(decoded(cache, fp16_keys=True)[0], 64)
+            assert torch.equal(blocks.cpu(), ref_select(codes, scales, q, T, 64, 5, 1, 2)[0])
+            own = (T - S + torch.arange(S, device="cuda")) // 64
+            assert (blocks == own[:, None]).any(-1).all()
+            ref, _, vmax = ref_sparse(*decoded(cache), q, 128 ** -0.5, blocks, 64)
+            check_attention(out, ref, vmax)
+        seen.append((T, len(select_blocks) - before))
+        return out
+
+    monkeypatch.setattr(decoder, "chronoquant_sparse_sdpa", listed)
+    monkeypatch.setattr(m, "_chunk_attention", checked)
+    got = m.prefill(prompt(2, 333, seed=5), chunk=111)
+    assert torch.isfinite(got).all()
+    got = m.prefill(prompt(2, 217, seed=6), chunk=120)
+    assert torch.isfinite(got).all()
+    assert seen == [(t, int(t > 320)) for t in (111, 222, 333, 453, 550) for _ in range(2)]
+
+
+@gpu
+@pytest.mark.parametrize("kw", [FT, dict(stride_k=12, stride_v=4)])
+def test_sparse_prompt_over_every_block_is_the_dense_prompt(kw, monkeypatch):
+    """Chunks sent through selection and sparse attention with room for every
+    block: 64-bit attention over the whole cache, layer by layer, each over its own
+    cache.  The first layer's keys and values are the dense decoder's bit for bit;
+    the next layer's are not comparable in the end (a rounding of the first one's
+    output moves codes next to a border by a whole step, a third of the largest
+    residual in 3 bits)."""
+    m = Qwen3StyleDecoder(CFG, 2, 500, kw, seed=3, sparse=dict(top=8, block_tokens=64))
+    ran = []
+
+    def sparse(L, q):
+        cache, index = L["cache"], m._index(L)
+        blocks = index.select(q, 8)
+        S, T = q.shape[2], cache.offset
+        own = (T - S + torch.arange(S, device="cuda")) // 64
+        j = torch.arange(8, device="cuda")
+        assert torch.equal(blocks[1, 1], torch.where(j <= own[:, None], j, -1).int())
+        out = chronoquant_sparse_sdpa(q, cache, 128 ** -0.5, blocks, 64)
+        ref, _, vmax = ref_sparse(*decoded(cache), q, 128 ** -0.5, blocks, 64)
+        check_attention(out, ref, vmax)
+        ran.append(T)
+        return out
+
+    monkeypatch.setattr(m, "_chunk_attention", sparse)
+    ids = prompt(2, 450, seed=5)
+    dense = Qwen3StyleDecoder(CFG, 2, 500, kw, seed=3)
+    assert torch.isfinite(m.prefill(ids, chunk=150)).all() and torch.isfinite(dense.prefill(ids, chunk=150)).all()
+    for x, y in zip(m.layers[0]["cache"].state, dense.layers[0]["cache"].state):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    assert ran == [150, 150, 300, 300, 450, 450]
