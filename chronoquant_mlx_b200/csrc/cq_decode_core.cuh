@@ -422,7 +422,7 @@ __device__ __forceinline__ void v_tile(WarpState &st, const VAddr &A, int tb, ui
     // 64-token chunks have few V anchors (2 for stride 32): P is summed per
     // anchor slot of the chunk (rows of ps) by one MMA with an indicator
     // matrix (row a, token k: 1 when token k belongs to anchor a), and the
-    // anchors are applied once per chunk (see do_chunk) instead of gathered
+    // anchors are applied once per chunk (apply_v_anchors) instead of gathered
     // for every token
     constexpr uint32_t ONE2 = 0x3C003C00u;
     const int gg = lane >> 2, t2 = 2 * (lane & 3);
@@ -522,6 +522,24 @@ __device__ __forceinline__ void v_tile(WarpState &st, const VAddr &A, int tb, ui
     }
     // the offset 72 of every code value: 72 * sum_t P'_t, exactly as the MMAs above weight it
     ptx::mma_f16_16816(st.vb, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, ptx::HALF2_72, bS0, bS1);
+  }
+}
+
+// O += A_v^T PS of a chunk whose P was summed per V anchor (SPLIT geometries), and
+// the chunk's sum of P into the denominator.  row: the anchor row of slot lane & 7
+// (slots out of use have weight 0: any row in use).
+__device__ __forceinline__ void apply_v_anchors(WarpState &st, uint32_t row, int lane) {
+  const uint32_t b0 = ptx::movmatrix_trans(ptx::pack_half2(st.ps[0], st.ps[1]));
+  st.l[0] += st.ps[2];  // row 15 (lanes g == 7): this chunk's sum of P per head
+  st.l[1] += st.ps[3];
+  st.ps[0] = st.ps[1] = st.ps[2] = st.ps[3] = 0.f;
+  const uint32_t base = row + (lane >> 3) * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a0, a1, a2, a3;
+    ptx::ldmatrix_x4_trans(a0, a1, a2, a3, base + i * 64);
+    ptx::mma_f16_16816(st.o[2 * i], a0, a1, 0u, 0u, b0, 0u);
+    ptx::mma_f16_16816(st.o[2 * i + 1], a2, a3, 0u, 0u, b0, 0u);
   }
 }
 

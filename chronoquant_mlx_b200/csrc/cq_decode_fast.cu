@@ -323,20 +323,8 @@ __device__ __forceinline__ bool do_chunk(const Params &p, const Len &L, WarpStat
         if (!MASK || grp * 32 + tile * 16 < nvalid)
           v_tile<G, MASK>(st, A, grp * 32 + tile * 16, bp[grp][tile].x, bp[grp][tile].y, nvalid, lane);
     if (G::SPLIT) {
-      // O += A_v^T PS: the chunk's V anchors (rows = slots; past the valid ones, the last valid one, weight 0)
       const int nA = MASK ? ((nvalid - 1) >> G::LSV) + 1 : G::AV;
-      const uint32_t b0 = ptx::movmatrix_trans(ptx::pack_half2(st.ps[0], st.ps[1]));
-      st.l[0] += st.ps[2];  // row 15 (lanes g == 7): this chunk's sum of P per head
-      st.l[1] += st.ps[3];
-      st.ps[0] = st.ps[1] = st.ps[2] = st.ps[3] = 0.f;
-      const uint32_t base = vbuf + min(lane & 7, nA - 1) * (HD * 2) + (lane >> 3) * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t a0, a1, a2, a3;
-        ptx::ldmatrix_x4_trans(a0, a1, a2, a3, base + i * 64);
-        ptx::mma_f16_16816(st.o[2 * i], a0, a1, 0u, 0u, b0, 0u);
-        ptx::mma_f16_16816(st.o[2 * i + 1], a2, a3, 0u, 0u, b0, 0u);
-      }
+      apply_v_anchors(st, vbuf + min(lane & 7, nA - 1) * (HD * 2), lane);
     }
   }
   // every lane's reads of the V part are done before the refill

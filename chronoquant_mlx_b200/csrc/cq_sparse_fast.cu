@@ -145,20 +145,9 @@ __device__ __forceinline__ bool sparse_chunk(WarpState &st, const QFrag &f, int 
         if (MASK && (tb >= vhi || tb + 16 <= vlo)) continue;
         v_tile<G, MASK>(st, A, tb, bp[grp][tile].x, bp[grp][tile].y, vhi, lane, vlo);
       }
-    if (G::SPLIT) {  // the chunk's V anchors, weighted by P summed per anchor (anchors out of use: one in use, weight 0)
+    if (G::SPLIT) {  // rows of anchors that counted tokens use
       const int a0 = MASK ? vlo >> G::LSV : 0, a1 = MASK ? (vhi - 1) >> G::LSV : G::AV - 1;
-      const uint32_t b0 = ptx::movmatrix_trans(ptx::pack_half2(st.ps[0], st.ps[1]));
-      st.l[0] += st.ps[2];  // row 15 (lanes g == 7): this chunk's sum of P per head
-      st.l[1] += st.ps[3];
-      st.ps[0] = st.ps[1] = st.ps[2] = st.ps[3] = 0.f;
-      const uint32_t base = vb + max(a0, min(lane & 7, a1)) * (HD * 2) + (lane >> 3) * 16;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t x0, x1, x2, x3;
-        ptx::ldmatrix_x4_trans(x0, x1, x2, x3, base + i * 64);
-        ptx::mma_f16_16816(st.o[2 * i], x0, x1, 0u, 0u, b0, 0u);
-        ptx::mma_f16_16816(st.o[2 * i + 1], x2, x3, 0u, 0u, b0, 0u);
-      }
+      apply_v_anchors(st, vb + max(a0, min(lane & 7, a1)) * (HD * 2), lane);
     }
   }
   __syncwarp();
