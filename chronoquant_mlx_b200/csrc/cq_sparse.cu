@@ -1175,12 +1175,15 @@ int read_bounds_error_sparse(int clear) { return read_bounds_error_here(clear); 
 
 using namespace cq;
 
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
 static int bounds_checks(const cq_paged_cache *cache, int64_t T, int32_t bt, const void *codes, const void *scales,
                          int64_t max_blocks, const char *what) {
   int r = validate_cache(cache);
   if (r) return r;
   const std::string w(what);
   CQ_REQUIRE(codes && scales, CQ_ERR_INVALID, w + ": null pointer");
+  CQ_REQUIRE(aligned16(codes), CQ_ERR_INVALID, w + ": codes must be 16-byte aligned");
   CQ_REQUIRE(bt >= 1, CQ_ERR_INVALID, w + ": block_tokens must be >= 1");
   CQ_REQUIRE(T >= 1 && T <= (int64_t)cache->max_pages * cache->page_tokens, CQ_ERR_INVALID,
              w + ": tokens beyond the mapped pages (or none)");
@@ -1188,8 +1191,6 @@ static int bounds_checks(const cq_paged_cache *cache, int64_t T, int32_t bt, con
   CQ_REQUIRE((T - 1) / bt < (1LL << 30), CQ_ERR_UNSUPPORTED, w + ": too many blocks");
   return CQ_OK;
 }
-
-static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 static int launch_bounds(const sparse::BoundsArgs &A, cudaStream_t st, const char *what) {
   const int64_t units = (int64_t)A.cv.B * A.cv.H;
@@ -1237,6 +1238,8 @@ extern "C" int cq_block_bounds_at(const cq_paged_cache *cache, const int64_t *le
 extern "C" int cq_block_bounds_read(const int8_t *codes, const float *scales, int64_t units, int64_t max_blocks,
                                     int64_t first, int64_t n, int32_t head_dim, float *out, void *stream) {
   CQ_REQUIRE(codes && scales && out, CQ_ERR_INVALID, "cq_block_bounds_read: null pointer");
+  CQ_REQUIRE(aligned16(codes) && aligned16(out), CQ_ERR_INVALID,
+             "cq_block_bounds_read: codes and out must be 16-byte aligned");
   CQ_REQUIRE(units >= 1 && first >= 0 && n >= 0 && n <= max_blocks - first && head_dim >= 8 && head_dim <= 256,
              CQ_ERR_INVALID, "cq_block_bounds_read: bad sizes");
   if (n == 0) return CQ_OK;
@@ -1438,6 +1441,7 @@ extern "C" int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const
   const int splits = sparse::pick_list_splits(rows, top), D = cache->head_dim;
   CQ_REQUIRE(workspace && workspace_bytes >= sparse::generic_bytes(rows, splits, D), CQ_ERR_WORKSPACE,
              "cq_sparse_attention: workspace too small");
+  CQ_REQUIRE(((uintptr_t)workspace & 3) == 0, CQ_ERR_INVALID, "cq_sparse_attention: workspace must be 4-byte aligned");
   CQ_REQUIRE(rows * splits < (1LL << 31), CQ_ERR_INVALID, "cq_sparse_attention: grid too large");
   float *o = (float *)workspace, *m = o + rows * splits * D, *l = m + rows * splits;
   sparse::SparseArgs A{make_view(*cache), q,     q_dtype, n_q_heads, q_len, top,    block_tokens, splits, q_sb, q_sh, q_sq,

@@ -389,7 +389,7 @@ int cq_qk_norm_rope_rows(const void *qkv, int64_t seq_stride, int64_t row_stride
  * max_len), for captured graphs.  cq_block_bounds_read: code * scale of blocks
  * first .. first+n-1 of every unit, fp32 [units][n][2][head_dim].
  *
- * codes is 16-byte aligned in all of these. */
+ * codes is 16-byte aligned in all of these, and so is cq_block_bounds_read's out. */
 int cq_block_bounds(const cq_paged_cache *cache, int64_t t0, int64_t T, int32_t block_tokens, int8_t *codes,
                     float *scales, int64_t max_blocks, void *stream);
 int cq_block_bounds_at(const cq_paged_cache *cache, const int64_t *len_dev, int64_t max_len, int32_t S,
@@ -432,10 +432,11 @@ int cq_block_select(const int8_t *codes, const float *scales, int64_t max_blocks
  * cq_block_select; a device-resident length outside [q_len, T] gives zeros and
  * sets cq_device_error (4).  workspace: cq_sparse_attention_workspace bytes (0
  * for the layouts that the sm_100a kernel takes: those of the decode kernel,
- * block_tokens a multiple of cq_decode_chunk_tokens, a GQA group <= 8).  For
- * those layouts q * scale is held in fp16 as in the decode kernel, so it has to
- * stay in fp16's range, and so is a weight (up to 2^8) times its token's V scale,
- * which has to stay below 256.  Both workspace functions answer for the current device. */
+ * block_tokens a multiple of cq_decode_chunk_tokens, a GQA group <= 8), 4-byte
+ * aligned.  For those layouts q * scale is held in fp16 as in the decode kernel,
+ * so it has to stay in fp16's range, and so is a weight (up to 2^8) times its
+ * token's V scale, which has to stay below 256.  Both workspace functions answer
+ * for the current device. */
 int cq_sparse_attention_workspace(const cq_paged_cache *cache, int64_t T, int32_t n_q_heads, int32_t q_len,
                                   int32_t top, int32_t block_tokens, size_t *bytes);
 int cq_sparse_attention(const cq_paged_cache *cache, int64_t T, const int64_t *len_dev, const void *q, int q_dtype,

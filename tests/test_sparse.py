@@ -881,6 +881,7 @@ def test_an_index_does_not_grow_in_a_capture():
     graph = torch.cuda.CUDAGraph()
     with pytest.raises(RuntimeError, match="reserve"):
         with torch.cuda.graph(graph):
+            index.bounds()  # (a graph of something)
             index.update()
     assert index.covered == 250
     assert torch.equal(index.update().bounds(), BlockIndex(cache, 32).update().bounds())
@@ -1005,3 +1006,17 @@ def test_select_by_parts_lists_what_each_token_alone_does():
         t = T - 700 + i + 1
         one, one_s = _lib.calls().block_select(codes, scales, bt, t, q[:, :, i:i + 1], top, 1, 2, None, True)
         assert torch.equal(got[:, :, i], one[:, :, 0]) and torch.equal(s[:, :, i], one_s[:, :, 0])
+
+
+def test_c_alignment_refusals():
+    """Vector accesses to pointers off their alignment would fault on the device: refused on the host."""
+    L, d = _lib.lib(), ctypes.byref(_desc())
+    for off in (1, 4, 8):
+        assert L.cq_block_bounds(d, *{**BOUNDS, "codes": P + off}.values(), None) == -1
+        assert L.cq_block_bounds_at(d, P, 1000, 1, 64, P + off, P, 16, None) == -1
+        assert L.cq_block_bounds_read(P + off, P, 16, 16, 0, 4, 128, P, None) == -1
+        assert L.cq_block_bounds_read(P, P, 16, 16, 0, 4, 128, P + off, None) == -1
+        assert b"aligned" in L.cq_last_error()
+    for off in (1, 2):
+        assert L.cq_sparse_attention(d, *{**SPARSE_ARGS, "ws": P + off}.values(), None) == -1
+        assert b"aligned" in L.cq_last_error()
