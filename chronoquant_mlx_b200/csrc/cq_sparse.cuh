@@ -10,7 +10,8 @@ namespace sparse {
 constexpr int ERR_LENGTH = 4;  // a device-resident length outside [q_len, mapped tokens]
 constexpr int kMaxTop = 4096;  // longest block list
 
-// Records a bad device-resident length for cq_device_error (one word for all sparse kernels).
+// Records a bad device-resident length for cq_device_error (the word of cq_sparse.cu's kernels; cq_sparse_fast.cu has
+// its own).
 __device__ void set_length_error();
 
 // Cached tokens of a launch: T, or the device-resident length (which must lie

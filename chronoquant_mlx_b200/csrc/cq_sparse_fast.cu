@@ -25,8 +25,10 @@
 // and by instructions where they are many: 4096 units of 32 chunks take 217 us,
 // 1025 instructions a chunk of which half run on the half-rate integer pipe, at
 // 58 % issue with the 16 warps an SM that registers and buffers leave room for.
-// Several query tokens per unit, sharing the chunks that more than one of them
-// lists, took 255 to 301 us (neighbouring lists overlap by a third).
+// Each listed chunk is decoded once per query token that lists it (16 times on
+// average over 512 tokens).  Several neighbouring tokens per unit, sharing the
+// chunks that more than one of them lists, took 255 to 301 us (their lists overlap
+// by a third).
 //
 // Requirements (sparse_fast_supported): the decode kernel's layouts, a GQA
 // group of at most 8, block_tokens a multiple of the chunk.
@@ -400,9 +402,9 @@ static const SparseGeo *sparse_layout(const cq_paged_cache &c, int n_q_heads, in
 // plus a fixed part of about 2.5 (lookups, query fragments, the merge); the
 // machine runs 16 warps per SM at a time, and where that takes more than one
 // round the last one is half empty.  The W with the least such time is taken.
-// (4096 units of 32 chunks: 245, 221, 233, 261, 360 us with W = 1, 2, 4, 8, 16;
-// 128 units of 64: 42, 25.5, 25.0, 32 us with 4, 8, 16, 32; 8 units of 64: 17.3,
-// 12.2, 9.3, 7.9 us with 8, 16, 32, 64.)
+// (4096 units of 32 chunks: 240, 217, 228, 256, 356 us with W = 1, 2, 4, 8, 16;
+// 128 units of 64: 42, 25.6, 24.6, 31.9 us with 4, 8, 16, 32; 8 units of 64: 17.1,
+// 12.1, 9.1, 7.8 us with 8, 16, 32, 64.)
 static int pick_warps(int64_t units, int n, int sms) {
   const double slots = (double)sms * 2 * kSW;
   int best = 1;
