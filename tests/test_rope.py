@@ -202,3 +202,21 @@ def test_angles_of_positions_up_to_2_to_53(pairs, D):
         ref.append(y.transpose(1, 2))
         mag.append(m.transpose(1, 2))
     check(qk_norm_rope(qkv, 4, 2, f, torch.tensor(pos, device="cuda"), pairs=pairs), ref, mag, D)
+
+
+@gpu
+@pytest.mark.parametrize("Hkv", [8, 7])
+def test_offsets_past_32_bits(Hkv):
+    """Rows past 2^32 bytes (and 2^31 elements) of a prompt: the last ones come out as they do alone."""
+    S, Hq, D = 400_000, 32, 128
+    width = (Hq + 2 * Hkv) * D
+    qkv = torch.empty((1, S, width), dtype=torch.bfloat16, device="cuda")
+    assert qkv.numel() > 2 ** 31
+    qkv[:, -50:] = inputs(1, 50, Hq, Hkv, D, torch.bfloat16)[0]
+    qkv[:, :-50] = 1
+    _, wq, wk = inputs(1, 1, 1, 1, D, torch.bfloat16)
+    f, pos = freqs(D), torch.arange(S, device="cuda")
+    got = qk_norm_rope(qkv, Hq, Hkv, f, pos, wq, wk)
+    want = qk_norm_rope(qkv[:, -50:], Hq, Hkv, f, pos[-50:], wq, wk)
+    for a, b in zip(got, want):
+        assert torch.equal(a[:, :, -50:], b)

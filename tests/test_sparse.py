@@ -1020,3 +1020,30 @@ def test_c_alignment_refusals():
     for off in (1, 2):
         assert L.cq_sparse_attention(d, *{**SPARSE_ARGS, "ws": P + off}.values(), None) == -1
         assert b"aligned" in L.cq_last_error()
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """A cache of 4.5 GB (four million tokens of 8 heads): its last tokens'
+    ranges, lists and attention are those of a cache that holds them alone."""
+    H, n, chunk, kw = 8, 62, 65536, dict(stride_k=64, stride_v=32, delta_bits_v=3)
+    last = chunk + 333
+    T, t0 = n * chunk + last, n * chunk
+    big, tail = ChronoQuantCache(max_tokens=T, **kw), ChronoQuantCache(**kw)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    k, v = (torch.randn((1, H, last, 128), generator=g, device="cuda").half() for _ in range(2))
+    for i in range(n):
+        big.update_and_fetch(k[:, :, :chunk] + i / 8, v[:, :, :chunk])
+    big.update_and_fetch(k, v)
+    tail.update_and_fetch(k, v)
+    assert big.store.buf.numel() > 2 ** 32 and big.offset == T
+    whole, part = BlockIndex(big, 64).update(), BlockIndex(tail, 64).update()
+    assert torch.equal(whole.bounds(t0 // 64), part.bounds())
+    whole.codes[:, :, t0 // 64:] = 0
+    assert torch.equal(whole.update(t0).bounds(t0 // 64), part.bounds())
+    for S in (1, 40):
+        q = queries(1, 4 * H, S, 128, torch.bfloat16)
+        got = whole.select(q, 12, starts=torch.tensor([t0], device="cuda"))
+        want = part.select(q, 12)
+        assert torch.equal(got, torch.where(want >= 0, want + t0 // 64, -1))
+        assert torch.equal(chronoquant_sparse_sdpa(q, big, 0.1, got, 64), chronoquant_sparse_sdpa(q, tail, 0.1, want, 64))
