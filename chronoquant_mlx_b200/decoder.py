@@ -151,6 +151,10 @@ class Qwen3StyleDecoder:
             sparse = {"block_tokens": 64, "first": 1, "recent": 2, **sparse}
             if sparse["recent"] < 1:
                 raise ValueError("sparse: recent must be at least 1 (a step attends to its own block)")
+            if (sparse["block_tokens"] < 16 or sparse["block_tokens"] % 16 or sparse["first"] < 0
+                    or not sparse["first"] + sparse["recent"] <= sparse["top"] <= 4096):
+                raise ValueError("sparse: block_tokens must be a positive multiple of 16, first >= 0 and first + recent "
+                                 f"<= top <= 4096, got {sparse}")
         self.sparse = sparse
         self.cfg, self.B, self.max_len = cfg, batch, max_len
         self.device, self.dtype = torch.device(device), dtype

@@ -362,3 +362,14 @@ def test_sparse_prompt_over_every_block_is_the_dense_prompt(kw, monkeypatch):
     for x, y in zip(m.layers[0]["cache"].state, dense.layers[0]["cache"].state):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
     assert ran == [150, 150, 300, 300, 450, 450]
+
+
+def test_sparse_options_that_no_step_could_take_are_refused():
+    """At once, not by the first prompt that grows past its lists."""
+    for sparse in (dict(top=2), dict(top=4, first=2, recent=3), dict(top=0), dict(top=-3), dict(top=5000),
+                   dict(top=8, first=-1), dict(top=8, block_tokens=0), dict(top=8, block_tokens=40),
+                   dict(top=8, block_tokens=-16)):
+        with pytest.raises(ValueError):
+            Qwen3StyleDecoder(CFG, 1, 64, sparse=sparse, device="cpu")
+    m = Qwen3StyleDecoder(CFG, 1, 64, sparse=dict(top=3, block_tokens=16), device="cpu")
+    assert m.sparse == dict(top=3, block_tokens=16, first=1, recent=2)
