@@ -412,6 +412,15 @@ class Qwen3StyleDecoder:
                                            wsb, st), "decoder")
         return self.attn_out
 
+    def _check_storage(self) -> None:
+        """Steps hold the addresses of the caches' pages, a captured one those of the indexes too."""
+        moved = any(L["cache"].store is not L["store"] or L["store"].descriptor() is not L["desc"] for L in self.layers)
+        if self.graph is not None and self.sparse is not None:
+            moved = moved or any(L["index"].codes is not L["codes"] for L in self.layers)
+        if moved:
+            raise RuntimeError("a cache's storage moved since the decoder prepared its steps: run a prompt or "
+                               "fill_context, and capture again")
+
     # -- one decode step --------------------------------------------------------
     def _attention(self, L: dict, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Encode this step's k/v [B, Hkv, D] into the layer's cache and attend
@@ -515,12 +524,16 @@ class Qwen3StyleDecoder:
         replace the kernel, e.g. by a reference).  Returns logits [B, vocab].
         No host sync: the length on the device advances, and the caches' host-side
         offsets follow at the next ``prefill`` or ``fill_context``."""
+        if attention is None:
+            self._check_storage()
         return self._step_body(attention)
 
     def capture(self) -> None:
         """Capture one decode step as a CUDA graph (after ``fill_context`` or
         ``prefill``).  The dense step runs in the decode kernel and takes its
         layouts; a sparse one takes every layout and group of the cache."""
+        self.graph = None
+        self._check_storage()
         lib = _lib.lib()
         c = self.cfg
         # one-time set-up outside the capture: cuBLAS handles (one matmul of each
@@ -546,9 +559,13 @@ class Qwen3StyleDecoder:
                                            cq_dtype(self.attn_out), None, self.workspace.data_ptr(),
                                            self.workspace.numel() * 4, stream_ptr(self.device)), "decoder")
         torch.cuda.synchronize(self.device)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self.logits = self._step_body()
+        self.graph = graph
+        if self.sparse is not None:
+            for L in self.layers:
+                L["codes"] = L["index"].codes
         torch.cuda.synchronize(self.device)
 
     def decode(self, steps: int) -> torch.Tensor:
@@ -558,6 +575,7 @@ class Qwen3StyleDecoder:
         start = self.layers[0]["cache"].offset
         if self.graph is None:
             raise RuntimeError("decode replays a captured step: call capture() first")
+        self._check_storage()
         if start + steps > self.max_len:
             raise ValueError(f"decode past max_len {self.max_len}")
         for _ in range(steps):

@@ -373,3 +373,38 @@ def test_sparse_options_that_no_step_could_take_are_refused():
             Qwen3StyleDecoder(CFG, 1, 64, sparse=sparse, device="cpu")
     m = Qwen3StyleDecoder(CFG, 1, 64, sparse=dict(top=3, block_tokens=16), device="cpu")
     assert m.sparse == dict(top=3, block_tokens=16, first=1, recent=2)
+
+
+@gpu
+@pytest.mark.parametrize("sparse", [None, dict(top=4)])
+def test_steps_over_moved_storage_are_refused(sparse):
+    """Steps hold addresses of the caches' pages (a captured one of the indexes
+    too): a restored state, pages that had to grow or an index that moved."""
+    def fresh():
+        m = Qwen3StyleDecoder(CFG, 2, 300, FT, seed=3, sparse=sparse)
+        m.fill_context(100)
+        m.capture()
+        m.decode(1)
+        return m
+
+    m = fresh()
+    other = type(m.layers[1]["cache"])(**FT)
+    other.update_and_fetch(*(torch.randn((2, 2, 40, 128), device="cuda").bfloat16() for _ in range(2)))
+    m.layers[1]["cache"].state = other.state
+    for step in (lambda: m.decode(1), m.step_eager, m.capture):
+        with pytest.raises(RuntimeError, match="moved"):
+            step()
+    m = fresh()
+    m.layers[0]["cache"].update_and_fetch(*(torch.randn((2, 2, 700, 128), device="cuda").bfloat16() for _ in range(2)))
+    for step in (lambda: m.decode(1), m.step_eager, m.capture):
+        with pytest.raises(RuntimeError, match="moved"):
+            step()
+    m = fresh()
+    before = m.layers[1]["cache"].offset
+    if sparse:
+        m.layers[1]["index"].reserve(5000)
+        with pytest.raises(RuntimeError, match="moved"):
+            m.decode(1)
+        assert m.layers[1]["cache"].offset == before
+        m.capture()
+    assert torch.isfinite(m.decode(3)).all()
