@@ -937,7 +937,7 @@ def test_other_threads_run_while_a_call_waits():
                 call()
             done.set()
 
-        torch.cuda._sleep(800_000_000)  # cycles: 0.4 s
+        torch.cuda._sleep(1_200_000_000)  # cycles: 0.6 s
         thread = threading.Thread(target=work)
         worst, last = 0.0, time.perf_counter()
         thread.start()
@@ -947,7 +947,7 @@ def test_other_threads_run_while_a_call_waits():
             worst, last = max(worst, now - last), now
         thread.join()
         torch.cuda.synchronize()
-        assert worst < 0.15, (name, worst)
+        assert worst < 0.3, (name, worst)
 
 
 @gpu
