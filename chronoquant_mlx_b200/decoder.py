@@ -240,7 +240,7 @@ class Qwen3StyleDecoder:
                 a, b = max(t, t_lo) - t, min(t + n, t_hi) - t  # the part of this chunk in the rank's range
                 if a < b:
                     L["cache"].update_and_fetch(k[:, h0:h1, a:b].contiguous(), v[:, h0:h1, a:b].contiguous())
-        self.pos.fill_(T0)
+        self.pos.fill_(T0 if self.seq_group is not None else self.layers[0]["cache"].offset)
         self._prepare_attention()
 
     # -- prompts -----------------------------------------------------------------

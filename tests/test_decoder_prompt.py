@@ -408,3 +408,14 @@ def test_steps_over_moved_storage_are_refused(sparse):
         assert m.layers[1]["cache"].offset == before
         m.capture()
     assert torch.isfinite(m.decode(3)).all()
+
+
+@gpu
+def test_a_context_filled_in_behind_another_goes_on_from_its_position():
+    """The next step's position is the number of tokens cached, however they came there."""
+    m = Qwen3StyleDecoder(CFG, 2, 200, FT, seed=3)
+    m.fill_context(60)
+    assert int(m.pos) == 60
+    m.step_eager()
+    m.fill_context(30)
+    assert int(m.pos) == m.layers[0]["cache"].offset == int(m.layers[0]["len"][0]) == 91
