@@ -326,13 +326,16 @@ class Qwen3StyleDecoder:
         """Bring the caches' host-side offsets up to what eager steps encoded:
         those advance the lengths on the device alone.  (A caller's own attention
         appends through the cache, whose offset is ahead then; a restored cache has
-        another store, which no step has written.)"""
+        another store, which no step has written.)  The layers have to agree."""
         if not self.tail:  # a sequence split's other ranks hold a fixed range
             return
         known = [L for L in self.layers if L.get("store") is not None and L["store"] is L["cache"].store]
         if known:
             for L, n in zip(known, torch.stack([L["len"][0] for L in known]).tolist()):
                 L["cache"].offset = max(L["cache"].offset, n)
+        lengths = {L["cache"].offset for L in self.layers}
+        if len(lengths) > 1:
+            raise RuntimeError(f"the layers' caches hold different lengths: {sorted(lengths)}")
 
     def _prepare_attention(self) -> None:
         """Per-layer descriptors, device-resident lengths and one shared

@@ -166,8 +166,9 @@ def chronoquant_sparse_sdpa(queries: torch.Tensor, cache, scale: float, blocks: 
     token's value scale in fp16, as it does: ``|queries * scale|`` has to stay
     below 65520 and keeps fp16's digits below 2^-14, and value scales have to stay
     below 256 (residuals of 1792 in 4-bit codes), or a head comes out infinite or
-    NaN.  Other layouts keep the query dtype's range.  No gradients: the cache is a store of encoded tokens, and
-    the result is detached whatever the queries require."""
+    NaN.  Other layouts keep the query dtype's range.  No gradients: the cache is a
+    store of encoded tokens, and the result is detached whatever the queries
+    require."""
     st, T = cache.store, cache.offset
     if st is None or T == 0:
         raise ValueError("chronoquant_sparse_sdpa: the cache is empty")

@@ -419,3 +419,19 @@ def test_a_context_filled_in_behind_another_goes_on_from_its_position():
     m.step_eager()
     m.fill_context(30)
     assert int(m.pos) == m.layers[0]["cache"].offset == int(m.layers[0]["len"][0]) == 91
+
+
+@gpu
+def test_prefill_refuses_layers_of_different_lengths():
+    """A state restored into some layers only: no position fits them all."""
+    m = Qwen3StyleDecoder(CFG, 2, 200, FT, seed=3)
+    m.prefill(prompt(2, 50))
+    other = type(m.layers[1]["cache"])(**FT)
+    other.update_and_fetch(*(torch.randn((2, 2, 40, 128), device="cuda").bfloat16() for _ in range(2)))
+    m.layers[1]["cache"].state = other.state
+    for call in (lambda: m.prefill(prompt(2, 5)), lambda: m.fill_context(5)):
+        with pytest.raises(RuntimeError, match="different lengths"):
+            call()
+    m.layers[0]["cache"].state = other.state
+    m.prefill(prompt(2, 5))
+    assert m.layers[0]["cache"].offset == m.layers[1]["cache"].offset == 45
